@@ -313,9 +313,9 @@ def run(state):
         return [out.detach(), *torch.autograd.grad(out, leaves, state["dout"])]
     if op == "append":
         ops.kv_cache_write(state["k"], state["v"], state["cache"], state["slots"])
-        return ops.kv_cache_read(state["cache"], state["table"], state["cu"], state["total"])
+        return ops.kv_cache_read(state["cache"], state["table"], state["cu"], state["total"], case["d"])
     if op == "read":
-        return ops.kv_cache_read(state["cache"], state["table"], state["cu"], state["total"])
+        return ops.kv_cache_read(state["cache"], state["table"], state["cu"], state["total"], case["d"])
     return ops.fmha_cache_fwd(state["q"], state["cache"], state["table"], state["lens"], state["cu_q"], case["new"],
                               state["longest"], state["scale"], 1, window, sinks=sinks)
 
