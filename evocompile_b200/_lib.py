@@ -97,6 +97,21 @@ SIGNATURES = {
         _int,
         [_int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _fl, _vp, _vp],
     ),
+    "gko_kv_cache_write": (
+        _int,
+        [_int, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
+         _vp],
+    ),
+    "gko_kv_cache_read": (
+        _int,
+        [_int, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "gko_fmha_cache_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int]),
+    "gko_fmha_cache_fwd": (
+        _int,
+        [_int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
+         _i64, _i64, _vp, _vp, _fl, _int, _int, _fl, _int, _vp, _vp, _vp, _i64, _vp, _vp],
+    ),
     "gko_set_gemm_ctas": (_int, [_int]),
     "gko_allreduce_residual_nvls": (_int, [_int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _fl, _vp, _vp]),
     "gko_swiglu_bwd": (_int, [_int, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),

@@ -1,0 +1,744 @@
+// Attention of a few new tokens per sequence over a paged 4-bit or 8-bit key / value cache
+// (gko_fmha_cache_fwd), written by gko_kv_cache_write.
+//
+// With K[j] = scale_k[j] c_j + zero_k[j] and V[j] = scale_v[j] e_j + zero_v[j] (c, e: codes):
+//   logit_ij = scale * (scale_k[j] (q_i . c_j) + zero_k[j] sum(q_i))
+//   out_i    = (sum_j (p_ij scale_v[j]) e_j + sum_j p_ij zero_v[j]) / sum_j p_ij
+// so the tensor cores multiply the codes themselves, exact in f16, and the pairs are applied in
+// f32 to the accumulators and probabilities. Nothing dequantised is ever stored.
+//
+// The cache is read once, so the kernel is bound by memory (d * bits / 8 + 4 bytes per row, 2
+// rows per token and kv head), and the work that unpacks 64 codes a clock per SM has to hide
+// behind it. Products run on m16n8k16 (mma.sync) with the codes as the 16-row operand and the
+// query heads of one kv head as the 8-column operand: S^T = K q^T and O^T = V^T P^T. The cache
+// rows come straight from memory in the operand's register layout, and a query group of 8 fills
+// the columns; tcgen05 would want the unpacked codes in shared memory and 128 rows of queries.
+//
+// Columns of a CTA are (new token, query head) pairs of one kv head, kCols at a time. A CTA takes
+// one range of keys (grid.x: column tile, then split); its warps take slabs of 32 keys in turn,
+// each with its own running maximum, sum and accumulators, and join at the end in a fixed order.
+// With more than one split the joined parts go to the workspace and a second kernel adds them,
+// again in a fixed order, so results do not vary from run to run.
+#include "host_common.h"
+#include "sm100_ptx.cuh"
+
+namespace gko {
+namespace fmha_cache {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kSlab = 32;            // keys a warp takes at a time
+constexpr int kMaxSplitSlabs = 64;   // at most 2048 keys per split, so that one long sequence spreads
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRescale = 8.f;      // log2: the running maximum moves only when it grows by more
+
+struct Params {
+  int b, hq, hkv, group, max_q;
+  int64_t tq;
+  const void* q;
+  int64_t q_st, q_sh;
+  const uint8_t* k_codes;
+  const uint8_t* v_codes;
+  const uint32_t* k_pairs;
+  const uint32_t* v_pairs;
+  int64_t pages;
+  int page_size;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_width;
+  const int32_t* lens;
+  const int32_t* cu_q;  // NULL: one new token per sequence
+  float scale, softcap;
+  int causal, window, sinks;
+  int tiles, splits, split_slabs;
+  void* out;
+  float* lse;
+  float* part_o;   // [splits][tq * hq][d]
+  float2* part_ml;  // [splits][tq * hq] (maximum in log2 units, sum)
+  unsigned* status;
+};
+
+// The query rows of sequence b and its cached length; whatever the arrays hold, no row leaves [0, tq).
+struct Seq {
+  int row0, n, len;
+};
+__device__ __forceinline__ Seq sequence(const Params& p, int b) {
+  Seq s;
+  if (p.cu_q) {
+    const int64_t a = min(max((int64_t)p.cu_q[b], (int64_t)0), p.tq);
+    const int64_t e = min(max((int64_t)p.cu_q[b + 1], a), p.tq);
+    s.row0 = (int)a;
+    s.n = (int)(e - a);
+  } else {
+    s.row0 = b;
+    s.n = b < p.tq ? 1 : 0;
+  }
+  const int64_t cap = (int64_t)p.table_width * p.page_size;
+  const int64_t len = p.lens[b];
+  s.len = (int)min(max(len, (int64_t)0), cap);
+  if (len > cap && threadIdx.x == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
+  return s;
+}
+
+// Slabs of 32 keys that the columns [c0, c0 + cols) of a sequence may see: [0, first) hold sinks,
+// then those of [lo, hi). Slab number v of the range stands for slab v < first ? v : lo + v - first.
+struct Range {
+  int first, lo, count;
+};
+__device__ __forceinline__ Range key_range(const Params& p, const Seq& s, int c0, int c1) {
+  const int pos_min = s.len - s.n + c0 / p.group, pos_max = s.len - s.n + (c1 - 1) / p.group;
+  int hi = s.len, lo = 0, sink = 0;
+  if (p.causal) hi = min(hi, pos_max + 1);
+  if (p.window > 0) {
+    sink = min(p.sinks, hi);
+    lo = max(0, pos_min - p.window);
+    hi = (int)min((int64_t)hi, (int64_t)pos_max + p.window + 1);
+  }
+  Range r;
+  r.first = sink > 0 ? (sink + kSlab - 1) / kSlab : 0;
+  r.lo = max(lo / kSlab, r.first);
+  const int end = hi > 0 ? (hi + kSlab - 1) / kSlab : 0;
+  r.count = r.first + max(0, end - r.lo);
+  return r;
+}
+
+// -------------------------------------------------------------- fragments
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
+                            *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Integers as f16: 0x6400 | u is 1024 + u, and a nibble four bits higher adds 16 u.
+constexpr uint32_t kMinus1024 = 0xE400E400u;  // f16 (-1024, -1024)
+constexpr uint32_t kSixteenth = 0x2C002C00u;  // f16 (1/16, 1/16)
+constexpr uint32_t kMinus64 = 0xD400D400u;    // f16 (-64, -64)
+
+// A word of 16-bit halves with four nibbles each -> four f16 pairs, (low half, high half) of
+// nibble 0, 1, 2, 3.
+__device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&f)[4]) {
+  const uint32_t s = w >> 8;
+  f[0] = h2_add((w & 0x000F000Fu) | 0x64006400u, kMinus1024);
+  f[1] = h2_fma((w & 0x00F000F0u) | 0x64006400u, kSixteenth, kMinus64);
+  f[2] = h2_add((s & 0x000F000Fu) | 0x64006400u, kMinus1024);
+  f[3] = h2_fma((s & 0x00F000F0u) | 0x64006400u, kSixteenth, kMinus64);
+}
+// Bytes 0, 1 and bytes 2, 3 of a word -> two f16 pairs.
+__device__ __forceinline__ uint32_t bytes01(uint32_t w) {
+  return h2_add(__byte_perm(w, 0x64646464u, 0x4140), kMinus1024);
+}
+__device__ __forceinline__ uint32_t bytes23(uint32_t w) {
+  return h2_add(__byte_perm(w, 0x64646464u, 0x4342), kMinus1024);
+}
+
+// N consecutive 32-bit words, as the widest loads that fit.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* src, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(src);
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(src);
+    w[0] = x.x;
+    w[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 x = reinterpret_cast<const uint4*>(src)[i];
+      w[4 * i] = x.x;
+      w[4 * i + 1] = x.y;
+      w[4 * i + 2] = x.z;
+      w[4 * i + 3] = x.w;
+    }
+  }
+}
+
+template <int D, int BITS>
+struct Row {
+  static constexpr int kBytes = D * BITS / 8;
+  static constexpr int kKWords = kBytes / 16;  // a lane's share of a key row: a quarter, D / 4 channels
+  static constexpr int kVWords = kBytes / 32;  // a lane's share of a value row: an eighth, D / 8 channels
+  static constexpr int kSteps = D / 16;        // m16n8k16 steps over the channels of S; m-tiles of O
+};
+
+// Channel (0 .. D/4 - 1, within the lane's share) of element e (0, 1: low / high half) of pair
+// `pr` (0, 1) of step s of S: the order in which the unpacking above meets a row's codes.
+template <int BITS>
+__device__ __forceinline__ int k_channel(int s, int pr, int e) {
+  if (BITS == 4) return (s >> 1) * 8 + (s & 1) * 2 + pr + 4 * e;
+  return s * 4 + pr * 2 + e;
+}
+
+// -------------------------------------------------------------- main kernel
+template <typename T, int D, int BITS, int NT>
+__global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
+  using R = Row<D, BITS>;
+  constexpr int kCols = 8 * NT;
+  constexpr int kPitch = D + 4;  // accumulators of one column in shared memory, padded against conflicts
+  __shared__ __align__(16) __half q_s[kCols][D + 8];
+  __shared__ float q_mul[kCols], q_sum[kCols];
+  __shared__ int q_pos[kCols];
+  __shared__ float w_max[kWarps][kCols], w_sum[kWarps][kCols], w_zero[kWarps][kCols];
+  __shared__ __align__(16) float o_s[kCols][kPitch];
+
+  const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const Seq sq = sequence(p, b);
+  const int c0 = tile * kCols;
+  const int c1 = min(c0 + kCols, sq.n * p.group);
+  if (c0 >= c1) return;
+  const Range rg = key_range(p, sq, c0, c1);
+  const int v0 = split * p.split_slabs;
+  // the last split takes whatever is left, should a sequence be longer than the caller's bound
+  const int v1 = split == p.splits - 1 ? rg.count : min(rg.count, v0 + p.split_slabs);
+  if (v0 >= v1 && split > 0) return;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int li = lane & 3, lj = lane >> 2;
+
+  // queries as f16, each column divided by the power of two below its largest value (exact, and
+  // within range for bf16 queries of any size), with the factor to undo it and the sum over d
+  for (int c = warp; c < kCols; c += kWarps) {
+    const int col = c0 + c;
+    const bool in = col < c1;
+    const int tok = in ? col / p.group : 0;
+    const int head = hk * p.group + (in ? col % p.group : 0);
+    constexpr int kPer = D / 32;
+    float x[kPer];
+    float big = 0.f;
+    const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(sq.row0 + tok) * p.q_st + (int64_t)head * p.q_sh +
+                   lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      x[i] = in ? Cvt<T>::to_f32(src[i]) : 0.f;
+      big = fmaxf(big, fabsf(x[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    // exponent kept in [-100, 100] so that both factors are normal numbers
+    int e = (big > 0.f && big < INFINITY) ? (int)((__float_as_uint(big) >> 23) & 255u) - 127 : 0;
+    e = min(max(e, -100), 100);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      x[i] *= down;
+      sum += x[i];
+      q_s[c][lane * kPer + i] = __float2half_rn(x[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      q_mul[c] = up * p.scale * (p.softcap > 0.f ? 1.f : kLog2e);
+      q_sum[c] = sum;
+      q_pos[c] = sq.len - sq.n + tok;
+    }
+  }
+  __syncthreads();
+
+  // query fragments (B operand: rows are channels, columns are queries)
+  uint32_t qf[NT][R::kSteps][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int s = 0; s < R::kSteps; ++s)
+#pragma unroll
+      for (int pr = 0; pr < 2; ++pr) {
+        const __half* row = q_s[n * 8 + lj] + li * (D / 4);
+        const __half2 h = __halves2half2(row[k_channel<BITS>(s, pr, 0)], row[k_channel<BITS>(s, pr, 1)]);
+        qf[n][s][pr] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+  float mul[NT][2], qsum[NT][2];
+  int pos[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int c = n * 8 + li * 2 + e;
+      mul[n][e] = q_mul[c];
+      qsum[n][e] = q_sum[c];
+      pos[n][e] = q_pos[c];
+    }
+  const int pos_min = sq.len - sq.n + c0 / p.group, pos_max = sq.len - sq.n + (c1 - 1) / p.group;
+
+  float o[R::kSteps][NT][4];
+  float m[NT][2], l[NT][2], z[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[n][e] = -INFINITY;
+      l[n][e] = z[n][e] = 0.f;
+    }
+#pragma unroll
+    for (int s = 0; s < R::kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[s][n][e] = 0.f;
+  }
+  // value scales are divided by the power of two above the largest so far, kept in `vexp` as the
+  // exponent bits of a float, so that p * scale_v fits f16 whatever the size of the values
+  uint32_t vexp = 0x00800000u;
+
+  const int32_t* table = p.table + (int64_t)b * p.table_stride;
+  const int64_t head_row = (int64_t)hk * p.page_size;
+  for (int v = v0 + warp; v < v1; v += kWarps) {
+    const int t0 = (v < rg.first ? v : rg.lo + v - rg.first) * kSlab;
+    // rows of the two 16-key halves of the slab (a page holds a multiple of 16)
+    int64_t row[2];
+    bool have[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int t = t0 + 16 * hf;
+      const int col = t / p.page_size;
+      const int page = t < sq.len && col < p.table_width ? table[col] : -1;
+      have[hf] = page >= 0 && page < p.pages;
+      if (t < sq.len && !have[hf] && lane == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
+      row[hf] = have[hf] ? ((int64_t)page * p.hkv) * p.page_size + head_row + t % p.page_size : 0;
+    }
+    float s[2][NT][4];
+    float vs[2][2], vz[2][2];
+    uint32_t vs_max = 0;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[hf][n][e] = 0.f;
+      uint32_t w[2][R::kKWords];
+      float ks[2] = {0.f, 0.f}, kz[2] = {0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int t = t0 + 16 * hf + 8 * r + lj;
+        const int64_t at = row[hf] + 8 * r + lj;
+        vs[hf][r] = vz[hf][r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < R::kKWords; ++i) w[r][i] = 0;
+        if (have[hf]) {
+          load_words<R::kKWords>(p.k_codes + at * R::kBytes + li * (R::kBytes / 4), w[r]);
+          if (t < sq.len) {
+            Cvt<T>::unpack(p.k_pairs[at], ks[r], kz[r]);
+            Cvt<T>::unpack(p.v_pairs[at], vs[hf][r], vz[hf][r]);
+          }
+        }
+        vs_max = max(vs_max, __float_as_uint(vs[hf][r]));
+      }
+      // S^T += K q^T
+#pragma unroll
+      for (int i = 0; i < R::kKWords; ++i) {
+        if constexpr (BITS == 4) {
+          uint32_t f0[4], f1[4];
+          nibbles(w[0][i], f0);
+          nibbles(w[1][i], f1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816(s[hf][n], f0[0], f1[0], f0[1], f1[1], qf[n][2 * i][0], qf[n][2 * i][1]);
+            mma16816(s[hf][n], f0[2], f1[2], f0[3], f1[3], qf[n][2 * i + 1][0], qf[n][2 * i + 1][1]);
+          }
+        } else {
+          const uint32_t a0 = bytes01(w[0][i]), a1 = bytes01(w[1][i]), a2 = bytes23(w[0][i]), a3 = bytes23(w[1][i]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(s[hf][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+        }
+      }
+      // logits in log2 units, masks
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int t = t0 + 16 * hf + 8 * r + lj;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaf(kz[r], qsum[n][e], ks[r] * s[hf][n][2 * r + e]) * mul[n][e];
+            if (p.softcap > 0.f) x = p.softcap * kLog2e * tanhf(x / p.softcap);
+            s[hf][n][2 * r + e] = x;
+          }
+        const bool edge = !have[hf] || t0 + kSlab > sq.len || (p.causal && t0 + kSlab - 1 > pos_min) ||
+                          (p.window > 0 && t0 + kSlab > p.sinks &&
+                           (t0 < pos_max - p.window || t0 + kSlab - 1 > pos_min + p.window));
+        if (edge) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              bool keep = have[hf] && t < sq.len && (!p.causal || t <= pos[n][e]);
+              if (p.window > 0) keep = keep && (abs(t - pos[n][e]) <= p.window || t < p.sinks);
+              if (!keep) s[hf][n][2 * r + e] = -INFINITY;
+            }
+        }
+      }
+    }
+    // running maximum per column and the exponent of the value scales; both move rarely
+    bool grow = false;
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[n][e] = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
+        grow |= top[n][e] > m[n][e] + kRescale;
+      }
+    vs_max = (__reduce_max_sync(0xffffffffu, vs_max) & 0x7f800000u) + 0x00800000u;
+    if (vs_max > vexp || __any_sync(0xffffffffu, grow)) {
+      // 2^(old exponent - new exponent): 0 when nothing was accumulated yet
+      const uint32_t vnew = max(vexp, vs_max);
+      const float vscale = __uint_as_float(vexp) / __uint_as_float(vnew);
+      vexp = vnew;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = top[n][e];
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, sh));
+          const float mn = x > m[n][e] + kRescale ? x : m[n][e];
+          const float alpha = m[n][e] == mn ? 1.f : fast_exp2(m[n][e] - mn);
+          m[n][e] = mn;
+          l[n][e] *= alpha;
+          z[n][e] *= alpha;
+#pragma unroll
+          for (int st = 0; st < R::kSteps; ++st) {
+            o[st][n][e] *= alpha * vscale;
+            o[st][n][2 + e] *= alpha * vscale;
+          }
+        }
+    }
+    const float vdown = __uint_as_float(0x7f000000u - vexp);  // 1 / 2^(exponent of vexp)
+    // probabilities, sums, and P^T as the B operand (rows are keys, columns are queries)
+    uint32_t pf[2][NT][2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float sv = vs[hf][r] * vdown;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float pv[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mm = m[n][e] == -INFINITY ? 0.f : m[n][e];
+            const float x = fast_exp2(s[hf][n][2 * r + e] - mm);
+            l[n][e] += x;
+            z[n][e] += x > 0.f ? x * vz[hf][r] : 0.f;
+            pv[e] = x * sv;
+          }
+          pf[hf][n][r] = transpose8x8(Cvt<__half>::pack(pv[0], pv[1]));
+        }
+      }
+    // O^T += V^T P^T
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      uint32_t w[4][R::kVWords];  // keys 2i, 2i + 1, 2i + 8, 2i + 9
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int i = 0; i < R::kVWords; ++i) w[r][i] = 0;
+        if (have[hf])
+          load_words<R::kVWords>(p.v_codes + (row[hf] + 2 * li + (r & 1) + 8 * (r >> 1)) * R::kBytes +
+                                     lj * (R::kBytes / 8), w[r]);
+      }
+#pragma unroll
+      for (int i = 0; i < R::kVWords; ++i) {
+        if constexpr (BITS == 4) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // channels 4 h .. 4 h + 3 of the word
+            uint32_t f0[4], f1[4];
+            nibbles(__byte_perm(w[0][i], w[1][i], h ? 0x7632 : 0x5410), f0);
+            nibbles(__byte_perm(w[2][i], w[3][i], h ? 0x7632 : 0x5410), f1);
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                mma16816(o[4 * i + 2 * h + mt][n], f0[2 * mt], f0[2 * mt + 1], f1[2 * mt], f1[2 * mt + 1],
+                         pf[hf][n][0], pf[hf][n][1]);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // channels 2 h, 2 h + 1 of the word
+            const uint32_t x = __byte_perm(w[0][i], w[1][i], h ? 0x7362 : 0x5140);
+            const uint32_t y = __byte_perm(w[2][i], w[3][i], h ? 0x7362 : 0x5140);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma16816(o[2 * i + h][n], bytes01(x), bytes23(x), bytes01(y), bytes23(y), pf[hf][n][0], pf[hf][n][1]);
+          }
+        }
+      }
+    }
+  }
+
+  // join the warps: sums over the lanes of a column, a common maximum, then warp after warp
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int sh = 4; sh < 32; sh <<= 1) {
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], sh);
+        z[n][e] += __shfl_xor_sync(0xffffffffu, z[n][e], sh);
+      }
+      if (lj == 0) {
+        w_max[warp][n * 8 + li * 2 + e] = m[n][e];
+        w_sum[warp][n * 8 + li * 2 + e] = l[n][e];
+        w_zero[warp][n * 8 + li * 2 + e] = z[n][e];
+      }
+    }
+  __syncthreads();
+  float f[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][n * 8 + li * 2 + e]);
+      f[n][e] = m[n][e] == -INFINITY ? 0.f : fast_exp2(m[n][e] - mx) * __uint_as_float(vexp);
+    }
+  for (int w = 0; w < kWarps; ++w) {
+    if (warp == w) {
+#pragma unroll
+      for (int st = 0; st < R::kSteps; ++st)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float* at = &o_s[n * 8 + li * 2 + (x & 1)][lj * (D / 8) + 2 * st + (x >> 1)];
+            const float val = o[st][n][x] * f[n][x & 1];
+            *at = w == 0 ? val : *at + val;
+          }
+    }
+    __syncthreads();
+  }
+  for (int c = warp; c < c1 - c0; c += kWarps) {
+    const int col = c0 + c, tok = col / p.group, head = hk * p.group + col % p.group;
+    float mx = -INFINITY, sum = 0.f, zero = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][c]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float a = w_max[w][c] == -INFINITY ? 0.f : fast_exp2(w_max[w][c] - mx);
+      sum += w_sum[w][c] * a;
+      zero += w_zero[w][c] * a;
+    }
+    constexpr int kPer = D / 32;
+    const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head;
+    if (p.splits > 1) {
+      float* dst = p.part_o + ((int64_t)split * p.tq * p.hq + r) * D;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) dst[lane + 32 * i] = o_s[c][lane + 32 * i] + zero;
+      if (lane == 0) p.part_ml[(int64_t)split * p.tq * p.hq + r] = make_float2(mx, sum);
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays
+      T* dst = reinterpret_cast<T*>(p.out) + r * D;
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i)
+        reinterpret_cast<uint32_t*>(dst)[lane + 32 * i] = Cvt<T>::pack(
+            (o_s[c][2 * (lane + 32 * i)] + zero) * inv, (o_s[c][2 * (lane + 32 * i) + 1] + zero) * inv);
+      if (lane == 0)
+        p.lse[(int64_t)head * p.tq + sq.row0 + tok] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+    }
+  }
+}
+
+// -------------------------------------------------------------- join the splits: one warp per (query, head)
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) fmha_cache_join_kernel(const Params p, int cols) {
+  const int hk = blockIdx.y, b = blockIdx.z;
+  const Seq sq = sequence(p, b);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = blockIdx.x * kWarps + warp;
+  if (col >= sq.n * p.group) return;
+  const int c0 = col / cols * cols, c1 = min(c0 + cols, sq.n * p.group);
+  const Range rg = key_range(p, sq, c0, c1);
+  const int used = min(max(1, (rg.count + p.split_slabs - 1) / p.split_slabs), p.splits);
+  const int tok = col / p.group, head = hk * p.group + col % p.group;
+  const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head, stride = p.tq * p.hq;
+  float mx = -INFINITY;
+  for (int s = 0; s < used; ++s) mx = fmaxf(mx, p.part_ml[s * stride + r].x);
+  constexpr int kPer = D / 32;
+  float acc[kPer], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+  for (int s = 0; s < used; ++s) {
+    const float2 ml = p.part_ml[s * stride + r];
+    const float a = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
+    sum += ml.y * a;
+    const float* src = p.part_o + (s * stride + r) * D + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(src[i], a, acc[i]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* dst = reinterpret_cast<T*>(p.out) + r * D + lane * kPer;
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i)
+    reinterpret_cast<uint32_t*>(dst)[i] = Cvt<T>::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  if (lane == 0) p.lse[(int64_t)head * p.tq + sq.row0 + tok] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+}
+
+// -------------------------------------------------------------- host side
+struct Plan {
+  int cols, tiles, splits, split_slabs;
+};
+
+// Columns per CTA, column tiles and key splits. Splits fill four CTAs on every SM, with at least
+// a slab for each warp and at most kMaxSplitSlabs slabs each.
+Plan plan(int64_t b, int64_t hkv, int64_t group, int64_t max_q, int64_t max_k, int window, int sinks) {
+  Plan pl;
+  const int64_t columns = max_q * group;
+  pl.cols = columns <= 8 ? 8 : 16;
+  pl.tiles = (int)((columns + pl.cols - 1) / pl.cols);
+  int64_t keys = max_k;
+  if (window > 0) {
+    const int64_t span = 2 * (int64_t)window + max_q + (int64_t)sinks + 3 * kSlab;
+    if (span < keys) keys = span;
+  }
+  const int64_t slabs = (keys + kSlab - 1) / kSlab > 0 ? (keys + kSlab - 1) / kSlab : 1;
+  const int64_t ctas = b * hkv * pl.tiles, slots = 4 * (int64_t)host::sm_count();
+  int64_t want = (slots + ctas - 1) / ctas;
+  int64_t per = (slabs + want - 1) / want;
+  if (per < kWarps) per = kWarps;
+  if (per > kMaxSplitSlabs) per = kMaxSplitSlabs;
+  pl.split_slabs = (int)per;
+  pl.splits = (int)((slabs + per - 1) / per);
+  return pl;
+}
+
+template <typename T, int D, int BITS>
+int launch(const Params& p, const Plan& pl, cudaStream_t s) {
+  const dim3 grid((unsigned)(pl.tiles * pl.splits), (unsigned)p.hkv, (unsigned)p.b);
+  if (pl.cols == 8) fmha_cache_kernel<T, D, BITS, 1><<<grid, kThreads, 0, s>>>(p);
+  else fmha_cache_kernel<T, D, BITS, 2><<<grid, kThreads, 0, s>>>(p);
+  int rc = host::cuda_check(cudaGetLastError(), "fmha cache kernel launch");
+  if (rc || pl.splits == 1) return rc;
+  const int64_t columns = (int64_t)p.max_q * p.group;
+  const dim3 jgrid((unsigned)((columns + kWarps - 1) / kWarps), (unsigned)p.hkv, (unsigned)p.b);
+  fmha_cache_join_kernel<T, D><<<jgrid, kThreads, 0, s>>>(p, pl.cols);
+  return host::cuda_check(cudaGetLastError(), "fmha cache join launch");
+}
+
+template <typename T>
+int dispatch(int d, int bits, const Params& p, const Plan& pl, cudaStream_t s) {
+  if (d == 64) return bits == 4 ? launch<T, 64, 4>(p, pl, s) : launch<T, 64, 8>(p, pl, s);
+  return bits == 4 ? launch<T, 128, 4>(p, pl, s) : launch<T, 128, 8>(p, pl, s);
+}
+
+int check_sizes(int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq, int64_t max_q, int64_t max_k, int window,
+                int sinks) {
+  using host::fail;
+  if (d != 64 && d != 128)
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache supports head dim 64 or 128, got %lld", (long long)d);
+  if (hq <= 0 || hkv <= 0 || hq % hkv)
+    return fail(GKO_ERR_INVALID, "query heads (%lld) must be a positive multiple of kv heads (%lld)", (long long)hq,
+                (long long)hkv);
+  if (b < 0 || tq < 0 || max_q < 0 || max_k < 0 || window < 0 || sinks < 0)
+    return fail(GKO_ERR_INVALID, "fmha over a cache: negative size, window or sinks");
+  if (b > 65535 || hkv > 65535 || tq * hq >= (1ll << 31) || max_q * (hq / hkv) >= (1 << 24) || max_k > (1 << 30) ||
+      window > (1 << 30) || sinks > (1 << 30))
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: sizes out of range");
+  return GKO_OK;
+}
+
+}  // namespace fmha_cache
+}  // namespace gko
+
+using namespace gko;
+using gko::host::fail;
+
+extern "C" int64_t gko_fmha_cache_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+                                                 int64_t max_seqlen_q, int64_t max_seqlen_k, int window, int sinks) {
+  if (fmha_cache::check_sizes(b, hq, hkv, d, tq, max_seqlen_q, max_seqlen_k, window, sinks)) return -1;
+  if (b == 0 || tq == 0 || max_seqlen_q == 0) return 0;
+  const fmha_cache::Plan pl = fmha_cache::plan(b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
+  return pl.splits > 1 ? pl.splits * tq * hq * (d * 4 + 8) : 0;
+}
+
+extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+                                  int64_t max_seqlen_q, int64_t max_seqlen_k, const void* q, int64_t q_st,
+                                  int64_t q_sh, const void* k_codes, const void* v_codes, const void* k_pairs,
+                                  const void* v_pairs, int64_t pages, int64_t page_size, const int32_t* table,
+                                  int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
+                                  const int32_t* cu_seqlens_q, float scale, int causal, int window, float softcap,
+                                  int sinks, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                  unsigned int* status, void* stream) {
+  if (dtype != GKO_F16 && dtype != GKO_BF16)
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache supports float16 and bfloat16 only (dtype code %d)", dtype);
+  if (bits != 4 && bits != 8)
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: codes have 4 or 8 bits, got %d", bits);
+  int rc = fmha_cache::check_sizes(b, hq, hkv, d, tq, max_seqlen_q, max_seqlen_k, window, sinks);
+  if (rc) return rc;
+  if (!(softcap >= 0.f)) return fail(GKO_ERR_INVALID, "softcap must be >= 0");
+  if (!(scale == scale)) return fail(GKO_ERR_INVALID, "scale is NaN");
+  if (page_size <= 0 || page_size % 16 || page_size > (1 << 20))
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: the page size must be a multiple of 16 up to 2^20, got %lld",
+                (long long)page_size);
+  if (pages < 0 || table_width < 0 || table_stride < 0) return fail(GKO_ERR_INVALID, "fmha over a cache: bad sizes");
+  if (table_width * page_size >= (1ll << 31) || pages >= (1ll << 31))
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: a sequence may hold fewer than 2^31 tokens");
+  if (b == 0 || tq == 0 || max_seqlen_q == 0) return GKO_OK;
+  if (!q || !k_codes || !v_codes || !k_pairs || !v_pairs || !table || !seq_lens || !out || !lse)
+    return fail(GKO_ERR_INVALID, "fmha over a cache: null pointer argument");
+  const void* ptrs[5] = {k_codes, v_codes, k_pairs, v_pairs, out};
+  for (const void* x : ptrs)
+    if (!host::aligned16(x)) return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache needs 16-byte aligned tensors");
+  const fmha_cache::Plan pl =
+      fmha_cache::plan(b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
+  const int64_t need = pl.splits > 1 ? pl.splits * tq * hq * (d * 4 + 8) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need || !host::aligned16(workspace)))
+    return fail(GKO_ERR_INVALID, "fmha over a cache needs a 16-byte aligned workspace of %lld bytes (got %lld)",
+                (long long)need, (long long)workspace_bytes);
+  if ((int64_t)pl.tiles * pl.splits >= (1ll << 31))
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: sizes out of range");
+  fmha_cache::Params p{};
+  p.b = (int)b;
+  p.hq = (int)hq;
+  p.hkv = (int)hkv;
+  p.group = (int)(hq / hkv);
+  p.max_q = (int)max_seqlen_q;
+  p.tq = tq;
+  p.q = q;
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.k_codes = static_cast<const uint8_t*>(k_codes);
+  p.v_codes = static_cast<const uint8_t*>(v_codes);
+  p.k_pairs = static_cast<const uint32_t*>(k_pairs);
+  p.v_pairs = static_cast<const uint32_t*>(v_pairs);
+  p.pages = pages;
+  p.page_size = (int)page_size;
+  p.table = table;
+  p.table_stride = table_stride;
+  p.table_width = (int)table_width;
+  p.lens = seq_lens;
+  p.cu_q = cu_seqlens_q;
+  p.scale = scale;
+  p.softcap = softcap;
+  p.causal = causal ? 1 : 0;
+  p.window = window;
+  p.sinks = window > 0 ? sinks : 0;
+  p.tiles = pl.tiles;
+  p.splits = pl.splits;
+  p.split_slabs = pl.split_slabs;
+  p.out = out;
+  p.lse = lse;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + (int64_t)pl.splits * tq * hq * d);
+  p.status = status;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == GKO_BF16 ? fmha_cache::dispatch<__nv_bfloat16>((int)d, bits, p, pl, s)
+                           : fmha_cache::dispatch<__half>((int)d, bits, p, pl, s);
+}

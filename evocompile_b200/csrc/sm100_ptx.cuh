@@ -22,6 +22,7 @@ enum : unsigned {
   kStatusTimeoutEpilogue = 1u << 2,
   kStatusTimeoutSoftmax = 1u << 3,
   kStatusTimeoutDrain = 1u << 4,
+  kStatusBadIndex = 1u << 5,  // a page, slot or length outside its table: the access was skipped
 };
 
 // A single wait never legitimately lasts this long; see wait_bounded.

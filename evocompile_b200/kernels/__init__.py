@@ -40,6 +40,11 @@ KERNELS: dict[str, dict] = {
         "match": "silu(x) * y split across two kernels (SwiGLU / SE)",
         "note": "one vectorised HBM-bound kernel.",
     },
+    "kv_cache": {
+        "module": __name__ + ".kv_cache",
+        "match": "called by name: a decoder's paged key / value cache",
+        "note": "4- or 8-bit paged cache: quantised write, read back, attention of new tokens over the codes.",
+    },
 }
 
 _installed: set[str] = set()

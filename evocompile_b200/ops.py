@@ -9,6 +9,7 @@ them falls back to another implementation.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -552,6 +553,195 @@ def fmha_varlen_bwd(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seq
             )
         _lib.check(rc, "gko_fmha_varlen_bwd")
     return dq, dk, dv
+
+
+# --------------------------------------------------------------------------- paged cache in 4 or 8 bits
+class KVCache(NamedTuple):
+    """A paged, quantised key / value cache: what ``kv_cache_write`` fills and ``kv_cache_read`` and
+    ``fmha_cache_fwd`` read (any tuple of four such tensors does).
+
+    codes uint8 [pages, kv heads, page size, d * bits / 8] (4 bits: channel 2i in the low half of byte
+    i) and (scale, zero) pairs [pages, kv heads, page size, 2] in the element type: a code c stands
+    for c * scale + zero.
+    """
+
+    k_codes: torch.Tensor
+    v_codes: torch.Tensor
+    k_pairs: torch.Tensor
+    v_pairs: torch.Tensor
+
+
+def kv_cache_alloc(pages, page_size, kv_heads, head_dim, bits=4, dtype=torch.bfloat16, device="cuda") -> KVCache:
+    """A zeroed cache of ``pages`` pages of ``page_size`` tokens (a multiple of 16) with 4- or 8-bit codes."""
+    if bits not in (4, 8):
+        raise RuntimeError(f"kv_cache_alloc: codes have 4 or 8 bits, got {bits}")
+    if head_dim not in (64, 128):
+        raise RuntimeError(f"kv_cache_alloc: head dim 64 or 128, got {head_dim}")
+    if page_size <= 0 or page_size % 16:
+        raise RuntimeError(f"kv_cache_alloc: the page size must be a multiple of 16, got {page_size}")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f"kv_cache_alloc: float16 or bfloat16, got {dtype}")
+    codes = lambda: torch.zeros(pages, kv_heads, page_size, head_dim * bits // 8, dtype=torch.uint8, device=device)  # noqa: E731
+    pairs = lambda: torch.zeros(pages, kv_heads, page_size, 2, dtype=dtype, device=device)  # noqa: E731
+    return KVCache(codes(), codes(), pairs(), pairs())
+
+
+def _cache_layout(name, cache, hkv=None, d=None, dtype=None):
+    """(dtype code, bits, kv heads, d) of a cache whose four tensors fit together and, where given, k and v."""
+    if len(cache) != 4:
+        raise RuntimeError(f"{name}: a cache is (k_codes, v_codes, k_pairs, v_pairs)")
+    kc, vc, kp, vp = cache
+    if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or kc.dim() != 4 or kc.shape != vc.shape:
+        raise RuntimeError(f"{name}: codes must be two uint8 [pages, kv heads, page, bytes] tensors of one shape")
+    if kp.shape != (*kc.shape[:3], 2) or vp.shape != kp.shape or kp.dtype != vp.dtype:
+        raise RuntimeError(f"{name}: pairs must be two [pages, kv heads, page, 2] tensors of one type")
+    if not (kc.is_contiguous() and vc.is_contiguous() and kp.is_contiguous() and vp.is_contiguous()):
+        raise RuntimeError(f"{name}: the cache's tensors must be contiguous")
+    if dtype is not None and kp.dtype != dtype:
+        raise RuntimeError(f"{name}: the cache holds {kp.dtype}, got {dtype}")
+    if hkv is not None and kc.shape[1] != hkv:
+        raise RuntimeError(f"{name}: the cache has {kc.shape[1]} kv heads, got {hkv}")
+    return _lib.dtype_code(kp.dtype)
+
+
+def _cache_bits(name, row_bytes, d):
+    if row_bytes * 2 == d:
+        return 4
+    if row_bytes == d:
+        return 8
+    raise RuntimeError(f"{name}: rows of {row_bytes} bytes hold neither 4- nor 8-bit codes of head dim {d}")
+
+
+def kv_cache_write(k, v, cache, slots):
+    """Quantise new keys and values into their slots of a paged cache, in place.
+
+    k, v [tokens, kv heads, d] in the cache's element type, any token and head strides with unit
+    stride along d; slots int64 [tokens] = page * page_size + place in the page. A negative slot skips
+    its token (padding); a slot past the cache skips it and sets a bit of the device status word
+    (``_lib.read_status``). The slots of one call must be distinct.
+    """
+    kc, vc, kp, vp = cache
+    dev = _lib.require_cuda(k, v, kc, vc, kp, vp, slots)
+    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
+        raise RuntimeError("kv_cache_write: k and v must be two [tokens, kv heads, d] tensors of one type")
+    t, hkv, d = k.shape
+    dt = _cache_layout("kv_cache_write", cache, hkv, d, k.dtype)
+    bits = _cache_bits("kv_cache_write", kc.shape[3], d)
+    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != t:
+        raise RuntimeError(f"kv_cache_write: slots must be int64 [{t}], got {slots.dtype} {tuple(slots.shape)}")
+    k, v = _bwd_fix(k), _bwd_fix(v)
+    slots = slots.contiguous()
+    with torch.cuda.device(dev):
+        rc = _lib.load().gko_kv_cache_write(
+            dt, bits, t, hkv, d, _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(slots),
+            _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), kc.shape[0], kc.shape[2], _status_ptr(dev), _stream(dev),
+        )
+    _lib.check(rc, "gko_kv_cache_write")
+
+
+def _check_table(name, block_table, b, what):
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b:
+        raise RuntimeError(f"{name}: block_table must be int32 [{b}, columns] for {what}, got "
+                           f"{block_table.dtype} {tuple(block_table.shape)}")
+    return block_table if block_table.stride(1) == 1 or block_table.shape[1] == 0 else block_table.contiguous()
+
+
+def kv_cache_read(cache, block_table, cu_seqlens, tokens, head_dim, out=None):
+    """Read cached sequences back -> (k, v), each [tokens, kv heads, head_dim] in the cache's element type.
+
+    Sequence s holds cu_seqlens[s + 1] - cu_seqlens[s] tokens (int32 [b + 1] on the device, from 0) and
+    goes to those rows, ready for ``fmha_varlen_fwd``; its token i is at place i % page_size of page
+    block_table[s, i // page_size] (int32 [b, columns]). ``tokens`` is the number of rows of k and v;
+    rows behind the last sequence are not written (``out``, a (k, v) pair of contiguous tensors, keeps
+    what it had there).
+    """
+    kc, vc, kp, vp = cache
+    dev = _lib.require_cuda(kc, vc, kp, vp, block_table, cu_seqlens, *(out or ()))
+    dt = _cache_layout("kv_cache_read", cache)
+    pages, hkv, page_size, row = kc.shape
+    d = int(head_dim)
+    bits = _cache_bits("kv_cache_read", row, d)
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise RuntimeError("kv_cache_read: cu_seqlens must be int32 [b + 1]")
+    b = cu_seqlens.shape[0] - 1
+    block_table = _check_table("kv_cache_read", block_table, b, f"cu_seqlens of {b} sequences")
+    if out is None:
+        out = tuple(torch.empty((tokens, hkv, d), device=dev, dtype=kp.dtype) for _ in range(2))
+    for t in out:
+        if t.shape != (tokens, hkv, d) or t.dtype != kp.dtype or not t.is_contiguous():
+            raise RuntimeError(f"kv_cache_read: out must be two contiguous [{tokens}, {hkv}, {d}] {kp.dtype} tensors")
+    cu_seqlens = cu_seqlens.contiguous()
+    with torch.cuda.device(dev):
+        rc = _lib.load().gko_kv_cache_read(
+            dt, bits, b, hkv, d, tokens, _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), pages, page_size, _ptr(block_table),
+            block_table.stride(0), block_table.shape[1], _ptr(cu_seqlens), _ptr(out[0]), _ptr(out[1]),
+            _status_ptr(dev), _stream(dev),
+        )
+    _lib.check(rc, "gko_kv_cache_read")
+    return tuple(out)
+
+
+def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqlen_q=1, max_seqlen_k=None, scale=None,
+                   causal=1, window=0, softcap=0.0, sinks=0, out=None):
+    """Attention of new tokens over a paged, quantised cache -> (out [tq, hq, d], lse f32 [hq, tq]).
+
+    q [tq, hq, d] (any token and head strides, unit stride along d); sequence s owns query rows
+    [cu_seqlens_q[s], cu_seqlens_q[s + 1]) (int32 [b + 1]; None: row s alone), at most ``max_seqlen_q``
+    of them. Its seq_lens[s] (int32 [b]) cached tokens, the new ones included (write them first), are in
+    the pages block_table[s] (int32 [b, columns]); query i of n is at position seq_lens[s] - n + i.
+    causal keeps keys up to that position, window > 0 those within it, plus the first ``sinks`` keys.
+    ``max_seqlen_k`` (default: what the block table holds) sets how the work is split, not what is
+    read. Rows that see no key give zeros and -inf; rows of no sequence are not written (``out`` keeps
+    what it had). One call per cache step: repeated calls give the same bits.
+    """
+    kc, vc, kp, vp = cache
+    dev = _lib.require_cuda(q, kc, vc, kp, vp, block_table, seq_lens, cu_seqlens_q, out)
+    if q.dim() != 3:
+        raise RuntimeError("fmha_cache: q must be 3-D [tokens, heads, d]")
+    tq, hq, d = q.shape
+    dt = _cache_layout("fmha_cache", cache, None, None, q.dtype)
+    pages, hkv, page_size, row = kc.shape
+    bits = _cache_bits("fmha_cache", row, d)
+    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1:
+        raise RuntimeError("fmha_cache: seq_lens must be int32 [b]")
+    b = seq_lens.shape[0]
+    block_table = _check_table("fmha_cache", block_table, b, f"seq_lens of {b} sequences")
+    if cu_seqlens_q is None:
+        if tq != b or max_seqlen_q != 1:
+            raise RuntimeError(f"fmha_cache: without cu_seqlens_q there is one query row per sequence, got {tq} rows "
+                               f"for {b} sequences, max_seqlen_q {max_seqlen_q}")
+    else:
+        if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] != b + 1:
+            raise RuntimeError(f"fmha_cache: cu_seqlens_q must be int32 [{b + 1}]")
+        cu_seqlens_q = cu_seqlens_q.contiguous()
+    if scale is None:
+        scale = d ** -0.5
+    if max_seqlen_k is None:
+        max_seqlen_k = block_table.shape[1] * page_size
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty((tq, hq, d), device=dev, dtype=q.dtype)
+    elif out.shape != (tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
+        raise RuntimeError(f"fmha_cache: out must be a contiguous [{tq}, {hq}, {d}] {q.dtype} tensor")
+    lse = torch.empty((hq, tq), device=dev, dtype=torch.float32)
+    seq_lens = seq_lens.contiguous()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        ws_bytes = lib.gko_fmha_cache_workspace_size(b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k),
+                                                     int(window or 0), int(sinks or 0))
+        if ws_bytes < 0:
+            _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_cache_workspace_size")
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+        rc = lib.gko_fmha_cache_fwd(
+            dt, bits, b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k), _ptr(q), q.stride(0), q.stride(1),
+            _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), pages, page_size, _ptr(block_table), block_table.stride(0),
+            block_table.shape[1], _ptr(seq_lens), _ptr(cu_seqlens_q), float(scale), int(bool(causal)),
+            int(window or 0), float(softcap or 0.0), int(sinks or 0), _ptr(out), _ptr(lse), _ptr(ws), ws_bytes,
+            _status_ptr(dev), _stream(dev),
+        )
+    _lib.check(rc, "gko_fmha_cache_fwd")
+    return out, lse
 
 
 # --------------------------------------------------------------------------- tensor-parallel GEMM + all-reduce

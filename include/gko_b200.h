@@ -52,6 +52,7 @@ extern "C" {
 #define GKO_STATUS_TIMEOUT_EPILOGUE 0x4u
 #define GKO_STATUS_TIMEOUT_SOFTMAX 0x8u
 #define GKO_STATUS_TIMEOUT_DRAIN 0x10u
+#define GKO_STATUS_BAD_INDEX 0x20u /* a page, slot or length outside its table; the access was skipped */
 
 /* Message for the last error returned on this host thread ("" if none). */
 const char* gko_last_error(void);
@@ -286,6 +287,60 @@ int gko_linear_allreduce(int dtype, int64_t m, int64_t n, int64_t k, const void*
                          int64_t x_sk, const void* w, int64_t w_sn, int64_t w_sk, void* out,
                          int64_t ldo, void* out_multicast, void* const* out_peers, int world,
                          unsigned int* status, void* stream);
+
+/*
+ * A paged key / value cache in 4 or 8 bits. No reference counterpart: the reference has no serving
+ * path; these entries are what a decoder needs beside gko_fmha_varlen_fwd.
+ *
+ * One row (a token of one kv head, d values x) is kept as d codes and a pair (scale, zero) in the
+ * element type: zero = min x, scale = (max x - min x) / (2^bits - 1) rounded up to the element type
+ * (at least 2^-100 for bf16, 2^-24 for f16), code = rint((x - zero) / scale); a code stands for
+ * code * scale + zero, within scale / 2 of x. A row with a NaN, an infinity or a range beyond f32
+ * reads back as NaN. Layout, contiguous and 16-byte aligned:
+ *   codes  [pages, hkv, page_size, d * bits / 8] bytes (4 bits: channel 2i in the low half of byte i)
+ *   pairs  [pages, hkv, page_size, 2] elements (scale, zero)
+ * page_size is a multiple of 16; d is 64 or 128; dtype GKO_F16 or GKO_BF16; bits 4 or 8.
+ *
+ * gko_kv_cache_write: k and v are [tokens, hkv, d] with element strides (token, head), multiples of
+ * 8. slots[t] = page * page_size + place in the page; a negative slot skips the token, one past the
+ * cache skips it and sets GKO_STATUS_BAD_INDEX. Slots of one call are distinct (a slot given twice
+ * holds an unspecified mix of the rows).
+ *
+ * gko_kv_cache_read: token i of sequence s is at place i % page_size of page table[s, i / page_size]
+ * (row stride table_stride, table_width columns). Sequence s goes to rows [cu_seqlens[s],
+ * cu_seqlens[s + 1]) of the contiguous k and v [tokens, hkv, d]; rows of no sequence, and rows whose
+ * page is outside [0, pages) or the table (GKO_STATUS_BAD_INDEX), are left as they were.
+ */
+int gko_kv_cache_write(int dtype, int bits, int64_t tokens, int64_t hkv, int64_t d, const void* k, int64_t k_st,
+                       int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int64_t* slots,
+                       void* k_codes, void* v_codes, void* k_pairs, void* v_pairs, int64_t pages,
+                       int64_t page_size, unsigned int* status, void* stream);
+int gko_kv_cache_read(int dtype, int bits, int64_t b, int64_t hkv, int64_t d, int64_t tokens, const void* k_codes,
+                      const void* v_codes, const void* k_pairs, const void* v_pairs, int64_t pages,
+                      int64_t page_size, const int32_t* table, int64_t table_stride, int64_t table_width,
+                      const int32_t* cu_seqlens, void* k, void* v, unsigned int* status, void* stream);
+
+/*
+ * Attention of new tokens over that cache. q is [tq, hq, d] with element strides (token, head);
+ * sequence s owns rows [cu_seqlens_q[s], cu_seqlens_q[s + 1]) (NULL: row s alone), at most
+ * max_seqlen_q of them, and seq_lens[s] cached tokens, the new ones included: query i of n is at
+ * position seq_lens[s] - n + i. causal keeps key <= position; window > 0 keeps |key - position| <=
+ * window or key < sinks; softcap as for gko_fmha_fwd. max_seqlen_k is what the work is split by: a
+ * longer sequence is still answered in full. out [tq, hq, d] contiguous, lse f32 [hq, tq]; a row that
+ * sees no key gives zeros and -inf; rows of no sequence are left as they were. A page outside
+ * [0, pages) counts as masked and sets GKO_STATUS_BAD_INDEX, as does a length past the table, which
+ * is cut to it. The result does not vary from run to run. workspace: 16-byte aligned device memory of
+ * gko_fmha_cache_workspace_size bytes (may be 0; -1: sizes out of range), overwritten by the call.
+ */
+int64_t gko_fmha_cache_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+                                      int64_t max_seqlen_q, int64_t max_seqlen_k, int window, int sinks);
+int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+                       int64_t max_seqlen_q, int64_t max_seqlen_k, const void* q, int64_t q_st, int64_t q_sh,
+                       const void* k_codes, const void* v_codes, const void* k_pairs, const void* v_pairs,
+                       int64_t pages, int64_t page_size, const int32_t* table, int64_t table_stride,
+                       int64_t table_width, const int32_t* seq_lens, const int32_t* cu_seqlens_q, float scale,
+                       int causal, int window, float softcap, int sinks, void* out, float* lse, void* workspace,
+                       int64_t workspace_bytes, unsigned int* status, void* stream);
 
 /*
  * out[i] = silu(x[i]) * y[i] over n contiguous elements (dtype f16, bf16 or f32).

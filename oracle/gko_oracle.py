@@ -34,6 +34,7 @@ __all__ = [
     "rmsnorm",
     "rope",
     "llama_block",
+    "kv_quantise", "kv_pack", "kv_unpack", "kv_values", "kv_sequence", "visible", "attention64",
 ]
 
 
@@ -269,3 +270,81 @@ def llama_block(x, w, cfg):
     h2 = rmsnorm(x1, w["mlp_norm"], cfg.eps)
     g = F.silu(F.linear(h2, _f32(w["w_gate"]))) * F.linear(h2, _f32(w["w_up"]))
     return x1 + F.linear(g, _f32(w["w_down"]))
+
+
+# --------------------------------------------------------------------------- paged quantised cache, windows with sinks
+KV_FLOOR = {torch.bfloat16: 2.0 ** -100, torch.float16: 2.0 ** -24}
+
+
+def kv_quantise(x, bits):
+    """Codes (uint8) and (scale, zero) pairs (x's type) of rows x [..., d]: zero = min, scale =
+    (max - min) / (2^bits - 1) rounded up to the type (at least KV_FLOOR), code = rint((x - zero) / scale).
+    f32 arithmetic, each operation rounded once. A row with a non-finite value, or a range beyond f32,
+    gets scale 0, zero NaN, codes 0. No reference counterpart (the reference has no cache)."""
+    f = x.detach().float().cpu()
+    low, high = f.amin(-1, keepdim=True), f.amax(-1, keepdim=True)
+    want = (high - low) / torch.full_like(high, 2.0 ** bits - 1)
+    near = want.to(x.dtype)
+    scale = torch.where(near.float() < want, (near.view(torch.int16) + 1).view(x.dtype), near).float()
+    scale = torch.clamp_min(scale, KV_FLOOR[x.dtype])
+    fine = torch.isfinite(f).all(-1, keepdim=True) & torch.isfinite(scale)
+    codes = torch.where(fine, torch.round((f - low) / scale).clamp(0, 2 ** bits - 1), torch.zeros_like(f))
+    scale = torch.where(fine, scale, torch.zeros_like(scale))
+    zero = torch.where(fine, low, torch.full_like(low, float("nan")))
+    return codes.to(torch.uint8), torch.cat([scale, zero], -1).to(x.dtype)
+
+
+def kv_pack(codes, bits):
+    """Codes [..., d] as cache bytes: for 4 bits, channel 2i in the low half of byte i."""
+    return codes if bits == 8 else codes[..., 0::2] | (codes[..., 1::2] << 4)
+
+
+def kv_unpack(codes, bits):
+    return codes if bits == 8 else torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+
+
+def kv_values(codes, pairs, bits):
+    """What cache rows stand for, in 64 bits: code * scale + zero."""
+    pairs = pairs.double()
+    return kv_unpack(codes, bits).double() * pairs[..., :1] + pairs[..., 1:]
+
+
+def kv_sequence(codes, pairs, table_row, length, bits):
+    """Rows 0 .. length - 1 of one sequence -> f64 [length, kv heads, d], from its pages."""
+    page = codes.shape[2]
+    used = table_row[: -(-length // page)].long()
+    rows = kv_values(codes[used], pairs[used], bits)
+    return rows.transpose(1, 2).flatten(0, 1)[:length]
+
+
+def visible(i, j, causal=0, window=0, sinks=0):
+    """Keys j that a query at position i sees: key <= i when causal, and |i - j| <= window or j < sinks."""
+    keep = torch.ones(torch.broadcast_shapes(i.shape, j.shape), dtype=torch.bool)
+    if causal:
+        keep = keep & (j <= i)
+    if window:
+        keep = keep & (((i - j).abs() <= window) | (j < sinks))
+    return keep
+
+
+def attention64(q, k, v, scale, causal=0, window=0, softcap=0.0, sinks=0, offset=0):
+    """One sequence in 64 bits: q [sq, hq, d] at positions offset + i over k, v [sk, hkv, d] ->
+    (out [sq, hq, d], lse [hq, sq], P [hq, sq, sk]); a row that sees no key gives zeros and -inf."""
+    q, k, v = q.double(), k.double(), v.double()
+    g = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    s = torch.einsum("ihd,jhd->hij", q, k) * scale
+    if softcap:
+        s = softcap * torch.tanh(s / softcap)
+    i = torch.arange(q.shape[0])[:, None] + offset
+    keep = visible(i, torch.arange(k.shape[0])[None, :], causal, window, sinks)
+    s = s.masked_fill(~keep, -math.inf)
+    if k.shape[0] == 0:
+        return torch.zeros_like(q), torch.full((q.shape[1], q.shape[0]), -math.inf, dtype=torch.float64), s
+    m = s.amax(-1, keepdim=True)
+    m = torch.where(m == -math.inf, torch.zeros_like(m), m)
+    e = torch.exp(s - m).masked_fill(~keep, 0.0)
+    l = e.sum(-1, keepdim=True)
+    p = e / torch.where(l == 0, torch.ones_like(l), l)
+    out = torch.einsum("hij,jhd->ihd", p, v.masked_fill(~keep.any(0)[:, None, None], 0.0))
+    return out, torch.where(l == 0, torch.full_like(l, -math.inf), m + torch.log(l)).squeeze(-1), p

@@ -1,0 +1,112 @@
+"""The paged cache without a GPU: the C entries' refusals, the workspace rule, fake shapes, and the oracle's
+quantisation against its own promise."""
+
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import oracle
+from evocompile_b200 import _lib, kernels
+
+
+def _p(x=1 << 20):
+    return ctypes.c_void_p(x)  # never dereferenced: validation fails first, or there is nothing to do
+
+
+def _write(lib, dtype=_lib.BF16, bits=4, tokens=4, hkv=2, d=64, k=1 << 20, st=128, page=16, codes=1 << 20):
+    return lib.gko_kv_cache_write(dtype, bits, tokens, hkv, d, _p(k), st, 64, _p(), st, 64, _p(), _p(codes), _p(), _p(),
+                                  _p(), 4, page, None, None)
+
+
+def _read(lib, dtype=_lib.BF16, bits=4, b=2, tokens=4, d=64, page=16, width=4, table=1 << 20, out=1 << 20):
+    return lib.gko_kv_cache_read(dtype, bits, b, 2, d, tokens, _p(), _p(), _p(), _p(), 4, page, _p(table), 4, width, _p(),
+                                 _p(out), _p(), None, None)
+
+
+def _attend(lib, dtype=_lib.BF16, bits=4, b=2, hq=4, hkv=2, d=64, tq=2, max_q=1, max_k=64, q=1 << 20, page=16, width=4,
+            window=0, softcap=0.0, sinks=0, scale=0.1, out=1 << 20, ws=0, ws_bytes=0):
+    return lib.gko_fmha_cache_fwd(dtype, bits, b, hq, hkv, d, tq, max_q, max_k, _p(q), 256, 64, _p(), _p(), _p(), _p(), 4,
+                                  page, _p(), 4, width, _p(), None, scale, 1, window, softcap, sinks, _p(out), _p(), _p(ws),
+                                  ws_bytes, None, None)
+
+
+@pytest.mark.parametrize("call,bad,code,message", [
+    (_write, dict(dtype=_lib.F32), _lib.ERR_UNSUPPORTED, "float16 and bfloat16"),
+    (_write, dict(bits=5), _lib.ERR_UNSUPPORTED, "4 or 8 bits"),
+    (_write, dict(d=96), _lib.ERR_UNSUPPORTED, "head dim"),
+    (_write, dict(page=24), _lib.ERR_UNSUPPORTED, "multiple of 16"),
+    (_write, dict(tokens=-1), _lib.ERR_INVALID, "bad sizes"),
+    (_write, dict(k=0), _lib.ERR_INVALID, "null"),
+    (_write, dict(st=130), _lib.ERR_UNSUPPORTED, "multiples of 8"),
+    (_write, dict(codes=(1 << 20) + 8), _lib.ERR_UNSUPPORTED, "16-byte"),
+    (_read, dict(dtype=_lib.F32), _lib.ERR_UNSUPPORTED, "float16 and bfloat16"),
+    (_read, dict(bits=2), _lib.ERR_UNSUPPORTED, "4 or 8 bits"),
+    (_read, dict(page=0), _lib.ERR_UNSUPPORTED, "multiple of 16"),
+    (_read, dict(b=-1), _lib.ERR_INVALID, "bad sizes"),
+    (_read, dict(table=0), _lib.ERR_INVALID, "null"),
+    (_read, dict(out=(1 << 20) + 2), _lib.ERR_UNSUPPORTED, "16-byte"),
+    (_attend, dict(dtype=_lib.F32), _lib.ERR_UNSUPPORTED, "float16 and bfloat16"),
+    (_attend, dict(bits=16), _lib.ERR_UNSUPPORTED, "4 or 8 bits"),
+    (_attend, dict(d=256), _lib.ERR_UNSUPPORTED, "head dim"),
+    (_attend, dict(hq=5), _lib.ERR_INVALID, "multiple of kv heads"),
+    (_attend, dict(window=-1), _lib.ERR_INVALID, "negative"),
+    (_attend, dict(sinks=-1), _lib.ERR_INVALID, "negative"),
+    (_attend, dict(softcap=-1.0), _lib.ERR_INVALID, "softcap"),
+    (_attend, dict(scale=float("nan")), _lib.ERR_INVALID, "scale"),
+    (_attend, dict(page=8), _lib.ERR_UNSUPPORTED, "multiple of 16"),
+    (_attend, dict(width=1 << 27), _lib.ERR_UNSUPPORTED, "2^31"),
+    (_attend, dict(b=70000, tq=70000), _lib.ERR_UNSUPPORTED, "out of range"),
+    (_attend, dict(q=0), _lib.ERR_INVALID, "null"),
+    (_attend, dict(out=(1 << 20) + 4), _lib.ERR_UNSUPPORTED, "16-byte"),
+    (_attend, dict(max_k=100000), _lib.ERR_INVALID, "workspace"),
+])
+def test_refusals(lib, call, bad, code, message):
+    assert call(lib, **bad) == code
+    assert message in _lib.last_error()
+
+
+def test_nothing_to_do(lib):
+    assert _write(lib, tokens=0, k=0) == _lib.OK
+    assert _read(lib, tokens=0, table=0) == _lib.OK
+    assert _read(lib, b=0, table=0) == _lib.OK
+    assert _attend(lib, b=0, tq=0, q=0) == _lib.OK
+    assert _attend(lib, tq=0, q=0) == _lib.OK
+
+
+def test_workspace_rule(lib):
+    """Nothing when the keys fit one split; refused sizes give -1; a window bounds what a long cache needs."""
+    size = lib.gko_fmha_cache_workspace_size
+    assert size(1, 8, 8, 128, 1, 1, 100, 0, 0) == 0
+    long_ = size(1, 8, 8, 128, 1, 1, 100000, 0, 0)
+    assert long_ > 0 and long_ % (8 * (128 * 4 + 8)) == 0
+    assert size(1, 8, 8, 128, 1, 1, 100000, 64, 4) <= size(1, 8, 8, 128, 1, 1, 400, 0, 0)
+    assert size(0, 8, 8, 128, 0, 1, 100000, 0, 0) == 0
+    assert size(1, 8, 3, 128, 1, 1, 100, 0, 0) == -1
+    assert size(1, 8, 8, 100, 1, 1, 100, 0, 0) == -1
+
+
+def test_fake_shapes():
+    kernels.register("kv_cache")
+    with FakeTensorMode():
+        codes = torch.empty(4, 2, 16, 64, dtype=torch.uint8)
+        pairs = torch.empty(4, 2, 16, 2, dtype=torch.bfloat16)
+        table, lens = torch.empty(3, 5, dtype=torch.int32), torch.empty(3, dtype=torch.int32)
+        k, v = torch.ops.gko.kv_cache_read(codes, codes, pairs, pairs, table, torch.empty(4, dtype=torch.int32), 30, 128)
+        assert k.shape == v.shape == (30, 2, 128) and k.dtype == torch.bfloat16
+        out, lse = torch.ops.gko.fmha_cache_fwd(torch.empty(3, 8, 128, dtype=torch.bfloat16), codes, codes, pairs, pairs,
+                                                table, lens, None, 1, 80, 0.1, 1, 0, 0.0, 0)
+        assert out.shape == (3, 8, 128) and lse.shape == (8, 3) and lse.dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_oracle_quantisation(dtype, bits):
+    x = (torch.randn(200, 64, generator=torch.Generator().manual_seed(1)) + 3).to(dtype)
+    codes, pairs = oracle.kv_quantise(x, bits)
+    assert int(codes.min()) == 0 and int(codes.max()) <= 2 ** bits - 1
+    packed = oracle.kv_pack(codes, bits)
+    assert packed.shape[-1] == 64 * bits // 8 and torch.equal(oracle.kv_unpack(packed, bits), codes)
+    off = (oracle.kv_values(packed, pairs, bits) - x.double()).abs()
+    assert (off <= pairs[:, :1].double() * (0.5 + 2.0 ** -14)).all()

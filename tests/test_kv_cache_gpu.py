@@ -1,0 +1,410 @@
+"""The paged 4- and 8-bit cache on the GPU: writing, reading back and attention over it, against 64 bits.
+
+Tolerances, from the arithmetic (u = half a step of a type: f16 2^-11, bf16 2^-8, f32 2^-24):
+
+* codes and pairs are equal to the formulas evaluated in f32, operation by operation;
+* a value read back is code * scale (exact in f32) + zero, rounded to f32 and then to the type;
+* attention: a logit is an f32 sum of d exact products, two f32 multiply-adds and a product, off by at
+  most (d + 8) u32 times the sum of the products' magnitudes (``mag``), and its exponential by 2^-21 more.
+  Each probability times scale_v is rounded to f16 (u16, or 2^-25 of twice the largest scale_v when it
+  underflows), so the code part of the output is off by u16 of itself; the output is rounded once.
+"""
+
+import pytest
+import torch
+
+import oracle
+from evocompile_b200 import _lib, kernels, ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _status_clear(bits=0):
+    torch.cuda.synchronize()
+    assert _lib.read_status(torch.device("cuda", 0)) == bits
+
+
+def _rows(gen, *shape, dtype):
+    x = torch.randn(*shape, generator=gen) + 1.5 * torch.randn(shape[-1], generator=gen)
+    return x.to(dtype)
+
+
+def _same(a, b):
+    """Bit patterns equal, any NaN equal to any NaN."""
+    a, b = a.cpu(), b.cpu()
+    return bool(((a == b) | (a.isnan() & b.isnan())).all()) if a.is_floating_point() else torch.equal(a, b)
+
+
+def _cache(gen, lens, page, hkv, d, bits, dtype, spare=2):
+    """A filled cache (CPU tensors) with shuffled pages; places behind a sequence's end, and spare pages, hold
+    codes of their own and pairs of NaN, which nothing may look at."""
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + spare
+    order = torch.randperm(pages, generator=gen)
+    table = torch.full((len(lens), max(max(need), 1) + 1), pages + 7, dtype=torch.int32)  # unused entries are no pages
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n].to(torch.int32)
+        at += n
+    out = []
+    for _ in range(2):
+        codes, pairs = oracle.kv_quantise(_rows(gen, pages, hkv, page, d, dtype=dtype), bits)
+        keep = torch.zeros(pages, page, dtype=torch.bool)
+        for i, n in enumerate(lens):
+            for t in range(0, n, page):
+                keep[table[i, t // page], : min(page, n - t)] = True
+        pairs = torch.where(keep[:, None, :, None], pairs, torch.full_like(pairs, float("nan")))
+        out.append((oracle.kv_pack(codes, bits), pairs))
+    return ops.KVCache(out[0][0], out[1][0], out[0][1], out[1][1]), table
+
+
+def _to(cache):
+    return ops.KVCache(*(t.to(DEV) for t in cache))
+
+
+# --------------------------------------------------------------------------- write
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d,hkv,tokens,page", [(64, 1, 1, 16), (64, 3, 37, 16), (128, 8, 5, 48), (128, 2, 300, 64)])
+def test_write(dtype, bits, d, hkv, tokens, page):
+    gen = torch.Generator().manual_seed(tokens * 8 + bits)
+    pages = -(-tokens // page) + 2
+    cache = ops.kv_cache_alloc(pages, page, hkv, d, bits, dtype)
+    before = [t.clone() for t in cache]
+    k, v = _rows(gen, tokens, hkv, d, dtype=dtype), _rows(gen, tokens, hkv, d, dtype=dtype)
+    slots = torch.randperm(pages * page, generator=gen)[:tokens]
+    slots[::5] = -1 - slots[::5]  # padding
+    ops.kv_cache_write(k.to(DEV), v.to(DEV), cache, slots.to(DEV))
+    _status_clear()
+    want = [t.cpu() for t in before]
+    live = slots >= 0
+    at, row = slots[live] // page, slots[live] % page
+    for x, c, p in ((k, 0, 2), (v, 1, 3)):
+        codes, pairs = oracle.kv_quantise(x[live], bits)
+        want[c][at, :, row] = oracle.kv_pack(codes, bits)
+        want[p][at, :, row] = pairs
+        # and the promise itself: within half a step of what was written
+        back = oracle.kv_values(cache[c].cpu()[at, :, row], cache[p].cpu()[at, :, row], bits)
+        step = cache[p].cpu()[at, :, row][..., :1].double()
+        assert ((back - x[live].double()).abs() <= step * (0.5 + 2.0 ** -14)).all()
+    for got, w in zip(cache, want):
+        assert _same(got, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_write_special_rows(dtype, bits):
+    """Constant rows, zeros, ties, tiny and huge values; a NaN or an infinity makes its row NaN and no other."""
+    d, big = 64, torch.finfo(dtype).max
+    rows = torch.zeros(10, d)
+    rows[1] = 3.25
+    rows[2, 5] = float("nan")
+    rows[3, 7], rows[4, 9] = float("inf"), float("-inf")
+    rows[5] = torch.arange(d) % 31 * 0.5  # ties at half steps for 4 bits: a range of 15 and values at k + 0.5
+    rows[6] = torch.linspace(-1, 1, d) * torch.finfo(dtype).tiny
+    rows[7] = torch.linspace(-0.25, 0.25, d) * big
+    rows[8] = torch.linspace(1000, 1001, d)
+    rows[9, 3] = -torch.finfo(dtype).tiny / 2  # a subnormal
+    rows = rows.to(dtype)[:, None, :]
+    cache = ops.kv_cache_alloc(1, 16, 1, d, bits, dtype)
+    ops.kv_cache_write(rows.to(DEV), rows.flip(0).to(DEV), cache, torch.arange(10, device=DEV))
+    _status_clear()
+    for x, c, p in ((rows, 0, 2), (rows.flip(0), 1, 3)):
+        codes, pairs = oracle.kv_quantise(x, bits)
+        assert _same(cache[c][0, 0, :10], oracle.kv_pack(codes, bits)[:, 0])
+        assert _same(cache[p][0, 0, :10], pairs[:, 0])
+
+
+def test_write_strided_views_and_bad_slots():
+    """k and v as column ranges of one projection output; slots past the cache are skipped with a status bit."""
+    gen = torch.Generator().manual_seed(3)
+    t, hq, hkv, d, page = 20, 4, 2, 128, 16
+    qkv = _rows(gen, t, (hq + 2 * hkv) * d, dtype=torch.bfloat16).to(DEV)
+    k = qkv[:, hq * d:(hq + hkv) * d].view(t, hkv, d)
+    v = qkv[:, (hq + hkv) * d:].view(t, hkv, d)
+    cache = ops.kv_cache_alloc(2, page, hkv, d, 4)
+    slots = torch.arange(t) + 5
+    slots[3], slots[4] = 2 * page, 1 << 40
+    ops.kv_cache_write(k, v, cache, slots.to(DEV))
+    _status_clear(0x20)
+    good = [i for i in range(t) if i not in (3, 4)]
+    codes, pairs = oracle.kv_quantise(v.cpu()[good], 4)
+    at = slots[good]
+    assert _same(cache.v_codes.cpu()[at // page, :, at % page], oracle.kv_pack(codes, 4))
+    assert _same(cache.v_pairs.cpu()[at // page, :, at % page], pairs)
+    untouched = cache.k_pairs.cpu()[0, :, :5]
+    assert not untouched.any() and not cache.k_pairs.cpu()[0, :, 8:10].any()
+
+
+# --------------------------------------------------------------------------- read
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d,hkv,page,lens", [(64, 1, 16, [1]), (128, 3, 48, [0, 47, 48, 0, 49, 0]),
+                                             (64, 8, 32, [100, 3, 65]), (128, 2, 64, [5, 700])])
+def test_read(dtype, bits, d, hkv, page, lens):
+    gen = torch.Generator().manual_seed(sum(lens) + bits)
+    cache, table = _cache(gen, lens, page, hkv, d, bits, dtype)
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32)
+    total = int(cu[-1])
+    out = tuple(torch.full((total + 3, hkv, d), 7.0, dtype=dtype, device=DEV) for _ in range(2))
+    got = ops.kv_cache_read(_to(cache), table.to(DEV), cu.to(DEV), total + 3, d, out=out)
+    _status_clear()
+    for x, c, p in ((got[0], 0, 2), (got[1], 1, 3)):
+        want = torch.cat([oracle.kv_sequence(cache[c], cache[p], table[i], n, bits) for i, n in enumerate(lens)])
+        assert ((x[:total].cpu().double() - want).abs() <= want.abs() * (HALF[dtype] + 2.0 ** -23)).all()
+        assert (x[total:] == 7.0).all()
+
+
+def test_read_bad_page_leaves_rows():
+    gen = torch.Generator().manual_seed(4)
+    cache, table = _cache(gen, [40, 20], 16, 2, 64, 8, torch.float16)
+    table[0, 1] = -5
+    cu = torch.tensor([0, 40, 60], dtype=torch.int32)
+    out = tuple(torch.full((60, 2, 64), 7.0, dtype=torch.float16, device=DEV) for _ in range(2))
+    ops.kv_cache_read(_to(cache), table.to(DEV), cu.to(DEV), 60, 64, out=out)
+    _status_clear(0x20)
+    assert (out[0][16:32] == 7.0).all() and not (out[0][:16] == 7.0).all(-1).any()
+    assert not (out[0][32:] == 7.0).all(-1).any()
+
+
+# --------------------------------------------------------------------------- attention over the cache
+def _check_attention(got, q, cache, table, lens, news, bits, causal, window, softcap, sinks, scale):
+    out, lse = (t.cpu().double() for t in got)
+    dtype, d, hq = q.dtype, q.shape[2], q.shape[1]
+    at = 0
+    for i, (n, new) in enumerate(zip(lens, news)):
+        k, v = (oracle.kv_sequence(cache[c], cache[c + 2], table[i], n, bits) for c in (0, 1))
+        qs = q[at:at + new].cpu()
+        want, want_lse, p = oracle.attention64(qs, k, v, scale, causal, window, softcap, sinks, n - new)
+        rows = slice(at, at + new)
+        at += new
+        empty = want_lse == -float("inf")
+        assert torch.equal(lse[:, rows] == -float("inf"), empty)
+        assert (out[rows][empty.T] == 0).all()
+        if n == 0 or new == 0:
+            continue
+        # magnitudes: |codes part| + |zero part| of a logit, and the code part of the output
+        used = table[i, : -(-n // cache[0].shape[2])].long()
+        pair = [c[used].transpose(1, 2).flatten(0, 1)[:n].double() for c in (cache[2], cache[3])]
+        group = hq // cache[0].shape[1]
+        qa = qs.double().abs().sum(-1).amax().item()
+        mag = abs(scale) * qa * ((2 ** bits - 1) * pair[0][..., 0].amax() + pair[0][..., 1].abs().amax()).item()
+        logit = (d + 8) * 2.0 ** -24 * mag + 2.0 ** -21
+        codes = (v - pair[1][..., 1:]).repeat_interleave(group, 1)
+        part = torch.einsum("hij,jhd->ihd", p, codes)
+        under = n * 2.0 ** -25 * 2 * pair[1][..., 0].amax().item() * (2 ** bits - 1)
+        tol = want.abs() * HALF[dtype] + part * 2.0 ** -11 + under + 2 * logit * v.abs().amax().item()
+        assert ((out[rows] - want).abs() <= tol).all(), (i, ((out[rows] - want).abs() / tol).max())
+        fin = ~empty
+        bound = logit + 2.0 ** -22 * want_lse[fin].abs()
+        assert ((lse[:, rows][fin] - want_lse[fin]).abs() <= bound).all()
+
+
+def _attend(gen, lens, news, page, hq, hkv, d, bits, dtype, causal=1, window=0, softcap=0.0, sinks=0, bound=None, grow=0.0):
+    cache, table = _cache(gen, lens, page, hkv, d, bits, dtype)
+    if grow:  # keys whose scales rise along the sequence, values whose scales jump
+        for i, n in enumerate(lens):
+            for t in range(0, n, page):
+                cache.k_pairs[table[i, t // page]] *= 1 + grow * t / max(n, 1)
+                cache.v_pairs[table[i, t // page]] *= 2.0 ** (t // page % 7 - 3)
+    q = _rows(gen, sum(news), hq, d, dtype=dtype)
+    cu = torch.tensor([0] + torch.tensor(news).cumsum(0).tolist(), dtype=torch.int32)
+    scale = d ** -0.5
+    args = (q.to(DEV), _to(cache), table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
+            None if all(n == 1 for n in news) else cu.to(DEV), max(news), bound or max(max(lens), 1), scale, causal, window,
+            softcap, sinks)
+    got = ops.fmha_cache_fwd(*args)
+    _status_clear()
+    _check_attention(got, q, cache, table, lens, news, bits, causal, window, softcap, sinks, scale)
+    again = ops.fmha_cache_fwd(*args)
+    assert _same(got[0], again[0]) and _same(got[1], again[1])  # the same bits
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(8, 1), (4, 4), (6, 2)])
+def test_attend_single_tokens(dtype, bits, d, hq, hkv):
+    gen = torch.Generator().manual_seed(bits + d + hq)
+    _attend(gen, [1, 33, 0, 500, 64], [1] * 5, 32, hq, hkv, d, bits, dtype)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("page", [16, 48, 128])
+@pytest.mark.parametrize("lens,news", [([17, 5, 200], [3, 5, 0]), ([700, 2, 31], [1, 4, 9]), ([90], [40])])
+def test_attend_several_tokens(bits, page, lens, news):
+    """Fewer cached tokens than new ones leave rows empty; a column tile ends inside a token's heads."""
+    gen = torch.Generator().manual_seed(bits + page + sum(lens))
+    _attend(gen, lens, news, page, 6, 2, 128, bits, torch.bfloat16)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("causal,window,sinks,softcap", [(1, 50, 0, 0.0), (1, 100, 4, 0.0), (0, 20, 70, 0.0), (1, 1, 33, 0.0),
+                                                         (0, 0, 9, 0.0), (1, 64, 5, 20.0), (1, 10000, 3, 0.0)])
+def test_attend_window_sinks_softcap(bits, causal, window, sinks, softcap):
+    gen = torch.Generator().manual_seed(window + sinks + bits)
+    _attend(gen, [300, 7, 1200], [2, 2, 2], 16, 8, 2, 64, bits, torch.float16, causal, window, softcap, sinks)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_attend_long_in_splits(bits):
+    """Many key splits, one of them longer than the bound the caller gave; scales that rise and jump."""
+    gen = torch.Generator().manual_seed(9 + bits)
+    _attend(gen, [9000, 300], [1, 1], 64, 8, 1, 128, bits, torch.bfloat16, grow=4.0)
+    _attend(gen, [9000, 300], [1, 1], 64, 8, 1, 128, bits, torch.float16, bound=1000)
+
+
+def test_attend_bad_values_and_pages():
+    """A row read as NaN reaches the queries that see it and no other; a page that is none counts as masked;
+    a length past the table is cut."""
+    gen = torch.Generator().manual_seed(12)
+    d, page, lens = 128, 16, [40, 48, 40]
+    cache, table = _cache(gen, lens, page, 2, d, 4, torch.bfloat16)
+    q = _rows(gen, 3, 4, d, dtype=torch.bfloat16)
+    nan = ops.KVCache(*(t.clone() for t in cache))
+    nan.k_pairs[table[1, 0], 0, 3] = torch.tensor([0.0, float("nan")])
+    nan.v_pairs[table[2, 1], 1, 2] = torch.tensor([0.0, float("nan")])
+    ln = torch.tensor(lens, dtype=torch.int32)
+    call = lambda c, tb, n: ops.fmha_cache_fwd(q.to(DEV), _to(c), tb.to(DEV), n.to(DEV))  # noqa: E731
+    base, _ = call(cache, table, ln)
+    got, lse = call(nan, table, ln)
+    _status_clear()
+    assert got[1, :2].isnan().all() and lse[:2, 1].isnan().all() and not lse[2:, 1].isnan().any()
+    assert got[2, 2:].isnan().all() and not lse[:, 2].isnan().any()
+    assert _same(got[0], base[0]) and _same(got[1, 2:], base[1, 2:]) and _same(got[2, :2], base[2, :2])
+    # page 1 of sequence 0 is none: its 16 keys do not count
+    bad = table.clone()
+    bad[0, 1] = 10 ** 6
+    got, _ = call(cache, bad, ln)
+    _status_clear(0x20)
+    k, v = (oracle.kv_sequence(cache[c], cache[c + 2], table[0], 40, 4) for c in (0, 1))
+    keep = torch.tensor([t for t in range(40) if not 16 <= t < 32])
+    want, _, _ = oracle.attention64(q[:1], k[keep], v[keep], d ** -0.5)
+    assert (got[0].cpu().double() - want[0]).abs().max() <= 0.01 * want.abs().max()
+    assert _same(got[1:], base[1:])
+    # a length past the table's three columns is cut to them
+    got, _ = call(cache, table[:, :3].contiguous(), torch.tensor([40, 1000, 40], dtype=torch.int32))
+    _status_clear(0x20)
+    assert _same(got, base)
+
+
+def test_attend_rows_of_no_sequence_and_strides():
+    """q as a column range of a projection output; rows behind the last sequence keep what out had."""
+    gen = torch.Generator().manual_seed(14)
+    d, hq, hkv = 64, 4, 2
+    cache, table = _cache(gen, [50, 20], 16, hkv, d, 8, torch.float16)
+    wide = _rows(gen, 6, (hq + 2 * hkv) * d, dtype=torch.float16).to(DEV)
+    q = wide[:, : hq * d].view(6, hq, d)
+    cu = torch.tensor([0, 2, 4], dtype=torch.int32, device=DEV)
+    ln = torch.tensor([50, 20], dtype=torch.int32, device=DEV)
+    out = torch.full((6, hq, d), 7.0, dtype=torch.float16, device=DEV)
+    got, lse = ops.fmha_cache_fwd(q, _to(cache), table.to(DEV), ln, cu, 2, out=out)
+    assert got is out and (out[4:] == 7.0).all()
+    _status_clear()
+    _check_attention((out[:4], lse[:, :4]), q[:4], cache, table, [50, 20], [2, 2], 8, 1, 0, 0.0, 0, d ** -0.5)
+
+
+def test_attend_captured_on_a_side_stream():
+    """A decode step (write, attend) captured into a graph and replayed with other inputs and lengths."""
+    gen = torch.Generator().manual_seed(15)
+    b, hq, hkv, d, page = 3, 8, 2, 128, 16
+    lens = [1000, 30, 1]
+    cache_cpu, table = _cache(gen, lens, page, hkv, d, 4, torch.bfloat16)
+    cache, tb = _to(cache_cpu), table.to(DEV)
+    ln = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    slots = torch.tensor([int(table[i, (n - 1) // page]) * page + (n - 1) % page for i, n in enumerate(lens)], device=DEV)
+    k, v, q = (_rows(gen, b, h, d, dtype=torch.bfloat16).to(DEV) for h in (hkv, hkv, hq))
+
+    def step():
+        ops.kv_cache_write(k, v, cache, slots)
+        return ops.fmha_cache_fwd(q, cache, tb, ln, None, 1, 1100)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, lse = step()
+    for t in (k, v, q):
+        t.copy_(_rows(gen, *t.shape, dtype=torch.bfloat16))
+    ln.copy_(torch.tensor([900, 30, 1]))
+    graph.replay()
+    _status_clear()
+    now = ops.KVCache(*(t.cpu() for t in cache))
+    _check_attention((out, lse), q, now, table, [900, 30, 1], [1] * b, 4, 1, 0, 0.0, 0, d ** -0.5)
+    eager = step()
+    assert _same(out, eager[0]) and _same(lse, eager[1])
+
+
+# --------------------------------------------------------------------------- together, and refusals
+@pytest.mark.parametrize("bits,tol", [(4, 0.2), (8, 0.02)])
+def test_prompt_then_tokens(bits, tol):
+    """A prompt is written, read back for the packed attention, and answered token by token from the cache: the
+    cached answers equal those over the read-back rows, and are near those over the unquantised ones."""
+    kernels.register("kv_cache")
+    gen = torch.Generator().manual_seed(20)
+    lens, hq, hkv, d, page, steps = [70, 33], 8, 2, 128, 16, 3
+    full = [n + steps for n in lens]
+    table = torch.randperm(12, generator=gen)[:12].view(2, 6).to(torch.int32)
+    cache = ops.kv_cache_alloc(12, page, hkv, d, bits)
+    q, k, v = ([_rows(gen, n, h, d, dtype=torch.bfloat16) for n in full] for h in (hq, hkv, hkv))
+    slot = lambda i, t: int(table[i, t // page]) * page + t % page  # noqa: E731
+    prompt = lambda x: torch.cat([t[:n] for t, n in zip(x, lens)]).to(DEV)  # noqa: E731
+    torch.ops.gko.kv_cache_write(prompt(k), prompt(v), *cache,
+                                 torch.tensor([slot(i, t) for i, n in enumerate(lens) for t in range(n)], device=DEV))
+    for s in range(steps):
+        at = [n + s for n in lens]
+        now = lambda x: torch.stack([t[n] for t, n in zip(x, at)]).to(DEV)  # noqa: E731
+        torch.ops.gko.kv_cache_write(now(k), now(v), *cache, torch.tensor([slot(i, t) for i, t in enumerate(at)], device=DEV))
+        out, _ = torch.ops.gko.fmha_cache_fwd(now(q), *cache, table.to(DEV),
+                                              torch.tensor([t + 1 for t in at], dtype=torch.int32, device=DEV), None, 1,
+                                              100, d ** -0.5, 1, 24, 0.0, 4)
+        for i, t in enumerate(at):
+            want, _, _ = oracle.attention64(q[i][t:t + 1], k[i][:t + 1], v[i][:t + 1], d ** -0.5, 1, 24, 0.0, 4, t)
+            assert (out[i].cpu().double() - want[0]).abs().max() <= tol * want.abs().max()
+    cu = torch.tensor([0, full[0], sum(full)], dtype=torch.int32, device=DEV)
+    kb, vb = torch.ops.gko.kv_cache_read(*cache, table.to(DEV), cu, sum(full), d)
+    packed, _ = ops.fmha_varlen_fwd(torch.cat(q).to(DEV), kb, vb, cu, cu, max(full), max(full), d ** -0.5, 1)
+    last = torch.tensor([full[0] - 1, sum(full) - 1])
+    out, _ = ops.fmha_cache_fwd(torch.cat(q)[last].to(DEV), cache, table.to(DEV),
+                                torch.tensor(full, dtype=torch.int32, device=DEV))
+    _status_clear()
+    # both round P (bf16 there) and their outputs; the read-back rows are rounded to bf16 once more
+    assert (out - packed[last]).abs().max() <= 4 * 2.0 ** -8 * packed[last].abs().max()
+
+
+def test_refusals():
+    cache = ops.kv_cache_alloc(4, 16, 2, 64, 4)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=DEV)
+    slots = torch.zeros(3, dtype=torch.int64, device=DEV)
+    for bad in ((x.half(), x.half(), cache, slots), (x[:, :1], x[:, :1], cache, slots), (x, x, cache, slots[:2]),
+                (x, x, cache, slots.int()), (x, x[:2], cache, slots), (x, x, ops.kv_cache_alloc(4, 16, 2, 128, 8), slots),
+                (x, x, cache._replace(k_codes=cache.k_codes.transpose(0, 2)), slots)):
+        with pytest.raises(RuntimeError, match="kv_cache_write"):
+            ops.kv_cache_write(*bad)
+    table = torch.zeros(2, 4, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 3, 5], dtype=torch.int32, device=DEV)
+    for bad in ((cache, table.long(), cu, 5, 64), (cache, table[:1], cu, 5, 64), (cache, table, cu.long(), 5, 64),
+                (cache, table, cu, 5, 96)):
+        with pytest.raises(RuntimeError, match="kv_cache_read"):
+            ops.kv_cache_read(*bad)
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    lens = torch.tensor([3, 2], dtype=torch.int32, device=DEV)
+    for bad in ((q.half(), cache, table, lens), (q[:1], cache, table, lens), (q, cache, table, lens.long()),
+                (q, cache, table, lens, cu[:2], 1), (q[0], cache, table, lens)):
+        with pytest.raises(RuntimeError, match="fmha_cache"):
+            ops.fmha_cache_fwd(*bad)
+    with pytest.raises(RuntimeError, match="multiple of kv heads"):
+        ops.fmha_cache_fwd(q[:, :3], cache, table, lens)
+    with pytest.raises(RuntimeError, match="negative"):
+        ops.fmha_cache_fwd(q, cache, table, lens, window=-1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.fmha_cache_fwd(q.cpu(), cache, table, lens)
+    for bad in (dict(bits=3), dict(head_dim=96), dict(page_size=24), dict(dtype=torch.float32)):
+        with pytest.raises(RuntimeError, match="kv_cache_alloc"):
+            ops.kv_cache_alloc(**{**dict(pages=1, page_size=16, kv_heads=1, head_dim=64), **bad})
+    _status_clear()
