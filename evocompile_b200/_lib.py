@@ -72,6 +72,29 @@ SIGNATURES = {
          _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _fl, _int, _int, _fl, _vp, _i64, _i64, _vp,
          _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp],
     ),
+    "gko_fmha_sinks_fwd": (
+        _int,
+        [_int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _p64, _vp, _p64, _vp, _p64, _vp, _int, _int,
+         _p64, _i64, _p64, _fl, _int, _int, _fl, _int, _vp, _vp, _vp, _vp],
+    ),
+    "gko_fmha_sinks_varlen_fwd": (
+        _int,
+        [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+         _i64, _vp, _vp, _fl, _int, _int, _fl, _int, _vp, _vp, _vp, _vp],
+    ),
+    "gko_fmha_sinks_bwd_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _int]),
+    "gko_fmha_sinks_bwd": (
+        _int,
+        [_int, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _p64, _vp, _p64, _vp, _p64, _vp, _int, _int,
+         _p64, _i64, _vp, _p64, _vp, _p64, _vp, _fl, _int, _int, _fl, _int, _vp, _p64, _vp, _p64, _vp, _p64,
+         _vp, _i64, _vp, _vp],
+    ),
+    "gko_fmha_sinks_varlen_bwd": (
+        _int,
+        [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+         _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _fl, _int, _int, _fl, _int, _vp, _i64, _i64, _vp,
+         _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp],
+    ),
     "gko_linear_allreduce": (
         _int,
         [_int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _int, _vp, _vp],

@@ -15,6 +15,11 @@
 //                head of the GQA group, 64-query block) the masks allow.
 //   3. convert   dq = scale * accumulator, cast to the input dtype.
 //
+// With a window and sinks (leading keys that stay visible) the key tiles that hold sinks are seen by
+// every query, the others by a window of them. A sink tile's queries are split over several CTAs of
+// about a window tile's work each, first in the grid; their dk / dv parts go to the workspace in f32 and
+// a fourth kernel adds them in a fixed order.
+//
 // The main kernel is laid out around two costs of B200: shared-memory bandwidth
 // (about 128 B per clock per SM, which limits MMAs that read both operands from shared
 // memory at N <= 64) and the latency of a hand-off between warps through an mbarrier
@@ -72,6 +77,11 @@ struct Params {
   int zh_kv;      // batch (or sequences) x kv heads
   float scale, scale_log2, softcap;
   int causal, window;
+  int sinks;       // leading keys that the window does not hide (0 without a window)
+  int sink_tiles;  // 128-key tiles that hold sinks (0: no tile is split)
+  int pieces;      // CTAs that share a sink tile's query blocks
+  int piece;       // query blocks each takes
+  float* parts;    // pieces > 1: [batch x kv head][sink tile][piece][dk, dv][128][D]
   const void* bias;
   int bias_mode, bias_dtype, bias_z;
   int64_t b_sz, b_sh, b_sq, b_sk;
@@ -155,12 +165,18 @@ struct Layout {
   static_assert(1024 + kMeta + 256 <= 232448, "shared memory budget");
 };
 
-template <typename T, int D, bool VARLEN, bool EXTRA>
+// What a kernel's recomputation of P handles: kPlain an optional causal mask; kExtra also bias, softcap
+// and windows, element by element; kWindow a window with sinks, where the queries that see a key are one
+// interval, so the mask is two bounds per key row.
+enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
+
+template <typename T, int D, bool VARLEN, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     fmha_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                     const Params p) {
   using L = Layout<D>;
+  constexpr bool EXTRA = MODE == kExtra;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = make_idesc_f16(kBF16, kBN, kBM, false, false);  // S^T, dP^T
   constexpr uint32_t kIdescKV = make_idesc_f16(kBF16, kBN, D, false, true);    // dV, dK
@@ -171,7 +187,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (bh >= p.zh_kv) return;
   const int hk = bh % p.hkv;
   const int zb = bh / p.hkv;
-  const int n0 = (int)blockIdx.x * kBN;  // first key of this CTA (sequence-local)
+  // with sinks, grid.x is (sink tile, piece) pairs and then the other key tiles
+  int kv_tile = (int)blockIdx.x, piece = -1;
+  if constexpr (MODE != kPlain) {
+    if (p.sink_tiles > 0) {
+      const int shared = p.sink_tiles * p.pieces;
+      piece = kv_tile < shared ? kv_tile % p.pieces : -1;
+      kv_tile = kv_tile < shared ? kv_tile / p.pieces : kv_tile - shared + p.sink_tiles;
+    }
+  }
+  const int n0 = kv_tile * kBN;  // first key of this CTA (sequence-local)
   int len_q, len_k, row_q0, row_k0;
   if constexpr (VARLEN) {
     varlen_rows(p.cu_q, zb, p.total_q, row_q0, len_q);
@@ -191,8 +216,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     q_lo = max(q_lo, n0 - p.window);
     q_hi = min(q_hi, n0 + kBN - 1 + p.window + 1);
   }
-  const int jb_lo = q_lo / kBM;
-  const int nq = q_hi > q_lo ? (q_hi + kBM - 1) / kBM - jb_lo : 0;
+  int jb_lo = q_lo / kBM;
+  int nq = q_hi > q_lo ? (q_hi + kBM - 1) / kBM - jb_lo : 0;
+  float* part = nullptr;  // this CTA's dk / dv part, when the tile's queries are shared
+  if constexpr (MODE != kPlain) {
+    if (piece >= 0) {
+      const int first = p.causal ? n0 / kBM : 0, blocks = (len_q + kBM - 1) / kBM;
+      jb_lo = first + piece * p.piece;
+      // the last piece takes what is left, should a sequence be longer than the caller's bound
+      nq = max(0, (piece == p.pieces - 1 ? blocks : min(blocks, jb_lo + p.piece)) - jb_lo);
+      if (p.pieces > 1)
+        part = p.parts + (((int64_t)bh * p.sink_tiles + kv_tile) * p.pieces + piece) * (2 * kBN * D);
+    }
+  }
   const int n_steps = nq * p.group;
   const int64_t tile_base = VARLEN ? varlen_block_base(row_q0, zb) : 0;
   auto tile_of = [&](int hh, int jb) -> int64_t {  // workspace block of (query head, 64-query block)
@@ -212,6 +248,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     dv_base = reinterpret_cast<T*>(p.dv) + (int64_t)zb * p.dv_sz + (int64_t)hk * p.dv_sh;
   }
   if (n_steps == 0) {  // no query sees these keys: dk = dv = 0
+    if (MODE != kPlain && part) {
+      for (int i = threadIdx.x; i < 2 * kBN * D / 4; i += kThreads)
+        reinterpret_cast<float4*>(part)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      return;
+    }
     for (int i = threadIdx.x; i < kBN * (D / 8); i += kThreads) {
       const int r = i / (D / 8), c = i % (D / 8);
       if (n0 + r < len_k) {
@@ -474,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           bool keep = row_valid;
           if (p.causal) keep = keep && (kj <= qi);
-          if (p.window > 0) keep = keep && (kj - qi <= p.window) && (qi - kj <= p.window);
+          if (p.window > 0) keep = keep && ((kj - qi <= p.window && qi - kj <= p.window) || kj < p.sinks);
           const float2 nlp = nl2[c >> 1];
           pv[c] = keep ? fast_exp2(fmaf(x, kLog2e, (c & 1) ? nlp.y : nlp.x)) : 0.f;
           gsc[c] = g;
@@ -488,8 +529,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           pv[c] = fast_exp2(a);
           pv[c + 1] = fast_exp2(bb);
         }
+        if constexpr (MODE == kWindow) {
+          // queries [first, last] see this key: all of them a sink, else those within the window
+          const int first = max(p.causal ? kj : 0, kj < p.sinks ? 0 : kj - p.window) - q0;
+          const int last = !row_valid ? -1 : (kj < p.sinks ? 31 : kj + p.window - q0);
+          if (first > 0 || last < 31) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pv[c] = (c >= first && c <= last) ? pv[c] : 0.f;
+          }
+        }
         // keys past the end, and (causal) queries before the key, get P = 0
-        const int lim = row_valid ? (p.causal ? kj - q0 : 0) : 32;
+        const int lim = MODE == kWindow ? 0 : row_valid ? (p.causal ? kj - q0 : 0) : 32;
         if (lim > 0) {
 #pragma unroll
           for (int c = 0; c < 32; ++c) pv[c] = (c < lim) ? 0.f : pv[c];
@@ -558,6 +608,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t v[32];
         tmem_ld32(tm_row + kTmDK + col, v);
         tmem_wait_ld();
+        if constexpr (MODE != kPlain) {
+          if (part) {
+            float4* dst = reinterpret_cast<float4*>(part + r * D + col);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_float4(__uint_as_float(v[4 * e]) * p.scale, __uint_as_float(v[4 * e + 1]) * p.scale,
+                                   __uint_as_float(v[4 * e + 2]) * p.scale, __uint_as_float(v[4 * e + 3]) * p.scale);
+            continue;
+          }
+        }
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -609,6 +669,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t w32[32];
         tmem_ld32(tm_row + kTmDV + c * 32, w32);
         tmem_wait_ld();
+        if constexpr (MODE != kPlain) {
+          if (part) {
+            uint4* dst = reinterpret_cast<uint4*>(part + kBN * D + dr * D + c * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_uint4(w32[4 * e], w32[4 * e + 1], w32[4 * e + 2], w32[4 * e + 3]);
+            continue;
+          }
+        }
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = Cvt<T>::pack(__uint_as_float(w32[2 * e]), __uint_as_float(w32[2 * e + 1]));
@@ -731,8 +800,61 @@ __global__ void __launch_bounds__(256) fmha_bwd_dq_kernel(const RowParams p) {
   }
 }
 
+// ------------------------------------------------------------------ sinks: dk, dv = sum of a tile's parts
+// One CTA per (sink tile, dk or dv) of one kv head; each thread adds four elements of the pieces in order.
+template <typename T, int D, bool VARLEN>
+__global__ void __launch_bounds__(256) fmha_bwd_sinks_kernel(const Params p) {
+  const int bh = (int)blockIdx.y + (int)blockIdx.z * (int)gridDim.y;
+  if (bh >= p.zh_kv) return;
+  const int hk = bh % p.hkv, zb = bh / p.hkv;
+  const int tile = (int)blockIdx.x >> 1, which = (int)blockIdx.x & 1;
+  int row_k0 = 0, len_k = p.sk;
+  if constexpr (VARLEN) varlen_rows(p.cu_k, zb, p.total_k, row_k0, len_k);
+  const float* src = p.parts + ((int64_t)bh * p.sink_tiles + tile) * p.pieces * (2 * kBN * D) + which * (kBN * D);
+  const int64_t ss = which ? p.dv_ss : p.dk_ss;
+  T* dst = reinterpret_cast<T*>(which ? p.dv : p.dk) + (int64_t)hk * (which ? p.dv_sh : p.dk_sh) +
+           (VARLEN ? (int64_t)row_k0 * ss : (int64_t)zb * (which ? p.dv_sz : p.dk_sz));
+  for (int i = threadIdx.x; i < kBN * D / 4; i += 256) {
+    const int r = i / (D / 4), c = i % (D / 4);
+    if (tile * kBN + r >= len_k) break;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int e = 0; e < p.pieces; ++e) {
+      const float4 x = reinterpret_cast<const float4*>(src + (int64_t)e * (2 * kBN * D))[i];
+      a.x += x.x;
+      a.y += x.y;
+      a.z += x.z;
+      a.w += x.w;
+    }
+    *reinterpret_cast<uint2*>(dst + (int64_t)(tile * kBN + r) * ss + c * 4) =
+        make_uint2(Cvt<T>::pack(a.x, a.y), Cvt<T>::pack(a.z, a.w));
+  }
+}
 
 // ------------------------------------------------------------------ host side
+constexpr int kMaxWindow = (1 << 30) - 1024;  // wider ones hide nothing; position + window stays an int
+
+// How the key tiles that hold sinks are shared out. `pieces` gives each CTA about the query blocks of a
+// window tile (at least 8), without more CTAs than two per SM, which also bounds the workspace.
+struct SinkPlan {
+  int tiles, pieces, piece;
+  int64_t part_floats;
+};
+SinkPlan sink_plan(int64_t zh_kv, int64_t max_q, int64_t max_k, int64_t d, int causal, int window, int sinks) {
+  SinkPlan s{0, 1, 0, 0};
+  if (window <= 0 || sinks <= 0 || max_q <= 0 || max_k <= 0 || zh_kv <= 0) return s;
+  const int64_t keys = sinks < max_k ? sinks : max_k;
+  s.tiles = (int)((keys + kBN - 1) / kBN);
+  const int64_t blocks = (max_q + kBM - 1) / kBM;
+  int64_t piece = ((int64_t)window * (causal ? 1 : 2) + kBN) / kBM + 2;
+  if (piece < 8) piece = 8;
+  const int64_t most = (2 * (int64_t)host::sm_count() + zh_kv * s.tiles - 1) / (zh_kv * s.tiles);
+  if (piece * most < blocks) piece = (blocks + most - 1) / most;
+  s.pieces = (int)((blocks + piece - 1) / piece);
+  s.piece = (int)piece;
+  if (s.pieces > 1) s.part_floats = zh_kv * s.tiles * s.pieces * 2 * kBN * d;
+  return s;
+}
+
 dim3 grid_of(int x, int64_t yz) {
   const unsigned y = (unsigned)(yz < 65535 ? yz : 65535);
   return dim3((unsigned)x, y, (unsigned)((yz + (int64_t)y - 1) / (int64_t)y));
@@ -746,10 +868,10 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t z, int64_t h,
   return host::encode_tmap(m, dtype, 4, base, dims, str, box);
 }
 
-template <typename T, int D, bool VARLEN, bool EXTRA>
+template <typename T, int D, bool VARLEN, int MODE>
 int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                 const Params& p, dim3 grid, cudaStream_t s) {
-  auto kern = fmha_bwd_kernel<T, D, VARLEN, EXTRA>;
+  auto kern = fmha_bwd_kernel<T, D, VARLEN, MODE>;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -764,7 +886,7 @@ int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
 
 template <typename T, int D, bool VARLEN>
 int run_all(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
-            const Params& p, const RowParams& rp, int q_blocks, int kv_tiles, bool extra, cudaStream_t s) {
+            const Params& p, const RowParams& rp, int q_blocks, int kv_tiles, int mode, cudaStream_t s) {
   const dim3 rgrid = grid_of(q_blocks, rp.zh);
   if (q_blocks > 0) {
     fmha_bwd_prep_kernel<T, D, VARLEN><<<rgrid, 256, 0, s>>>(rp);
@@ -772,10 +894,16 @@ int run_all(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
     if (rc) return rc;
   }
   if (kv_tiles > 0) {
-    const dim3 g = grid_of(kv_tiles, p.zh_kv);
-    int rc = extra ? launch_main<T, D, VARLEN, true>(tq, tk, tv, tdo, p, g, s)
-                   : launch_main<T, D, VARLEN, false>(tq, tk, tv, tdo, p, g, s);
+    const dim3 g = grid_of(kv_tiles + p.sink_tiles * (p.pieces - 1), p.zh_kv);
+    int rc = mode == kPlain    ? launch_main<T, D, VARLEN, kPlain>(tq, tk, tv, tdo, p, g, s)
+             : mode == kWindow ? launch_main<T, D, VARLEN, kWindow>(tq, tk, tv, tdo, p, g, s)
+                               : launch_main<T, D, VARLEN, kExtra>(tq, tk, tv, tdo, p, g, s);
     if (rc) return rc;
+    if (p.sink_tiles > 0 && p.pieces > 1) {
+      fmha_bwd_sinks_kernel<T, D, VARLEN><<<grid_of(2 * p.sink_tiles, p.zh_kv), 256, 0, s>>>(p);
+      rc = host::cuda_check(cudaGetLastError(), "fmha bwd sinks launch");
+      if (rc) return rc;
+    }
   }
   if (q_blocks > 0) {
     fmha_bwd_dq_kernel<T, D, VARLEN><<<rgrid, 256, 0, s>>>(rp);
@@ -786,13 +914,13 @@ int run_all(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
 
 template <bool VARLEN>
 int dispatch(int dtype, int d, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-             const CUtensorMap& tdo, const Params& p, const RowParams& rp, int q_blocks, int kv_tiles, bool extra,
+             const CUtensorMap& tdo, const Params& p, const RowParams& rp, int q_blocks, int kv_tiles, int mode,
              cudaStream_t s) {
   if (dtype == GKO_BF16)
-    return d == 64 ? run_all<__nv_bfloat16, 64, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, extra, s)
-                   : run_all<__nv_bfloat16, 128, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, extra, s);
-  return d == 64 ? run_all<__half, 64, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, extra, s)
-                 : run_all<__half, 128, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, extra, s);
+    return d == 64 ? run_all<__nv_bfloat16, 64, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, mode, s)
+                   : run_all<__nv_bfloat16, 128, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, mode, s);
+  return d == 64 ? run_all<__half, 64, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, mode, s)
+                 : run_all<__half, 128, VARLEN>(tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, mode, s);
 }
 
 int64_t workspace_tiles(int64_t batch, int64_t hq, int64_t sq_or_tq, int varlen) {
@@ -800,8 +928,16 @@ int64_t workspace_tiles(int64_t batch, int64_t hq, int64_t sq_or_tq, int varlen)
   return varlen ? hq * (blocks + batch + 1) : batch * hq * blocks;
 }
 
-int check_common(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int window, float softcap) {
+// Windows with sinks run on kWindow unless a bias or a softcap needs kExtra; windows alone keep kExtra.
+int mode_of(bool bias, float softcap, int window, int sinks) {
+  if (bias || softcap > 0.f) return kExtra;
+  if (window > 0) return sinks > 0 ? kWindow : kExtra;
+  return kPlain;
+}
+
+int check_common(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int window, float softcap, int sinks) {
   using host::fail;
+  if (sinks < 0) return fail(GKO_ERR_INVALID, "sinks must be >= 0");
   if (dtype != GKO_F16 && dtype != GKO_BF16)
     return fail(GKO_ERR_UNSUPPORTED, "fmha backward supports float16 and bfloat16 only (dtype code %d)", dtype);
   if (d != 64 && d != 128)
@@ -834,18 +970,41 @@ extern "C" int64_t gko_fmha_bwd_workspace_size(int64_t batch, int64_t hq, int64_
   return tiles * (fmha_bwd::kBM * d * 4 + 2 * fmha_bwd::kBM * 4);
 }
 
-extern "C" int gko_fmha_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk, int64_t d,
+extern "C" int64_t gko_fmha_sinks_bwd_workspace_size(int64_t batch, int64_t hq, int64_t hkv, int64_t sq_or_tq,
+                                                     int64_t max_seqlen_q, int64_t max_seqlen_k, int64_t d,
+                                                     int causal, int window, int sinks, int varlen) {
+  const int64_t base = gko_fmha_bwd_workspace_size(batch, hq, sq_or_tq, d, varlen);
+  if (base < 0 || hkv <= 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || window < 0 || sinks < 0) return -1;
+  const fmha_bwd::SinkPlan sp =
+      fmha_bwd::sink_plan(batch * hkv, varlen ? max_seqlen_q : sq_or_tq, max_seqlen_k, d, causal, window, sinks);
+  return base + sp.part_floats * 4;
+}
+
+extern "C" int gko_fmha_sinks_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk, int64_t d,
                             const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v,
                             const int64_t* vs, const void* bias, int bias_mode, int bias_dtype,
                             const int64_t* bs, int64_t bias_batch, const void* out, const int64_t* os,
                             const void* dout, const int64_t* dos, const float* lse, float scale, int causal,
-                            int window, float softcap, void* dq, const int64_t* dqs, void* dk,
+                            int window, float softcap, int sinks, void* dq, const int64_t* dqs, void* dk,
                             const int64_t* dks, void* dv, const int64_t* dvs, void* workspace,
                             int64_t workspace_bytes, unsigned int* status, void* stream) {
-  int rc = fmha_bwd::check_common(dtype, hq, hkv, d, scale, window, softcap);
+  int rc = fmha_bwd::check_common(dtype, hq, hkv, d, scale, window, softcap, sinks);
   if (rc) return rc;
   if (z < 0 || sq < 0 || sk < 0) return fail(GKO_ERR_INVALID, "negative attention size");
   if (z == 0 || (sq == 0 && sk == 0)) return GKO_OK;
+  if (sk == 0) {  // no key to read or write: any mapped address will do
+    k = v = q;
+    dk = dv = dq;
+    ks = vs = qs;
+    dks = dvs = dqs;
+  }
+  if (sq == 0) {  // no query likewise
+    q = out = dout = k;
+    dq = dk;
+    lse = static_cast<const float*>(k);
+    qs = os = dos = ks;
+    dqs = dks;
+  }
   if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !qs || !ks || !vs || !os || !dos || !dqs ||
       !dks || !dvs)
     return fail(GKO_ERR_INVALID, "null pointer argument");
@@ -870,7 +1029,7 @@ extern "C" int gko_fmha_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64
       return fail(GKO_ERR_INVALID, "bias batch count %lld must divide the batch %lld", (long long)bias_batch,
                   (long long)z);
   }
-  const int64_t need = gko_fmha_bwd_workspace_size(z, hq, sq, d, 0);
+  const int64_t need = gko_fmha_sinks_bwd_workspace_size(z, hq, hkv, sq, sq, sk, d, causal, window, sinks, 0);
   if (!workspace || workspace_bytes < need || !host::aligned16(workspace))
     return fail(GKO_ERR_INVALID, "fmha backward needs a 16-byte aligned workspace of %lld bytes (got %lld)",
                 (long long)need, (long long)workspace_bytes);
@@ -894,7 +1053,12 @@ extern "C" int gko_fmha_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64
   p.scale_log2 = scale * fmha_bwd::kLog2e;
   p.softcap = softcap;
   p.causal = causal ? 1 : 0;
-  p.window = window;
+  p.window = window < fmha_bwd::kMaxWindow ? window : fmha_bwd::kMaxWindow;
+  p.sinks = window > 0 ? sinks : 0;
+  const fmha_bwd::SinkPlan sp = fmha_bwd::sink_plan(p.zh_kv, sq, sk, d, causal, window, sinks);
+  p.sink_tiles = sp.tiles;
+  p.pieces = sp.pieces;
+  p.piece = sp.piece;
   p.bias = bias;
   p.bias_mode = bias_mode;
   p.bias_dtype = bias_dtype;
@@ -911,6 +1075,7 @@ extern "C" int gko_fmha_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64
   p.dq_acc = ws;
   p.nl = ws + tiles * fmha_bwd::kBM * d;
   p.nd = p.nl + tiles * fmha_bwd::kBM;
+  p.parts = ws + tiles * (fmha_bwd::kBM * d + 2 * fmha_bwd::kBM);
   p.tiles_per_head = (sq + fmha_bwd::kBM - 1) / fmha_bwd::kBM;
   p.dk = dk;
   p.dk_sz = dks[0];
@@ -944,27 +1109,53 @@ extern "C" int gko_fmha_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64
   rp.dq_sh = dqs[1];
   rp.dq_ss = dqs[2];
   rp.scale = scale;
-  const bool extra = bias_mode != GKO_BIAS_NONE || softcap > 0.f || window > 0;
+  const int mode = fmha_bwd::mode_of(bias_mode != GKO_BIAS_NONE, softcap, window, p.sinks);
   const int q_blocks = (int)((sq + fmha_bwd::kBM - 1) / fmha_bwd::kBM);
   const int kv_tiles = (int)((sk + fmha_bwd::kBN - 1) / fmha_bwd::kBN);
-  return fmha_bwd::dispatch<false>(dtype, (int)d, tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, extra,
+  return fmha_bwd::dispatch<false>(dtype, (int)d, tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, mode,
                                    reinterpret_cast<cudaStream_t>(stream));
 }
 
-extern "C" int gko_fmha_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+extern "C" int gko_fmha_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk, int64_t d,
+                            const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v,
+                            const int64_t* vs, const void* bias, int bias_mode, int bias_dtype,
+                            const int64_t* bs, int64_t bias_batch, const void* out, const int64_t* os,
+                            const void* dout, const int64_t* dos, const float* lse, float scale, int causal,
+                            int window, float softcap, void* dq, const int64_t* dqs, void* dk,
+                            const int64_t* dks, void* dv, const int64_t* dvs, void* workspace,
+                            int64_t workspace_bytes, unsigned int* status, void* stream) {
+  return gko_fmha_sinks_bwd(dtype, z, hq, hkv, sq, sk, d, q, qs, k, ks, v, vs, bias, bias_mode, bias_dtype, bs,
+                            bias_batch, out, os, dout, dos, lse, scale, causal, window, softcap, 0, dq, dqs, dk, dks,
+                            dv, dvs, workspace, workspace_bytes, status, stream);
+}
+
+extern "C" int gko_fmha_sinks_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
                                    int64_t tk, int64_t max_seqlen_q, int64_t max_seqlen_k, const void* q,
                                    int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                                    const void* v, int64_t v_st, int64_t v_sh, const void* out, int64_t o_st,
                                    int64_t o_sh, const void* dout, int64_t do_st, int64_t do_sh, const float* lse,
                                    const int32_t* cu_q, const int32_t* cu_k, float scale, int causal, int window,
-                                   float softcap, void* dq, int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_st,
-                                   int64_t dk_sh, void* dv, int64_t dv_st, int64_t dv_sh, void* workspace,
-                                   int64_t workspace_bytes, unsigned int* status, void* stream) {
-  int rc = fmha_bwd::check_common(dtype, hq, hkv, d, scale, window, softcap);
+                                   float softcap, int sinks, void* dq, int64_t dq_st, int64_t dq_sh, void* dk,
+                                   int64_t dk_st, int64_t dk_sh, void* dv, int64_t dv_st, int64_t dv_sh,
+                                   void* workspace, int64_t workspace_bytes, unsigned int* status, void* stream) {
+  int rc = fmha_bwd::check_common(dtype, hq, hkv, d, scale, window, softcap, sinks);
   if (rc) return rc;
   if (b < 0 || tq < 0 || tk < 0 || max_seqlen_q < 0 || max_seqlen_k < 0)
     return fail(GKO_ERR_INVALID, "negative size");
   if (b == 0 || (tq == 0 && tk == 0)) return GKO_OK;
+  if (tk == 0) {  // no key to read or write: any mapped address will do
+    k = v = q;
+    dk = dv = dq;
+    k_st = v_st = q_st;
+    k_sh = v_sh = q_sh;
+  }
+  if (tq == 0) {  // no query likewise
+    q = out = dout = k;
+    dq = dk;
+    lse = static_cast<const float*>(k);
+    q_st = o_st = do_st = k_st;
+    q_sh = o_sh = do_sh = k_sh;
+  }
   if (!q || !k || !v || !out || !dout || !lse || !cu_q || !cu_k || !dq || !dk || !dv)
     return fail(GKO_ERR_INVALID, "null pointer argument");
   const int64_t st[12] = {q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, do_st, do_sh, dq_st, dq_sh};
@@ -976,7 +1167,8 @@ extern "C" int gko_fmha_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv
     if (!host::aligned16(ptr)) return fail(GKO_ERR_UNSUPPORTED, "fmha backward needs 16-byte aligned tensors");
   if (tq >= (1ll << 31) || tk >= (1ll << 31) || b * hq >= (1ll << 31))
     return fail(GKO_ERR_UNSUPPORTED, "too many tokens");
-  const int64_t need = gko_fmha_bwd_workspace_size(b, hq, tq, d, 1);
+  const int64_t need =
+      gko_fmha_sinks_bwd_workspace_size(b, hq, hkv, tq, max_seqlen_q, max_seqlen_k, d, causal, window, sinks, 1);
   if (!workspace || workspace_bytes < need || !host::aligned16(workspace))
     return fail(GKO_ERR_INVALID, "fmha backward needs a 16-byte aligned workspace of %lld bytes (got %lld)",
                 (long long)need, (long long)workspace_bytes);
@@ -998,12 +1190,18 @@ extern "C" int gko_fmha_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv
   p.scale_log2 = scale * fmha_bwd::kLog2e;
   p.softcap = softcap;
   p.causal = causal ? 1 : 0;
-  p.window = window;
+  p.window = window < fmha_bwd::kMaxWindow ? window : fmha_bwd::kMaxWindow;
+  p.sinks = window > 0 ? sinks : 0;
+  const fmha_bwd::SinkPlan sp = fmha_bwd::sink_plan(p.zh_kv, max_seqlen_q, max_seqlen_k, d, causal, window, sinks);
+  p.sink_tiles = sp.tiles;
+  p.pieces = sp.pieces;
+  p.piece = sp.piece;
   p.bias_mode = GKO_BIAS_NONE;
   p.bias_z = 1;
   p.dq_acc = ws;
   p.nl = ws + tiles * fmha_bwd::kBM * d;
   p.nd = p.nl + tiles * fmha_bwd::kBM;
+  p.parts = ws + tiles * (fmha_bwd::kBM * d + 2 * fmha_bwd::kBM);
   p.tiles_per_head = tiles / hq;
   p.dk = dk;
   p.dk_sh = dk_sh;
@@ -1037,11 +1235,26 @@ extern "C" int gko_fmha_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv
   rp.scale = scale;
   rp.cu_q = cu_q;
   rp.total_q = (int)tq;
-  const bool extra = softcap > 0.f || window > 0;
+  const int mode = fmha_bwd::mode_of(false, softcap, window, p.sinks);
   const int q_blocks = (int)((max_seqlen_q + fmha_bwd::kBM - 1) / fmha_bwd::kBM);
   const int kv_tiles = (int)((max_seqlen_k + fmha_bwd::kBN - 1) / fmha_bwd::kBN);
-  return fmha_bwd::dispatch<true>(dtype, (int)d, mq, mk, mv, mdo, p, rp, q_blocks, kv_tiles, extra,
+  return fmha_bwd::dispatch<true>(dtype, (int)d, mq, mk, mv, mdo, p, rp, q_blocks, kv_tiles, mode,
                                   reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int gko_fmha_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+                                   int64_t tk, int64_t max_seqlen_q, int64_t max_seqlen_k, const void* q,
+                                   int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                                   const void* v, int64_t v_st, int64_t v_sh, const void* out, int64_t o_st,
+                                   int64_t o_sh, const void* dout, int64_t do_st, int64_t do_sh, const float* lse,
+                                   const int32_t* cu_q, const int32_t* cu_k, float scale, int causal, int window,
+                                   float softcap, void* dq, int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_st,
+                                   int64_t dk_sh, void* dv, int64_t dv_st, int64_t dv_sh, void* workspace,
+                                   int64_t workspace_bytes, unsigned int* status, void* stream) {
+  return gko_fmha_sinks_varlen_bwd(dtype, b, hq, hkv, d, tq, tk, max_seqlen_q, max_seqlen_k, q, q_st, q_sh, k, k_st,
+                                   k_sh, v, v_st, v_sh, out, o_st, o_sh, dout, do_st, do_sh, lse, cu_q, cu_k, scale,
+                                   causal, window, softcap, 0, dq, dq_st, dq_sh, dk, dk_st, dk_sh, dv, dv_st, dv_sh,
+                                   workspace, workspace_bytes, status, stream);
 }
 
 // ------------------------------------------------------------------ allocation-free variant
@@ -1093,7 +1306,7 @@ extern "C" int gko_fmha_bwd_noalloc(int dtype, int64_t z, int64_t hq, int64_t hk
                                     const int64_t* dvs, unsigned int* status, void* stream) {
   // the same argument checks and empty-problem return as gko_fmha_bwd, before the scratch
   // size check and before the scratch address is looked up
-  int rc = fmha_bwd::check_common(dtype, hq, hkv, d, scale, window, softcap);
+  int rc = fmha_bwd::check_common(dtype, hq, hkv, d, scale, window, softcap, 0);
   if (rc) return rc;
   if (z < 0 || sq < 0 || sk < 0) return fail(GKO_ERR_INVALID, "negative attention size");
   if (z == 0 || (sq == 0 && sk == 0)) return GKO_OK;

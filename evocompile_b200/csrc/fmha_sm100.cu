@@ -45,6 +45,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleThreshold = 8.f;  // log2 units
+constexpr int kMaxWindow = (1 << 30) - 1024;  // wider ones hide nothing; position + window stays an int
 // K tiles are double or triple buffered (V always double): the S MMA of the next key tile
 // waits on K, so a deeper K ring hides more TMA latency when shared memory allows it.
 #ifndef GKO_FMHA_K_STAGES
@@ -63,7 +64,7 @@ struct Params {
   int q_tiles;         // 256-row query blocks along the query axis (grid.x)
   int zh;              // batch (or sequences) x query heads
   float scale, scale_log2, softcap;
-  int causal, window;
+  int causal, window, sinks;  // sinks: leading keys that the window does not hide (0 without a window)
   // bias (dense only)
   const void* bias;
   int bias_mode, bias_dtype, bias_z;  // batch index = z % bias_z
@@ -101,11 +102,18 @@ __device__ __forceinline__ float bias_value(const Params& p, int z, int h, int q
   return __half2float(__ldg(reinterpret_cast<const __half*>(p.bias) + off));
 }
 
-template <typename T, int D, bool VARLEN, bool EXTRA>
+// What the softmax of a kernel handles: kPlain an optional causal mask; kExtra also bias, softcap and
+// windows, element by element; kWindow a window with sinks and a positive scale, the scale folded into
+// the exponent as in kPlain and masks only on the key tiles that cross the edge of what a warp's rows
+// see.
+enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
+
+template <typename T, int D, bool VARLEN, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     fmha_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const Params p) {
   using L = Layout<D>;
+  constexpr bool EXTRA = MODE == kExtra;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = make_idesc_f16(kBF16, kBM, kBN, false, false);
   constexpr uint32_t kIdescO = make_idesc_f16(kBF16, kBM, D, false, true);
@@ -135,8 +143,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int hk = h / p.group;
   const int zc = VARLEN ? 0 : zb;  // tensor-map batch coordinate
 
-  // key-tile range [lo_t, hi_t) of each query tile (empty when the tile is past the end)
-  int lo_t[kQTiles], hi_t[kQTiles];
+  // Key tiles of each query tile: [0, sk_t) hold sinks (none but with sinks), then [lo_t, hi_t),
+  // lo_t >= sk_t (both empty when the tile is past the end). The causal bound cuts sk_t of the first
+  // query tile below that of the second only where it leaves the first nothing else, so the tiles of
+  // both together are [0, sk) and [lo, hi) with lo >= sk.
+  int lo_t[kQTiles], hi_t[kQTiles], sk_t[kQTiles];
 #pragma unroll
   for (int t = 0; t < kQTiles; ++t) {
     const int mt = m0 + t * kBM;
@@ -146,21 +157,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       k_lo = max(k_lo, mt - p.window);
       k_hi = min(k_hi, mt + kBM + p.window);
     }
+    sk_t[t] = 0;
     if (mt >= len_q || k_hi <= k_lo) {
       lo_t[t] = hi_t[t] = 0;
     } else {
       lo_t[t] = k_lo / kBN;
       hi_t[t] = (k_hi + kBN - 1) / kBN;
     }
+    if constexpr (MODE != kPlain) {
+      if (p.sinks > 0 && mt < len_q) {
+        const int end = min(min(p.sinks, len_k), p.causal ? mt + kBM : len_k);
+        sk_t[t] = (end + kBN - 1) / kBN;
+        lo_t[t] = max(lo_t[t], sk_t[t]);
+        hi_t[t] = max(hi_t[t], lo_t[t]);
+      }
+    }
   }
-  int lo = 1 << 30, hi = 0;
+  int lo = 1 << 30, hi = 0, sk = 0;
 #pragma unroll
-  for (int t = 0; t < kQTiles; ++t)
+  for (int t = 0; t < kQTiles; ++t) {
+    sk = max(sk, sk_t[t]);
     if (hi_t[t] > lo_t[t]) {
       lo = min(lo, lo_t[t]);
       hi = max(hi, hi_t[t]);
     }
-  const int n_tiles = hi > lo ? hi - lo : 0;
+  }
+  const int n_tiles = sk + (hi > lo ? hi - lo : 0);
+  // u-th key tile of the block; whether query tile t uses key tile j, and as its how manieth
+  auto tile_at = [&](int u) { return u < sk ? u : lo + u - sk; };
+  auto uses = [&](int t, int j) { return j < sk_t[t] || (j >= lo_t[t] && j < hi_t[t]); };
+  auto nth = [&](int t, int j) { return j < sk_t[t] ? j : sk_t[t] + j - lo_t[t]; };
 
   // ---------------------------------------------------------- shared memory
   extern __shared__ uint8_t smem_raw[];
@@ -235,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t ph = (u >> 1) & 1;
         const int ks = u % kKStages;
         const uint32_t kph = (u / kKStages) & 1;
-        const int krow = row_k0 + (lo + u) * kBN;
+        const int krow = row_k0 + tile_at(u) * kBN;
         if (!wait_bounded(bar_kempty + 8 * ks, kph ^ 1, abort_flag, p.status, kStatusTimeoutProducer))
           break;
         mbar_arrive_expect_tx(bar_kfull + 8 * ks, L::kTile);
@@ -286,11 +312,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
 #pragma unroll
         for (int t = 0; t < kQTiles; ++t)
-          if (lo >= lo_t[t] && lo < hi_t[t]) issue_s(t, 0);
+          if (uses(t, tile_at(0))) issue_s(t, 0);
         mma_commit(bar_kempty);
       }
       for (int u = 0; u < n_tiles && ok; ++u) {
-        const int j = lo + u;
+        const int j = tile_at(u), jn = tile_at(u + 1);
         const int st = u & 1;
         const uint32_t ph = (u >> 1) & 1;
         ok = wait_bounded(bar_vfull + 8 * st, ph, abort_flag, p.status, kStatusTimeoutMma);
@@ -305,20 +331,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
 #pragma unroll
         for (int t = 0; t < kQTiles && ok; ++t) {
-          if (j >= lo_t[t] && j < hi_t[t]) {
+          if (uses(t, j)) {
             // softmax hands P over in two halves, one barrier each
 #pragma unroll
             for (int half = 0; half < 2 && ok; ++half) {
-              ok = wait_bounded(bar_pfull + 16 * t + 8 * half, (j - lo_t[t]) & 1, abort_flag, p.status,
+              ok = wait_bounded(bar_pfull + 16 * t + 8 * half, nth(t, j) & 1, abort_flag, p.status,
                                 kStatusTimeoutMma);
               if (!ok) break;
               tc_fence_after();
-              issue_pv(t, u, j == lo_t[t], half);
+              issue_pv(t, u, nth(t, j) == 0, half);
             }
             if (!ok) break;
-            if (j == hi_t[t] - 1) mma_commit(bar_ofinal + 8 * t);
+            if (nth(t, j) == sk_t[t] + hi_t[t] - lo_t[t] - 1) mma_commit(bar_ofinal + 8 * t);
           }
-          if (next && j + 1 >= lo_t[t] && j + 1 < hi_t[t]) {
+          if (next && uses(t, jn)) {
             if (!k_ready) {
               ok = wait_bounded(bar_kfull + 8 * kn, knph, abort_flag, p.status, kStatusTimeoutMma);
               if (!ok) break;
@@ -353,14 +379,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_tmem = tmem_base + lane_off + t * kBN;
     const uint32_t o_tmem = tmem_base + lane_off + 256 + t * 128;
     const int jlo = t ? lo_t[1] : lo_t[0];
-    const int jhi = t ? hi_t[1] : hi_t[0];
+    const int jsk = t ? sk_t[1] : sk_t[0];
+    const int n_mine = jsk + (t ? hi_t[1] : hi_t[0]) - jlo;
     const int mt = m0 + t * kBM;
     float m_run = -INFINITY;  // running max, log2 domain
     float l_run = 0.f;
     bool ok = true;
-    for (int j = jlo; j < jhi; ++j) {
-      const int i = j - jlo;
-      const int kbase = j * kBN;
+    for (int i = 0; i < n_mine; ++i) {
+      const int kbase = (i < jsk ? i : jlo + i - jsk) * kBN;
       if (!wait_bounded(bar_sfull + 8 * t, i & 1, abort_flag, p.status, kStatusTimeoutSoftmax)) {
         ok = false;
         break;
@@ -388,10 +414,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (p.softcap > 0.f) x = p.softcap * tanhf(fminf(fmaxf(x / p.softcap, -15.f), 15.f));
           bool keep = kj < len_k;
           if (p.causal) keep = keep && (kj <= qi);
-          if (p.window > 0) keep = keep && (kj - qi <= p.window) && (qi - kj <= p.window);
+          if (p.window > 0) keep = keep && ((kj - qi <= p.window && qi - kj <= p.window) || kj < p.sinks);
           s[c] = keep ? x * kLog2e : -INFINITY;
         }
         kmul = 1.f;
+      } else if constexpr (MODE == kWindow) {
+        // row qi sees keys [qi - window, last] and [0, sink); the tile needs masks unless the first
+        // and the last row of the warp see all of it
+        const int rw = mt + quarter * 32;
+        const int last_w = min(len_k - 1, p.causal ? rw : rw + p.window);
+        const int sink_w = min(min(p.sinks, len_k), p.causal ? rw + 1 : len_k);
+        if (kbase + kBN > sink_w && (kbase + kBN - 1 > last_w || kbase < rw + 31 - p.window)) {
+          const int last = min(len_k - 1, p.causal ? qi : qi + p.window) - kbase;
+          const int sink = min(min(p.sinks, len_k), p.causal ? qi + 1 : len_k) - kbase;
+          // [first, last] as one unsigned comparison; an empty range starts past the tile
+          const int first = last >= qi - p.window - kbase ? qi - p.window - kbase : kBN;
+          const unsigned span = last >= first ? (unsigned)(last - first) : 0u;
+#pragma unroll
+          for (int c = 0; c < kBN; ++c)
+            s[c] = ((unsigned)(c - first) <= span || c < sink) ? s[c] : -INFINITY;
+        }
+        kmul = p.scale_log2;
       } else {
         const bool need_mask = (kbase + kBN > len_k) || (p.causal && kbase + kBN - 1 > mt);
         if (need_mask) {
@@ -465,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     // ---------------------------------------------------------- epilogue
-    const bool has = jhi > jlo;
+    const bool has = n_mine > 0;
     if (ok && has) {
       ok = wait_bounded(bar_ofinal + 8 * t, 0, abort_flag, p.status, kStatusTimeoutSoftmax);
       tc_fence_after();
@@ -517,10 +560,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------ host side
-template <typename T, int D, bool VARLEN, bool EXTRA>
+template <typename T, int D, bool VARLEN, int MODE>
 int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Params& p,
            dim3 grid, cudaStream_t s) {
-  auto kern = fmha_fwd_kernel<T, D, VARLEN, EXTRA>;
+  auto kern = fmha_fwd_kernel<T, D, VARLEN, MODE>;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -534,14 +577,28 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
   return host::cuda_check(cudaGetLastError(), "fmha kernel launch");
 }
 
+template <typename T, int D, bool VARLEN>
+int dispatch_mode(int mode, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Params& p,
+                  dim3 grid, cudaStream_t s) {
+  if (mode == kPlain) return launch<T, D, VARLEN, kPlain>(tq, tk, tv, p, grid, s);
+  if (mode == kWindow) return launch<T, D, VARLEN, kWindow>(tq, tk, tv, p, grid, s);
+  return launch<T, D, VARLEN, kExtra>(tq, tk, tv, p, grid, s);
+}
+
 template <typename T, bool VARLEN>
-int dispatch(int d, bool extra, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-             const Params& p, dim3 grid, cudaStream_t s) {
-  if (d == 64)
-    return extra ? launch<T, 64, VARLEN, true>(tq, tk, tv, p, grid, s)
-                 : launch<T, 64, VARLEN, false>(tq, tk, tv, p, grid, s);
-  return extra ? launch<T, 128, VARLEN, true>(tq, tk, tv, p, grid, s)
-               : launch<T, 128, VARLEN, false>(tq, tk, tv, p, grid, s);
+int dispatch(int d, int mode, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Params& p,
+             dim3 grid, cudaStream_t s) {
+  return d == 64 ? dispatch_mode<T, 64, VARLEN>(mode, tq, tk, tv, p, grid, s)
+                 : dispatch_mode<T, 128, VARLEN>(mode, tq, tk, tv, p, grid, s);
+}
+
+// Windows with sinks run on kWindow unless a bias, a softcap or a scale that is not positive (masked
+// scores are -inf before the scale is applied) needs kExtra; windows alone keep kExtra, whose results
+// they have always had.
+int mode_of(bool bias, float softcap, int window, int sinks, float scale) {
+  if (bias || softcap > 0.f) return kExtra;
+  if (window > 0) return sinks > 0 && scale > 0.f ? kWindow : kExtra;
+  return kPlain;
 }
 
 // Grid: query blocks along x, (batch, head) pairs along y (and z beyond 65535).
@@ -559,8 +616,9 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t z, int64_t h,
   return host::encode_tmap(m, dtype, 4, base, dims, str, box);
 }
 
-int check_common(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int window, float softcap) {
+int check_common(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int window, float softcap, int sinks) {
   using host::fail;
+  if (sinks < 0) return fail(GKO_ERR_INVALID, "sinks must be >= 0");
   if (dtype != GKO_F16 && dtype != GKO_BF16)
     return fail(GKO_ERR_UNSUPPORTED, "fmha supports float16 and bfloat16 only (dtype code %d)", dtype);
   if (d != 64 && d != 128)
@@ -580,17 +638,21 @@ int check_common(int dtype, int64_t hq, int64_t hkv, int64_t d, float scale, int
 using namespace gko;
 using gko::host::fail;
 
-extern "C" int gko_fmha_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk,
-                            int64_t d, const void* q, const int64_t* qs, const void* k,
-                            const int64_t* ks, const void* v, const int64_t* vs, const void* bias,
-                            int bias_mode, int bias_dtype, const int64_t* bs, int64_t bias_batch,
-                            const int64_t* os, float scale,
-                            int causal, int window, float softcap, void* out, float* lse,
-                            unsigned int* status, void* stream) {
-  int rc = fmha::check_common(dtype, hq, hkv, d, scale, window, softcap);
+extern "C" int gko_fmha_sinks_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk,
+                                  int64_t d, const void* q, const int64_t* qs, const void* k,
+                                  const int64_t* ks, const void* v, const int64_t* vs, const void* bias,
+                                  int bias_mode, int bias_dtype, const int64_t* bs, int64_t bias_batch,
+                                  const int64_t* os, float scale,
+                                  int causal, int window, float softcap, int sinks, void* out, float* lse,
+                                  unsigned int* status, void* stream) {
+  int rc = fmha::check_common(dtype, hq, hkv, d, scale, window, softcap, sinks);
   if (rc) return rc;
   if (z < 0 || sq < 0 || sk < 0) return fail(GKO_ERR_INVALID, "negative attention size");
   if (z == 0 || sq == 0) return GKO_OK;
+  if (sk == 0) {  // no key to read: any mapped address will do
+    k = v = q;
+    ks = vs = qs;
+  }
   if (!q || !k || !v || !out || !lse || !qs || !ks || !vs)
     return fail(GKO_ERR_INVALID, "null pointer argument");
   if (qs[3] != 1 || ks[3] != 1 || vs[3] != 1)
@@ -626,7 +688,8 @@ extern "C" int gko_fmha_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64
   p.scale_log2 = scale * fmha::kLog2e;
   p.softcap = softcap;
   p.causal = causal ? 1 : 0;
-  p.window = window;
+  p.window = window < fmha::kMaxWindow ? window : fmha::kMaxWindow;
+  p.sinks = window > 0 ? sinks : 0;
   p.bias = bias;
   p.bias_mode = bias_mode;
   p.bias_dtype = bias_dtype;
@@ -663,25 +726,41 @@ extern "C" int gko_fmha_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64
   p.lse = lse;
   p.lse_stride_h = sq;
   p.status = status;
-  const bool extra = bias_mode != GKO_BIAS_NONE || softcap > 0.f || window > 0;
+  const int mode = fmha::mode_of(bias_mode != GKO_BIAS_NONE, softcap, window, p.sinks, scale);
   p.zh = (int)(z * hq);
   const dim3 grid = fmha::grid_of(p.q_tiles, p.zh);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, false>((int)d, extra, tq, tk, tv, p, grid, s);
-  return fmha::dispatch<__half, false>((int)d, extra, tq, tk, tv, p, grid, s);
+  if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, false>((int)d, mode, tq, tk, tv, p, grid, s);
+  return fmha::dispatch<__half, false>((int)d, mode, tq, tk, tv, p, grid, s);
 }
 
-extern "C" int gko_fmha_varlen_fwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d,
-                                   int64_t tq, int64_t tk, int64_t max_seqlen_q, const void* q,
-                                   int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
-                                   int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
-                                   const int32_t* cu_q, const int32_t* cu_k, float scale, int causal,
-                                   int window, float softcap, void* out, float* lse,
-                                   unsigned int* status, void* stream) {
-  int rc = fmha::check_common(dtype, hq, hkv, d, scale, window, softcap);
+extern "C" int gko_fmha_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk,
+                            int64_t d, const void* q, const int64_t* qs, const void* k,
+                            const int64_t* ks, const void* v, const int64_t* vs, const void* bias,
+                            int bias_mode, int bias_dtype, const int64_t* bs, int64_t bias_batch,
+                            const int64_t* os, float scale,
+                            int causal, int window, float softcap, void* out, float* lse,
+                            unsigned int* status, void* stream) {
+  return gko_fmha_sinks_fwd(dtype, z, hq, hkv, sq, sk, d, q, qs, k, ks, v, vs, bias, bias_mode, bias_dtype, bs,
+                            bias_batch, os, scale, causal, window, softcap, 0, out, lse, status, stream);
+}
+
+extern "C" int gko_fmha_sinks_varlen_fwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d,
+                                         int64_t tq, int64_t tk, int64_t max_seqlen_q, const void* q,
+                                         int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                         int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                                         const int32_t* cu_q, const int32_t* cu_k, float scale, int causal,
+                                         int window, float softcap, int sinks, void* out, float* lse,
+                                         unsigned int* status, void* stream) {
+  int rc = fmha::check_common(dtype, hq, hkv, d, scale, window, softcap, sinks);
   if (rc) return rc;
   if (b < 0 || tq < 0 || tk < 0 || max_seqlen_q < 0) return fail(GKO_ERR_INVALID, "negative size");
   if (b == 0 || tq == 0 || max_seqlen_q == 0) return GKO_OK;
+  if (tk == 0) {  // no key to read: any mapped address will do
+    k = v = q;
+    k_st = v_st = q_st;
+    k_sh = v_sh = q_sh;
+  }
   if (!q || !k || !v || !out || !lse || !cu_q || !cu_k)
     return fail(GKO_ERR_INVALID, "null pointer argument");
   if (q_st % 8 || q_sh % 8 || k_st % 8 || k_sh % 8 || v_st % 8 || v_sh % 8)
@@ -704,7 +783,8 @@ extern "C" int gko_fmha_varlen_fwd(int dtype, int64_t b, int64_t hq, int64_t hkv
   p.scale_log2 = scale * fmha::kLog2e;
   p.softcap = softcap;
   p.causal = causal ? 1 : 0;
-  p.window = window;
+  p.window = window < fmha::kMaxWindow ? window : fmha::kMaxWindow;
+  p.sinks = window > 0 ? sinks : 0;
   p.bias_mode = GKO_BIAS_NONE;
   p.bias_z = 1;
   p.out = out;
@@ -714,10 +794,21 @@ extern "C" int gko_fmha_varlen_fwd(int dtype, int64_t b, int64_t hq, int64_t hkv
   p.cu_k = cu_k;
   p.total_q = (int)tq;
   p.status = status;
-  const bool extra = softcap > 0.f || window > 0;
+  const int mode = fmha::mode_of(false, softcap, window, p.sinks, scale);
   p.zh = (int)(b * hq);
   const dim3 grid = fmha::grid_of(p.q_tiles, p.zh);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, true>((int)d, extra, mq, mk, mv, p, grid, s);
-  return fmha::dispatch<__half, true>((int)d, extra, mq, mk, mv, p, grid, s);
+  if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, true>((int)d, mode, mq, mk, mv, p, grid, s);
+  return fmha::dispatch<__half, true>((int)d, mode, mq, mk, mv, p, grid, s);
+}
+
+extern "C" int gko_fmha_varlen_fwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d,
+                                   int64_t tq, int64_t tk, int64_t max_seqlen_q, const void* q,
+                                   int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                   int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                                   const int32_t* cu_q, const int32_t* cu_k, float scale, int causal,
+                                   int window, float softcap, void* out, float* lse,
+                                   unsigned int* status, void* stream) {
+  return gko_fmha_sinks_varlen_fwd(dtype, b, hq, hkv, d, tq, tk, max_seqlen_q, q, q_st, q_sh, k, k_st, k_sh, v, v_st,
+                                   v_sh, cu_q, cu_k, scale, causal, window, softcap, 0, out, lse, status, stream);
 }

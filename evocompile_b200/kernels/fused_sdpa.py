@@ -17,6 +17,9 @@ Drop-in for eval/kernels/fused_sdpa.py:
 
 * ``torch.ops.gko.fmha_varlen_bwd`` — its backward (autograd of
   ``fmha_varlen_fwd`` is registered).
+* ``torch.ops.gko.fmha_sinks_pair`` / ``fmha_sinks_bwd`` and ``fmha_sinks_varlen_fwd`` /
+  ``fmha_sinks_varlen_bwd`` — the dense and packed attention whose window leaves the first ``sinks``
+  keys visible (``fused_attention(..., window, sinks=n)``), with autograd (no reference counterpart).
 
 Additions over the reference Triton path: GQA (k/v with H/g heads) and varlen.
 Supported: float16/bfloat16, D in {64, 128}; anything else raises (there is no
@@ -41,16 +44,21 @@ def fused_sdpa_forward(q, k, v, attn_bias, scale, causal=0):
     return ops.fmha_fwd(q, k, v, attn_bias, float(scale), int(causal))[0]
 
 
-def fused_attention(q, k, v, attn_bias, scale, causal=0, window=0, softcap=0.0):
-    """Differentiable fused attention; Dynamo-safe (calls the custom op)."""
+def fused_attention(q, k, v, attn_bias, scale, causal=0, window=0, softcap=0.0, sinks=0):
+    """Differentiable fused attention; Dynamo-safe (calls the custom op). With a window, the first
+    ``sinks`` keys stay visible."""
     squeeze = q.dim() == 3
     if squeeze:
         q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
     if attn_bias is None:
         attn_bias = q.new_empty((0,))
     _ensure_op()
-    out, _ = torch.ops.gko.fused_sdpa_pair(q, k, v, attn_bias, float(scale), int(causal), int(window or 0),
-                                           float(softcap or 0.0))
+    if sinks and window:
+        out, _ = torch.ops.gko.fmha_sinks_pair(q, k, v, attn_bias, float(scale), int(causal), int(window),
+                                               float(softcap or 0.0), int(sinks))
+    else:
+        out, _ = torch.ops.gko.fused_sdpa_pair(q, k, v, attn_bias, float(scale), int(causal), int(window or 0),
+                                               float(softcap or 0.0))
     return out.squeeze(1) if squeeze else out
 
 
@@ -66,6 +74,30 @@ def _bwd_pair(ctx, dout, dlse):
     dq, dk, dv = torch.ops.gko.fused_sdpa_bwd(q, k, v, attn_bias, out, lse, dout, ctx.scale, ctx.causal,
                                                ctx.window, ctx.softcap)
     return dq, dk, dv, None, None, None, None, None
+
+
+def _setup_sinks(ctx, inputs, output):
+    _setup_pair(ctx, inputs[:8], output)
+    ctx.sinks = int(inputs[8])
+
+
+def _bwd_sinks(ctx, dout, dlse):
+    q, k, v, attn_bias, out, lse = ctx.saved_tensors
+    dq, dk, dv = torch.ops.gko.fmha_sinks_bwd(q, k, v, attn_bias, out, lse, dout, ctx.scale, ctx.causal, ctx.window,
+                                              ctx.softcap, ctx.sinks)
+    return dq, dk, dv, None, None, None, None, None, None
+
+
+def _setup_sinks_varlen(ctx, inputs, output):
+    _setup_varlen(ctx, inputs[:9], output)
+    ctx.window, ctx.softcap, ctx.sinks = int(inputs[9]), float(inputs[10]), int(inputs[11])
+
+
+def _bwd_sinks_varlen(ctx, dout, dlse):
+    q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+    dq, dk, dv = torch.ops.gko.fmha_sinks_varlen_bwd(q, k, v, out, lse, dout, cu_q, cu_k, ctx.max_q, ctx.max_k,
+                                                     ctx.scale, ctx.causal, ctx.window, ctx.softcap, ctx.sinks)
+    return (dq, dk, dv) + (None,) * 9
 
 
 def _setup_context(ctx, inputs, output):
@@ -173,6 +205,60 @@ def _ensure_op():
         except RuntimeError as e:
             if "already" not in str(e).lower():
                 raise
+
+        if not have("fmha_sinks_pair"):
+
+            @torch.library.custom_op("gko::fmha_sinks_pair", mutates_args=())
+            def fmha_sinks_pair(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, attn_bias: torch.Tensor,
+                                scale: float, causal: int, window: int, softcap: float, sinks: int
+                                ) -> Tuple[torch.Tensor, torch.Tensor]:
+                return ops.fmha_fwd(q, k, v, attn_bias, scale, causal, window, softcap, sinks=sinks)
+
+            @fmha_sinks_pair.register_fake
+            def _(q, k, v, attn_bias, scale, causal, window, softcap, sinks):
+                return q.new_empty(q.shape), q.new_empty((q.size(0) * q.size(1), q.size(2)), dtype=torch.float32)
+
+            @torch.library.custom_op("gko::fmha_sinks_bwd", mutates_args=())
+            def fmha_sinks_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, attn_bias: torch.Tensor,
+                               out: torch.Tensor, lse: torch.Tensor, dout: torch.Tensor, scale: float, causal: int,
+                               window: int, softcap: float, sinks: int
+                               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                return ops.fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale, causal, window, softcap, sinks)
+
+            @fmha_sinks_bwd.register_fake
+            def _(q, k, v, attn_bias, out, lse, dout, scale, causal, window, softcap, sinks):
+                return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+            fmha_sinks_pair.register_autograd(_bwd_sinks, setup_context=_setup_sinks)
+
+            @torch.library.custom_op("gko::fmha_sinks_varlen_fwd", mutates_args=())
+            def fmha_sinks_varlen_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                                      cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, scale: float,
+                                      causal: int, window: int, softcap: float, sinks: int
+                                      ) -> Tuple[torch.Tensor, torch.Tensor]:
+                return ops.fmha_varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale,
+                                           causal, window, softcap, sinks)
+
+            @fmha_sinks_varlen_fwd.register_fake
+            def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, window, softcap,
+                  sinks):
+                return q.new_empty(q.shape), q.new_empty((q.size(1), q.size(0)), dtype=torch.float32)
+
+            @torch.library.custom_op("gko::fmha_sinks_varlen_bwd", mutates_args=())
+            def fmha_sinks_varlen_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                                      lse: torch.Tensor, dout: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                                      cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, scale: float,
+                                      causal: int, window: int, softcap: float, sinks: int
+                                      ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                return ops.fmha_varlen_bwd(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
+                                           max_seqlen_k, scale, causal, window, softcap, sinks)
+
+            @fmha_sinks_varlen_bwd.register_fake
+            def _(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal,
+                  window, softcap, sinks):
+                return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+            fmha_sinks_varlen_fwd.register_autograd(_bwd_sinks_varlen, setup_context=_setup_sinks_varlen)
 
         _OP_READY = True
     if not _AUTOGRADED:

@@ -352,7 +352,7 @@ def _bias_layout(q, k, attn_bias):
     )
 
 
-def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.0, out=None):
+def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.0, out=None, sinks=0):
     """Fused attention forward -> (out [z, hq, sq, d], lse f32 [z * hq, sq]).
 
     ``out`` (optional) is a preallocated output with any strides allowed by the kernel (e.g. a
@@ -361,7 +361,8 @@ def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.
     q [z, hq, sq, d], k/v [z, hkv, sk, d] with hq % hkv == 0 (GQA); any
     strides with unit stride along d (e.g. [z, s, h, d] storage viewed through
     transpose(1, 2)) are read in place. Contract of gko::fused_sdpa_pair
-    (eval/kernels/fused_sdpa.py:912-943).
+    (eval/kernels/fused_sdpa.py:912-943). With a window, the first ``sinks`` keys stay visible to
+    every query (that the causal mask lets see them).
     """
     dev = _lib.require_cuda(q, k, v, attn_bias)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -390,12 +391,12 @@ def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.
     lse = torch.empty((z * hq, sq), device=dev, dtype=torch.float32)
     if z and hq and sq:
         with torch.cuda.device(dev):
-            rc = _lib.load().gko_fmha_fwd(
+            rc = _lib.load().gko_fmha_sinks_fwd(
                 dt, z, hq, hkv, sq, sk, d,
                 _ptr(q), _I64x4(*q.stride()), _ptr(k), _I64x4(*k.stride()), _ptr(v), _I64x4(*v.stride()),
                 _ptr(bias_t), mode, _lib.dtype_code(bias_t.dtype) if bias_t is not None else 0,
                 _I64x4(*bstr), nb, _I64x4(*out.stride()), float(scale), int(bool(causal)), int(window or 0),
-                float(softcap or 0.0),
+                float(softcap or 0.0), int(sinks or 0),
                 _ptr(out), _ptr(lse), _status_ptr(dev), _stream(dev),
             )
         _lib.check(rc, "gko_fmha_fwd")
@@ -403,8 +404,9 @@ def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.
 
 
 def fmha_varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k=None, scale=None,
-                    causal=0, window=0, softcap=0.0):
-    """Attention over packed sequences -> (out [tq, hq, d], lse f32 [hq, tq]).
+                    causal=0, window=0, softcap=0.0, sinks=0):
+    """Attention over packed sequences -> (out [tq, hq, d], lse f32 [hq, tq]). With a window, the first
+    ``sinks`` keys of each sequence stay visible.
 
     q [tq, hq, d], k/v [tk, hkv, d]; cu_seqlens_* int32 [b + 1] on the device, non-decreasing from 0 to the
     token count (not checked on the host, which would need a device sync; the kernel writes no row outside
@@ -439,11 +441,11 @@ def fmha_varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqle
     lse = torch.empty((hq, tq), device=dev, dtype=torch.float32)
     if b and tq and hq:
         with torch.cuda.device(dev):
-            rc = _lib.load().gko_fmha_varlen_fwd(
+            rc = _lib.load().gko_fmha_sinks_varlen_fwd(
                 _lib.dtype_code(q.dtype), b, hq, hkv, d, tq, tk, int(max_seqlen_q),
                 _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
                 v.stride(1), _ptr(cq), _ptr(ck), float(scale), int(bool(causal)), int(window or 0),
-                float(softcap or 0.0), _ptr(out), _ptr(lse), _status_ptr(dev), _stream(dev),
+                float(softcap or 0.0), int(sinks or 0), _ptr(out), _ptr(lse), _status_ptr(dev), _stream(dev),
             )
         _lib.check(rc, "gko_fmha_varlen_fwd")
     return out, lse
@@ -456,7 +458,7 @@ def _bwd_fix(t):
     return t
 
 
-def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0, softcap=0.0):
+def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0, softcap=0.0, sinks=0):
     """Fused attention backward -> (dq, dk, dv), contiguous, dtypes of q / k / v.
 
     Inputs as for ``fmha_fwd`` plus its ``out`` and ``lse`` and the incoming gradient ``dout``
@@ -487,17 +489,18 @@ def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0,
     dv = torch.empty((z, hkv, sk, d), device=dev, dtype=v.dtype)
     if z and hq and (sq or sk):
         lib = _lib.load()
-        ws_bytes = lib.gko_fmha_bwd_workspace_size(z, hq, sq, d, 0)
-        if ws_bytes < 0:
-            _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_bwd_workspace_size")
-        ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
         with torch.cuda.device(dev):
-            rc = lib.gko_fmha_bwd(
+            ws_bytes = lib.gko_fmha_sinks_bwd_workspace_size(z, hq, hkv, sq, sq, sk, d, int(bool(causal)),
+                                                             int(window or 0), int(sinks or 0), 0)
+            if ws_bytes < 0:
+                _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_bwd_workspace_size")
+            ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
+            rc = lib.gko_fmha_sinks_bwd(
                 dt, z, hq, hkv, sq, sk, d,
                 _ptr(q), _I64x4(*q.stride()), _ptr(k), _I64x4(*k.stride()), _ptr(v), _I64x4(*v.stride()),
                 _ptr(bias_t), mode, _lib.dtype_code(bias_t.dtype) if bias_t is not None else 0,
                 _I64x4(*bstr), nb, _ptr(out), _I64x4(*out.stride()), _ptr(dout), _I64x4(*dout.stride()),
-                _ptr(lse), float(scale), int(bool(causal)), int(window or 0), float(softcap or 0.0),
+                _ptr(lse), float(scale), int(bool(causal)), int(window or 0), float(softcap or 0.0), int(sinks or 0),
                 _ptr(dq), _I64x4(*dq.stride()), _ptr(dk), _I64x4(*dk.stride()), _ptr(dv), _I64x4(*dv.stride()),
                 _ptr(ws), ws_bytes, _status_ptr(dev), _stream(dev),
             )
@@ -506,7 +509,7 @@ def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0,
 
 
 def fmha_varlen_bwd(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale=None,
-                    causal=0, window=0, softcap=0.0):
+                    causal=0, window=0, softcap=0.0, sinks=0):
     """Backward of ``fmha_varlen_fwd`` -> (dq [tq, hq, d], dk, dv [tk, hkv, d]). cu_seqlens must be
     non-decreasing from 0 to the token counts, as for the forward; the kernels clamp every
     sequence's rows to [0, tq) / [0, tk), so malformed cu_seqlens give wrong gradients but no
@@ -538,17 +541,18 @@ def fmha_varlen_bwd(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seq
     dv = torch.empty((tk, hkv, d), device=dev, dtype=v.dtype)
     if b and hq and (tq or tk):
         lib = _lib.load()
-        ws_bytes = lib.gko_fmha_bwd_workspace_size(b, hq, tq, d, 1)
-        if ws_bytes < 0:
-            _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_bwd_workspace_size")
-        ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
         with torch.cuda.device(dev):
-            rc = lib.gko_fmha_varlen_bwd(
+            ws_bytes = lib.gko_fmha_sinks_bwd_workspace_size(b, hq, hkv, tq, int(max_seqlen_q), int(max_seqlen_k), d,
+                                                             int(bool(causal)), int(window or 0), int(sinks or 0), 1)
+            if ws_bytes < 0:
+                _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_bwd_workspace_size")
+            ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
+            rc = lib.gko_fmha_sinks_varlen_bwd(
                 _lib.dtype_code(q.dtype), b, hq, hkv, d, tq, tk, int(max_seqlen_q), int(max_seqlen_k),
                 _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
                 v.stride(1), _ptr(out), out.stride(0), out.stride(1), _ptr(dout), dout.stride(0), dout.stride(1),
                 _ptr(lse), _ptr(cq), _ptr(ck), float(scale), int(bool(causal)), int(window or 0),
-                float(softcap or 0.0), _ptr(dq), dq.stride(0), dq.stride(1), _ptr(dk), dk.stride(0), dk.stride(1),
+                float(softcap or 0.0), int(sinks or 0), _ptr(dq), dq.stride(0), dq.stride(1), _ptr(dk), dk.stride(0), dk.stride(1),
                 _ptr(dv), dv.stride(0), dv.stride(1), _ptr(ws), ws_bytes, _status_ptr(dev), _stream(dev),
             )
         _lib.check(rc, "gko_fmha_varlen_bwd")

@@ -231,6 +231,52 @@ int gko_fmha_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d
                         int64_t workspace_bytes, unsigned int* status, void* stream);
 
 /*
+ * Windowed attention with sinks: as gko_fmha_fwd, gko_fmha_varlen_fwd, gko_fmha_bwd and
+ * gko_fmha_varlen_bwd, where a window > 0 hides a key unless |key - query| <= window or key < sinks:
+ * the first `sinks` keys of every sequence stay visible (the causal mask still applies to them).
+ * sinks = 0, or no window, gives the plain entries' results. No reference counterpart: the
+ * reference's window has no sinks (eval/kernels/fused_sdpa.py:136-138). The backward entries'
+ * workspace is gko_fmha_sinks_bwd_workspace_size bytes (-1 for invalid sizes; dense: sq_or_tq =
+ * max_seqlen_q = sq, max_seqlen_k = sk, varlen = 0; packed: sq_or_tq = tq, varlen = 1); with several
+ * pieces per sink tile a fourth kernel adds their f32 parts of dk and dv in a fixed order.
+ */
+int gko_fmha_sinks_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk, int64_t d,
+                       const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, const void* bias, int bias_mode,
+                       int bias_dtype, const int64_t* bias_strides, int64_t bias_batch,
+                       const int64_t* out_strides, float scale, int causal, int window, float softcap,
+                       int sinks, void* out, float* lse, unsigned int* status, void* stream);
+int gko_fmha_sinks_varlen_fwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+                              int64_t tk, int64_t max_seqlen_q, const void* q, int64_t q_st,
+                              int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                              int64_t v_st, int64_t v_sh, const int32_t* cu_seqlens_q,
+                              const int32_t* cu_seqlens_k, float scale, int causal, int window,
+                              float softcap, int sinks, void* out, float* lse, unsigned int* status,
+                              void* stream);
+int64_t gko_fmha_sinks_bwd_workspace_size(int64_t batch, int64_t hq, int64_t hkv, int64_t sq_or_tq,
+                                          int64_t max_seqlen_q, int64_t max_seqlen_k, int64_t d, int causal,
+                                          int window, int sinks, int varlen);
+int gko_fmha_sinks_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk, int64_t d,
+                       const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                       const void* v, const int64_t* v_strides, const void* bias, int bias_mode,
+                       int bias_dtype, const int64_t* bias_strides, int64_t bias_batch, const void* out,
+                       const int64_t* out_strides, const void* dout, const int64_t* dout_strides,
+                       const float* lse, float scale, int causal, int window, float softcap, int sinks,
+                       void* dq, const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                       const int64_t* dv_strides, void* workspace, int64_t workspace_bytes,
+                       unsigned int* status, void* stream);
+int gko_fmha_sinks_varlen_bwd(int dtype, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+                              int64_t tk, int64_t max_seqlen_q, int64_t max_seqlen_k, const void* q,
+                              int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                              const void* v, int64_t v_st, int64_t v_sh, const void* out, int64_t o_st,
+                              int64_t o_sh, const void* dout, int64_t do_st, int64_t do_sh,
+                              const float* lse, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                              float scale, int causal, int window, float softcap, int sinks, void* dq,
+                              int64_t dq_st, int64_t dq_sh, void* dk, int64_t dk_st, int64_t dk_sh,
+                              void* dv, int64_t dv_st, int64_t dv_sh, void* workspace,
+                              int64_t workspace_bytes, unsigned int* status, void* stream);
+
+/*
  * Training forms of gko_addmm_act and gko_linear_swiglu that also write what the backward
  * needs, so it recomputes no GEMM (the reference backward re-runs the forward GEMM,
  * eval/kernels/addmm_gelu.py:175-185, eval/kernels/gemm_swiglu.py:177-200).

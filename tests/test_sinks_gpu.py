@@ -1,0 +1,258 @@
+"""Windowed attention with sinks on the GPU, forward and backward, dense and packed, against 64 bits.
+
+Tolerances, element by element, from the arithmetic (u: half a step of the element type, bf16 2^-8, f16 2^-11;
+`e`: the error of a logit, an f32 sum of d exact products, plus 2^-21 of its exponential):
+
+* out: each probability is rounded to the type (u p, or 2^-25 where f16 underflows), the sum once more;
+* delta = sum(out dout) inherits out's error; dS = P (dP - delta) is rounded to the type;
+* dq, dk, dv: sums of those with exact factors, rounded once;
+* every output has a last rounding of its own: f16 holds multiples of 2^-24 below 2^-14, so one that small is off
+  by up to 2^-25 whatever its size.
+"""
+
+import pytest
+import torch
+
+import oracle
+from evocompile_b200 import _lib, ops
+from evocompile_b200.kernels import fused_sdpa
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _status_clear():
+    torch.cuda.synchronize()
+    assert _lib.read_status(torch.device("cuda", 0)) == 0
+
+
+def _head(q, k, v, dout, scale, causal, window, softcap, sinks, bias, dtype):
+    """One (batch, head) in 64 bits: (out, lse, dq, dk, dv) and how far a kernel may be from each."""
+    u, d, n = U[dtype], q.shape[1], k.shape[0]
+    i, j = torch.arange(q.shape[0])[:, None], torch.arange(n)[None, :]
+    keep = oracle.visible(i, j, causal, window, sinks)
+    x = q @ k.T * scale + (0 if bias is None else bias)
+    g = torch.ones_like(x)
+    if softcap:
+        t = torch.tanh(x / softcap)
+        x, g = softcap * t, 1 - t * t
+    x = x.masked_fill(~keep, -float("inf"))
+    lse = torch.logsumexp(x, 1)
+    p = torch.where(x == -float("inf"), 0.0, torch.exp(x - torch.where(lse == -float("inf"), 0.0, lse)[:, None]))
+    out = p @ v
+    e = (d + 8) * 2.0 ** -24 * (abs(scale) * (q.abs() @ k.abs().T).amax() + (0 if bias is None else 4)) + 2.0 ** -20
+    tiny = n * 2.0 ** -25
+    t_out = u * (p @ v.abs()) + u * out.abs() + (2 * e + tiny) * v.abs().amax()
+    dp = dout @ v.T
+    delta = (out * dout).sum(1, keepdim=True)
+    ds = p * (dp - delta) * g
+    e_delta = (t_out * dout.abs()).sum(1, keepdim=True) + d * 2.0 ** -24 * (out * dout).abs().sum(1, keepdim=True)
+    e_ds = (u + 3 * e) * ds.abs() + p * (e_delta + d * 2.0 ** -24 * (dout.abs() @ v.abs().T)) + 2.0 ** -25 * (p > 0)
+    e_p = (u + 3 * e) * p + 2.0 ** -25 * (p > 0)
+    dq, dk, dv = scale * ds @ k, scale * ds.T @ q, p.T @ dout
+    t_dq = abs(scale) * e_ds @ k.abs() + u * dq.abs()
+    t_dk = abs(scale) * e_ds.T @ q.abs()
+    t_dv = e_p.T @ dout.abs()
+    return (out, lse, dq, dk, dv), (t_out, e + 2.0 ** -21 + 2.0 ** -22 * lse.abs(), t_dq, t_dk, t_dv)
+
+
+def _sequence(q, k, v, dout, scale, causal, window, softcap, sinks, dtype, bias=None):
+    """One sequence, [h, s, d] each: results and tolerances, shared heads' gradients summed."""
+    hq, hkv = q.shape[0], k.shape[0]
+    got = [_head(q[h], k[h // (hq // hkv)], v[h // (hq // hkv)], dout[h], scale, causal, window, softcap, sinks,
+                 None if bias is None else bias[h], dtype) for h in range(hq)]
+    full = []
+    for part in (0, 1):
+        o, l, dq, dk, dv = (torch.stack([x[part][n] for x in got]) for n in range(5))
+        full.append([o, l, dq, dk.view(hkv, -1, *dk.shape[1:]).sum(1), dv.view(hkv, -1, *dv.shape[1:]).sum(1)])
+    for n in (3, 4):
+        full[1][n] = full[1][n] + U[dtype] * full[0][n].abs()
+    return full
+
+
+def _near(name, got, want, tol):
+    got = got.detach().cpu().double()
+    assert torch.equal(got == -float("inf"), want == -float("inf")), name
+    fin = want != -float("inf")
+    over = ((got - want).abs() / (tol + 2.0 ** -25))[fin]
+    assert not (over > 1).any(), (name, over.max())
+
+
+def _qkv(seed, z, hq, hkv, sq, sk, d, dtype):
+    """[z, s, h, d] storage seen as [z, h, s, d]."""
+    g = torch.Generator().manual_seed(seed)
+    make = lambda s, h: torch.randn(z, s, h, d, generator=g).to(dtype).transpose(1, 2)  # noqa: E731
+    return make(sq, hq), make(sk, hkv), make(sk, hkv), make(sq, hq)
+
+
+def _dev(t):
+    return t.transpose(1, 2).contiguous().cuda().transpose(1, 2)
+
+
+def _run(seed, z, hq, hkv, sq, sk, d, dtype, causal, window, sinks, softcap=0.0, bias=None, scale=None):
+    q, k, v, dout = _qkv(seed, z, hq, hkv, sq, sk, d, dtype)
+    scale = d ** -0.5 if scale is None else scale
+    dev = [_dev(t) for t in (q, k, v, dout)]
+    b = None if bias is None else bias.cuda()
+    out, lse = ops.fmha_fwd(*dev[:3], b, scale, causal, window, softcap, sinks=sinks)
+    grads = ops.fmha_bwd(*dev[:3], b, out, lse, dev[3], scale, causal, window, softcap, sinks)
+    _status_clear()
+    for i in range(z):
+        want, tol = _sequence(*(t[i].double() for t in (q, k, v, dout)), scale, causal, window, softcap, sinks, dtype,
+                              None if bias is None else bias[i].double().expand(hq, sq, sk))
+        for name, x, w, t in zip(("out", "lse", "dq", "dk", "dv"), (out[i], lse.view(z, hq, sq)[i], *(g[i] for g in grads)),
+                                 want, tol):
+            _near(name, x, w, t)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("s,window,sinks", [(1, 1, 1), (63, 5, 2), (257, 100, 1), (600, 64, 4), (513, 128, 130), (700, 1, 300)])
+def test_causal(dtype, d, s, window, sinks):
+    _run(s + d, 1, 2, 2, s, s, d, dtype, 1, window, sinks)
+
+
+@pytest.mark.parametrize("sq,sk,causal", [(300, 900, 0), (900, 300, 1), (900, 300, 0), (520, 520, 0), (5, 700, 1), (700, 3, 1)])
+@pytest.mark.parametrize("window,sinks", [(40, 3), (129, 140), (2000, 5)])
+def test_both_ways_and_cross_lengths(sq, sk, causal, window, sinks):
+    _run(sq + sk + window, 1, 2, 1, sq, sk, 128, torch.bfloat16, causal, window, sinks)
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (6, 1), (3, 3)])
+def test_shared_heads_and_batches(hq, hkv):
+    _run(hq, 3, hq, hkv, 333, 333, 64, torch.float16, 1, 50, 7)
+
+
+def test_many_pieces():
+    """A sink tile whose queries are shared by many CTAs; the second sink tile starts later when causal."""
+    _run(1, 1, 1, 1, 4000, 4000, 64, torch.bfloat16, 1, 16, 200)
+    _run(2, 1, 2, 1, 2500, 2000, 128, torch.float16, 0, 16, 1)
+
+
+@pytest.mark.parametrize("kind", ["softcap", "keypad", "full", "negative_scale", "zero_scale"])
+def test_general_path(kind):
+    """Bias, softcap and scales that are not positive, together with window and sinks."""
+    g = torch.Generator().manual_seed(4)
+    s, bias, softcap, scale = 300, None, 0.0, None
+    if kind == "softcap":
+        softcap = 4.0
+    elif kind == "keypad":  # the first sequence's sinks and the keys near its first rows are padding: empty rows
+        bias = torch.zeros(2, 1, 1, s)
+        bias[0, ..., :120] = -float("inf")
+        bias[1, ..., 250:] = torch.finfo(torch.bfloat16).min
+    elif kind == "full":
+        bias = torch.randn(2, 1, s, s, generator=g)
+    else:
+        scale = -0.1 if kind == "negative_scale" else 0.0
+    _run(7, 2, 2, 2, s, s, 64, torch.bfloat16, 1, 60, 5, softcap, bias, scale)
+
+
+def test_no_keys():
+    """No key at all: zeros and -inf, and zero gradients of the queries."""
+    q = torch.randn(1, 2, 9, 64, device="cuda", dtype=torch.bfloat16)
+    k = q.new_empty(1, 2, 0, 64)
+    out, lse = ops.fmha_fwd(q, k, k, None, 0.1, 1, 4, sinks=2)
+    dq, dk, dv = ops.fmha_bwd(q, k, k, None, out, lse, q, 0.1, 1, 4, 0.0, 2)
+    _status_clear()
+    assert not out.any() and (lse == -float("inf")).all() and not dq.any() and dk.numel() == dv.numel() == 0
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv,window,sinks", [(torch.bfloat16, 128, 4, 1, 100, 4), (torch.float16, 64, 2, 2, 30, 150)])
+def test_packed(dtype, d, hq, hkv, window, sinks):
+    """Packed sequences, empty ones among them, through the custom op and its gradient; a tail behind them."""
+    lens = [1, 0, 700, 64, 129, 0, 5]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    t = cu[-1] + 3
+    g = torch.Generator().manual_seed(d)
+    make = lambda h: torch.randn(t, h, d, generator=g).to(dtype)  # noqa: E731
+    q, k, v, dout = make(hq), make(hkv), make(hkv), make(hq)
+    dev = [x.cuda().requires_grad_(True) for x in (q, k, v)]
+    c = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    fused_sdpa.register()
+    out, lse = torch.ops.gko.fmha_sinks_varlen_fwd(*dev, c, c, 700, 700, d ** -0.5, 1, window, 0.0, sinks)
+    grads = torch.autograd.grad(out, dev, dout.cuda())
+    _status_clear()
+    for a, e in zip(cu[:-1], cu[1:]):
+        if a == e:
+            continue
+        want, tol = _sequence(*(x[a:e].transpose(0, 1).double() for x in (q, k, v, dout)), d ** -0.5, 1, window, 0.0, sinks,
+                              dtype)
+        got = [out[a:e].transpose(0, 1), lse[:, a:e], *(x[a:e].transpose(0, 1) for x in grads)]
+        for name, x, w, m in zip(("out", "lse", "dq", "dk", "dv"), got, want, tol):
+            _near(name, x, w, m)
+
+
+def test_autograd_and_window_off():
+    """fused_attention's gradients are the backward's; sinks without a window change nothing."""
+    q, k, v, dout = (_dev(t) for t in _qkv(5, 2, 4, 2, 200, 200, 64, torch.bfloat16))
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = fused_sdpa.fused_attention(*leaves, None, 0.125, 1, 30, sinks=3)
+    grads = torch.autograd.grad(out, leaves, dout)
+    o, lse = ops.fmha_fwd(q, k, v, None, 0.125, 1, 30, sinks=3)
+    direct = ops.fmha_bwd(q, k, v, None, o, lse, dout, 0.125, 1, 30, 0.0, 3)
+    assert torch.equal(out, o)
+    assert all(torch.equal(a, b) for a, b in zip(grads[1:], direct[1:]))  # dq adds in f32 in no fixed order
+    assert (grads[0] - direct[0]).abs().max() <= 2 ** -7 * direct[0].abs().max()
+    plain = ops.fmha_fwd(q, k, v, None, 0.125, 1)
+    assert all(torch.equal(a, b) for a, b in zip(ops.fmha_fwd(q, k, v, None, 0.125, 1, sinks=9), plain))
+    assert torch.equal(fused_sdpa.fused_attention(q, k, v, None, 0.125, 1, sinks=9), plain[0])
+    _status_clear()
+
+
+def test_gradient_by_differences():
+    """Along a random direction, the gradients predict how sum(out * dout) moves, computed in 64 bits."""
+    q, k, v, dout = _qkv(6, 1, 2, 1, 150, 150, 64, torch.float16)
+    dev = [_dev(t) for t in (q, k, v, dout)]
+    out, lse = ops.fmha_fwd(*dev[:3], None, 0.125, 1, 20, sinks=2)
+    grads = ops.fmha_bwd(*dev[:3], None, out, lse, dev[3], 0.125, 1, 20, 0.0, 2)
+    g = torch.Generator().manual_seed(1)
+    step = [torch.randn(t.shape, generator=g).double() for t in (q, k, v)]
+    h = 1e-5
+
+    def value(sign):
+        x = [t[0].transpose(0, 1).double() + sign * h * s[0].transpose(0, 1) for t, s in zip((q, k, v), step)]
+        return (oracle.attention64(*x, 0.125, 1, 20, 0.0, 2)[0] * dout[0].transpose(0, 1).double()).sum()
+
+    moved = (value(1) - value(-1)) / (2 * h)
+    told = sum((a.cpu().double() * s).sum() for a, s in zip(grads, step))
+    # every gradient element is off by a few u of terms its own size; independent signs add as a root of squares
+    spread = sum(((a.cpu().double() * s) ** 2).sum() for a, s in zip(grads, step)).sqrt()
+    assert (moved - told).abs() <= 16 * U[torch.float16] * spread
+
+
+def test_captured_backward():
+    """Forward and backward captured into a graph and replayed on other values equal the eager calls."""
+    q, k, v, dout = (_dev(t) for t in _qkv(8, 1, 4, 2, 300, 300, 64, torch.bfloat16))
+
+    def step():
+        o, lse = ops.fmha_fwd(q, k, v, None, 0.125, 1, 40, sinks=4)
+        return o, ops.fmha_bwd(q, k, v, None, o, lse, dout, 0.125, 1, 40, 0.0, 4)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out, grads = step()
+    for t, n in zip((q, k, v, dout), _qkv(9, 1, 4, 2, 300, 300, 64, torch.bfloat16)):
+        t.copy_(n)
+    graph.replay()
+    torch.cuda.synchronize()
+    o, direct = step()
+    _status_clear()
+    assert torch.equal(out, o) and torch.equal(grads[1], direct[1]) and torch.equal(grads[2], direct[2])
+
+
+def test_refusals():
+    q = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="sinks"):
+        ops.fmha_fwd(q, q, q, None, 0.1, 1, 4, sinks=-1)
+    out, lse = ops.fmha_fwd(q, q, q, None, 0.1, 1, 4, sinks=1)
+    with pytest.raises(RuntimeError, match="workspace_size|sinks"):
+        ops.fmha_bwd(q, q, q, None, out, lse, q, 0.1, 1, 4, 0.0, -1)
+    with pytest.raises(RuntimeError, match="window"):
+        ops.fmha_fwd(q, q, q, None, 0.1, 1, -4, sinks=1)
