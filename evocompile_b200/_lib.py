@@ -209,7 +209,24 @@ def read_status(device: torch.device, clear: bool = True) -> int:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of torch's current stream on ``device`` (without building a Stream object: 0.1 us, not 2)."""
+    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else torch.cuda.current_device())
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is current; costs nothing where it already is."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def require_cuda(*ts: torch.Tensor) -> torch.device:

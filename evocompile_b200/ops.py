@@ -18,16 +18,17 @@ from . import _lib
 _I64x4 = ctypes.c_int64 * 4
 
 
+# Addresses go to the library as plain integers (its arguments are declared void pointers); None is NULL.
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+    return t.data_ptr() if t is not None else None
 
 
 def _status_ptr(dev):
-    return ctypes.c_void_p(_lib.status_word(dev).data_ptr())
+    return _lib.status_word(dev).data_ptr()
 
 
 def _stream(dev):
-    return ctypes.c_void_p(_lib.stream_ptr(dev))
+    return _lib.stream_ptr(dev)
 
 
 def _byte_range(t):
@@ -123,7 +124,7 @@ def addmm_act(bias, mat1, mat2, act: int = _lib.ACT_GELU, save_pre: bool = False
         _check_no_overlap("addmm_act", out, mat1=mat1, mat2=mat2)
     z = torch.empty((M, N), device=dev, dtype=mat1.dtype) if save_pre else None
     if M and N:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             a_sm = a.stride(0) if M > 1 else max(K, 8)
             a_sk = a.stride(1)
             if a_mn and K == 1:
@@ -179,7 +180,7 @@ def linear_swiglu(x, weight, save_pre: bool = False):
     out = torch.empty((M, H), device=dev, dtype=x.dtype)
     gu = torch.empty((M, 2 * H), device=dev, dtype=x.dtype) if save_pre else None
     if M and H:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             a_sm = a.stride(0) if M > 1 else max(D, 8)
             if save_pre:
                 rc = _lib.load().gko_linear_swiglu_aux(
@@ -207,7 +208,7 @@ def swiglu_bwd(dy, gate_up):
     g2 = gate_up.reshape(-1, 2 * H).contiguous()
     out = torch.empty_like(g2)
     if d2.shape[0] and H:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_swiglu_bwd(
                 _lib.dtype_code(dy.dtype), d2.shape[0], H, _ptr(d2), d2.stride(0), _ptr(g2), g2.stride(0),
                 _ptr(out), out.stride(0), _status_ptr(dev), _stream(dev),
@@ -235,7 +236,7 @@ def silu_mul(x, y):
     out = torch.empty_like(xc)
     n = xc.numel()
     if n:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_silu_mul(
                 _lib.dtype_code(x.dtype), n, _ptr(xc), _ptr(yc), _ptr(out), _status_ptr(dev), _stream(dev)
             )
@@ -267,7 +268,7 @@ def rmsnorm(x, weight, eps=1e-5, residual=None, return_sum=False):
     total = torch.empty(x2.shape, device=dev, dtype=x.dtype) if (return_sum and r2 is not None) else None
     w = weight.contiguous()
     if x2.shape[0]:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_rmsnorm(
                 _lib.dtype_code(x.dtype), x2.shape[0], cols, _ptr(x2), _ptr(r2), _ptr(w), float(eps), _ptr(out),
                 _ptr(total), cols, _status_ptr(dev), _stream(dev),
@@ -294,7 +295,7 @@ def rope_(x, theta=500000.0, positions=None, seq_len=None):
     if pos is None and not seq_len:
         seq_len = t
     if t and h:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_rope(
                 _lib.dtype_code(x.dtype), t, h, d, _ptr(x), x.stride(0), x.stride(1), _ptr(pos),
                 int(seq_len or 0), float(theta), _status_ptr(dev), _stream(dev),
@@ -390,7 +391,7 @@ def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.
         raise RuntimeError(f"fmha: out must be [{z}, {hq}, {sq}, {d}] {q.dtype} on {dev}")
     lse = torch.empty((z * hq, sq), device=dev, dtype=torch.float32)
     if z and hq and sq:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_fmha_sinks_fwd(
                 dt, z, hq, hkv, sq, sk, d,
                 _ptr(q), _I64x4(*q.stride()), _ptr(k), _I64x4(*k.stride()), _ptr(v), _I64x4(*v.stride()),
@@ -440,7 +441,7 @@ def fmha_varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqle
     out = torch.empty((tq, hq, d), device=dev, dtype=q.dtype)
     lse = torch.empty((hq, tq), device=dev, dtype=torch.float32)
     if b and tq and hq:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_fmha_sinks_varlen_fwd(
                 _lib.dtype_code(q.dtype), b, hq, hkv, d, tq, tk, int(max_seqlen_q),
                 _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
@@ -489,7 +490,7 @@ def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0,
     dv = torch.empty((z, hkv, sk, d), device=dev, dtype=v.dtype)
     if z and hq and (sq or sk):
         lib = _lib.load()
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             ws_bytes = lib.gko_fmha_sinks_bwd_workspace_size(z, hq, hkv, sq, sq, sk, d, int(bool(causal)),
                                                              int(window or 0), int(sinks or 0), 0)
             if ws_bytes < 0:
@@ -541,7 +542,7 @@ def fmha_varlen_bwd(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seq
     dv = torch.empty((tk, hkv, d), device=dev, dtype=v.dtype)
     if b and hq and (tq or tk):
         lib = _lib.load()
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             ws_bytes = lib.gko_fmha_sinks_bwd_workspace_size(b, hq, hkv, tq, int(max_seqlen_q), int(max_seqlen_k), d,
                                                              int(bool(causal)), int(window or 0), int(sinks or 0), 1)
             if ws_bytes < 0:
@@ -592,8 +593,6 @@ def kv_cache_alloc(pages, page_size, kv_heads, head_dim, bits=4, dtype=torch.bfl
 
 def _cache_layout(name, cache, hkv=None, d=None, dtype=None):
     """(dtype code, bits, kv heads, d) of a cache whose four tensors fit together and, where given, k and v."""
-    if len(cache) != 4:
-        raise RuntimeError(f"{name}: a cache is (k_codes, v_codes, k_pairs, v_pairs)")
     kc, vc, kp, vp = cache
     if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or kc.dim() != 4 or kc.shape != vc.shape:
         raise RuntimeError(f"{name}: codes must be two uint8 [pages, kv heads, page, bytes] tensors of one shape")
@@ -635,7 +634,7 @@ def kv_cache_write(k, v, cache, slots):
         raise RuntimeError(f"kv_cache_write: slots must be int64 [{t}], got {slots.dtype} {tuple(slots.shape)}")
     k, v = _bwd_fix(k), _bwd_fix(v)
     slots = slots.contiguous()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = _lib.load().gko_kv_cache_write(
             dt, bits, t, hkv, d, _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(slots),
             _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), kc.shape[0], kc.shape[2], _status_ptr(dev), _stream(dev),
@@ -675,7 +674,7 @@ def kv_cache_read(cache, block_table, cu_seqlens, tokens, head_dim, out=None):
         if t.shape != (tokens, hkv, d) or t.dtype != kp.dtype or not t.is_contiguous():
             raise RuntimeError(f"kv_cache_read: out must be two contiguous [{tokens}, {hkv}, {d}] {kp.dtype} tensors")
     cu_seqlens = cu_seqlens.contiguous()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = _lib.load().gko_kv_cache_read(
             dt, bits, b, hkv, d, tokens, _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), pages, page_size, _ptr(block_table),
             block_table.stride(0), block_table.shape[1], _ptr(cu_seqlens), _ptr(out[0]), _ptr(out[1]),
@@ -731,7 +730,7 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
     lse = torch.empty((hq, tq), device=dev, dtype=torch.float32)
     seq_lens = seq_lens.contiguous()
     lib = _lib.load()
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         ws_bytes = lib.gko_fmha_cache_workspace_size(b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k),
                                                      int(window or 0), int(sinks or 0))
         if ws_bytes < 0:
@@ -772,7 +771,7 @@ def linear_allreduce(x, weight, out, multicast_ptr: int, peers_dev_ptr: int, wor
     if weight.stride(1) != 1:
         weight = weight.contiguous()
     if m and n:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_linear_allreduce(
                 _lib.dtype_code(x.dtype), m, n, k, _ptr(x), x.stride(0), 1, _ptr(weight), weight.stride(0), 1,
                 _ptr(out), out.stride(0), ctypes.c_void_p(multicast_ptr or 0), ctypes.c_void_p(peers_dev_ptr or 0),
@@ -812,7 +811,7 @@ def linear_residual(x, weight, resid, out=None):
     if resid.stride(1) != 1:
         resid = resid.contiguous()
     if m and n:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_linear_residual(
                 _lib.dtype_code(x.dtype), m, n, k, _ptr(x), x.stride(0), 1, _ptr(weight), weight.stride(0), 1,
                 _ptr(resid), resid.stride(0), _ptr(out), out.stride(0), _status_ptr(dev), _stream(dev),
@@ -832,7 +831,7 @@ def rms_stats(x, eps=1e-5, residual=None):
     inv = torch.empty(x2.shape[0], device=dev, dtype=torch.float32)
     total = torch.empty(x2.shape, device=dev, dtype=x.dtype) if r2 is not None else None
     if x2.shape[0]:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_rms_stats(
                 _lib.dtype_code(x.dtype), x2.shape[0], cols, _ptr(x2), _ptr(r2), float(eps), _ptr(total), _ptr(inv),
                 cols, _status_ptr(dev), _stream(dev),
@@ -879,7 +878,7 @@ def linear_rowscale(x, weight, row_scale, swiglu: bool = False, rope=None):
             raise RuntimeError("linear_rowscale: RoPE applies to the plain (non-SwiGLU) projection only")
         rope_cols, seq_len, theta = rope
         if m and n:
-            with torch.cuda.device(dev):
+            with _lib.on_device(dev):
                 rc = _lib.load().gko_linear_rowscale_rope(
                     _lib.dtype_code(x.dtype), m, n, k, _ptr(x), x.stride(0), 1, _ptr(weight), weight.stride(0), 1,
                     _ptr(row_scale), _ptr(out), out.stride(0), int(rope_cols), int(seq_len), float(theta),
@@ -888,7 +887,7 @@ def linear_rowscale(x, weight, row_scale, swiglu: bool = False, rope=None):
             _lib.check(rc, "gko_linear_rowscale_rope")
         return out
     if m and n:
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             rc = _lib.load().gko_linear_rowscale(
                 _lib.dtype_code(x.dtype), int(bool(swiglu)), m, n, k, _ptr(x), x.stride(0), 1, _ptr(weight),
                 weight.stride(0), 1, _ptr(row_scale), _ptr(out), out.stride(0), _status_ptr(dev), _stream(dev),
