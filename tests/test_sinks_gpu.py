@@ -247,6 +247,23 @@ def test_captured_backward():
     assert torch.equal(out, o) and torch.equal(grads[1], direct[1]) and torch.equal(grads[2], direct[2])
 
 
+def test_new_host_thread():
+    """The first CUDA call of a host thread may be one of these (autograd's thread when nothing is copied)."""
+    import threading
+
+    q = torch.randn(1, 2, 64, 64, dtype=torch.bfloat16, device="cuda")
+    want = ops.fmha_fwd(q, q, q, None, 0.1, 1, 4, sinks=1)
+    got = []
+    t = threading.Thread(target=lambda: got.append(ops.fmha_fwd(q, q, q, None, 0.1, 1, 4, sinks=1, out=torch.empty_like(q))))
+    t.start()
+    t.join()
+    assert torch.equal(got[0][0], want[0])
+    leaf = q.detach().requires_grad_(True)
+    out = fused_sdpa.fused_attention(leaf, q, q, None, 0.1, 1, 4, sinks=1)
+    assert torch.autograd.grad(out, leaf, torch.ones_like(out))[0].isfinite().all()
+    _status_clear()
+
+
 def test_refusals():
     q = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="sinks"):
