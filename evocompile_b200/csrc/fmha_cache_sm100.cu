@@ -17,6 +17,9 @@
 // Columns of a CTA are (new token, query head) pairs of one kv head, kCols at a time. A CTA takes
 // one range of keys (grid.x: column tile, then split); its warps take slabs of 32 keys in turn,
 // each with its own running maximum, sum and accumulators, and join at the end in a fixed order.
+// Every warp keeps a ring of slabs in flight for itself (bulk copies of codes and pairs into shared
+// memory, completing on an mbarrier of the warp), so the loop has no barrier between warps and the
+// memory system always has several slabs per warp to work on.
 // With more than one split the joined parts go to the workspace and a second kernel adds them,
 // again in a fixed order, so results do not vary from run to run.
 #include "host_common.h"
@@ -43,7 +46,7 @@ struct Params {
   const uint32_t* k_pairs;
   const uint32_t* v_pairs;
   int64_t pages;
-  int page_size;
+  int page_size, page_shift;  // page_shift: log2 of the page size, -1 when it is not a power of two
   const int32_t* table;
   int64_t table_stride;
   int table_width;
@@ -177,19 +180,36 @@ struct Row {
   static constexpr int kKWords = kBytes / 16;  // a lane's share of a key row: a quarter, D / 4 channels
   static constexpr int kVWords = kBytes / 32;  // a lane's share of a value row: an eighth, D / 8 channels
   static constexpr int kSteps = D / 16;        // m16n8k16 steps over the channels of S; m-tiles of O
+  // one slab of the ring: codes of K, of V, pairs of K, of V
+  static constexpr int kV = kSlab * kBytes;
+  static constexpr int kKP = 2 * kSlab * kBytes;
+  static constexpr int kVP = kKP + kSlab * 4;
+  static constexpr int kStage = kVP + kSlab * 4;
+  static constexpr int kStages = kStage > 8192 ? 2 : 3;
+  static constexpr int kRing = kWarps * kStages * kStage;
 };
 
-// Channel (0 .. D/4 - 1, within the lane's share) of element e (0, 1: low / high half) of pair
-// `pr` (0, 1) of step s of S: the order in which the unpacking above meets a row's codes.
-template <int BITS>
-__device__ __forceinline__ int k_channel(int s, int pr, int e) {
-  if (BITS == 4) return (s >> 1) * 8 + (s & 1) * 2 + pr + 4 * e;
-  return s * 4 + pr * 2 + e;
+// Key rows of 16 of a half slab go to the operand's rows in this order: neighbours swap places in
+// every other pair, so that the value rows 2i of the four lanes that share a channel lie in both
+// halves of the shared-memory banks when rows are 64 bytes.
+__device__ __forceinline__ int key_of(int row) { return row ^ ((row >> 1) & 1); }
+
+// A lane's share of a key row is 16 bytes of every 64 (8 bytes of a 32-byte row): byte of word i.
+template <int D, int BITS>
+__device__ __forceinline__ int k_byte(int li, int i) {
+  return Row<D, BITS>::kKWords >= 4 ? (i >> 2) * 64 + li * 16 + (i & 3) * 4 : li * 8 + i * 4;
+}
+// Channel of element e (0, 1: low / high half) of pair `pr` (0, 1) of step s of S: the order in
+// which the unpacking above meets the codes of a lane's words.
+template <int D, int BITS>
+__device__ __forceinline__ int k_channel(int li, int s, int pr, int e) {
+  if (BITS == 4) return k_byte<D, BITS>(li, s >> 1) * 2 + (s & 1) * 2 + pr + 4 * e;
+  return k_byte<D, BITS>(li, s) + pr * 2 + e;
 }
 
 // -------------------------------------------------------------- main kernel
 template <typename T, int D, int BITS, int NT>
-__global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha_cache_kernel(const Params p) {
   using R = Row<D, BITS>;
   constexpr int kCols = 8 * NT;
   constexpr int kPitch = D + 4;  // accumulators of one column in shared memory, padded against conflicts
@@ -197,7 +217,12 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
   __shared__ float q_mul[kCols], q_sum[kCols];
   __shared__ int q_pos[kCols];
   __shared__ float w_max[kWarps][kCols], w_sum[kWarps][kCols], w_zero[kWarps][kCols];
-  __shared__ __align__(16) float o_s[kCols][kPitch];
+  __shared__ __align__(8) uint64_t bars[kWarps][R::kStages];
+  __shared__ int have_s[kWarps][R::kStages];
+  __shared__ int abort_s;
+  extern __shared__ __align__(16) uint8_t ring[];
+  float(*o_s)[kPitch] = reinterpret_cast<float(*)[kPitch]>(ring);  // after the loop: the ring is done with
+  static_assert(kCols * kPitch * 4 <= R::kRing, "the joined accumulators reuse the ring");
 
   const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles;
   const int hk = blockIdx.y, b = blockIdx.z;
@@ -213,6 +238,63 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int li = lane & 3, lj = lane >> 2;
+  volatile int* abort_flag = &abort_s;
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    for (int w = 0; w < kWarps; ++w)
+      for (int i = 0; i < R::kStages; ++i) mbar_init(smem_u32(&bars[w][i]), 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  // The ring: lane 4 hf + x issues the copy of part x (codes of K, V, pairs of K, V) of half hf; a page
+  // of a multiple of 32 keys holds a slab whole, and lanes 0 .. 3 copy it at once. Page numbers are
+  // fetched one slab ahead, so the copies never wait for the block table.
+  const int32_t* table = p.table + (int64_t)b * p.table_stride;
+  const uint32_t my_ring = smem_u32(ring) + warp * (R::kStages * R::kStage);
+  const uint32_t my_bar = smem_u32(&bars[warp][0]);
+  const bool whole = p.page_size % kSlab == 0;
+  auto first_key = [&](int v) { return (v < rg.first ? v : rg.lo + v - rg.first) * kSlab; };
+  auto page_of = [&](int v) {
+    const int t = first_key(v) + ((lane >> 2) & 1) * 16;
+    const int col = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
+    return v < v1 && t < sq.len && col < p.table_width ? table[col] : -1;
+  };
+  auto fetch = [&](int v, int st, int page) {
+    const int t = first_key(v) + ((lane >> 2) & 1) * 16;
+    const bool ok = page >= 0 && page < p.pages;
+    if (t < sq.len && !ok && (lane & ~4) == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
+    const unsigned good = __ballot_sync(0xffffffffu, ok);
+    const int have = (good & 1) | ((good >> 3) & 2);
+    if (lane == 0) {
+      have_s[warp][st] = have;
+      const int rows = whole ? ((have & 1) ? kSlab : 0) : 16 * ((have & 1) + (have >> 1));
+      mbar_arrive_expect_tx(my_bar + 8 * st, rows * (2 * R::kBytes + 8));
+    }
+    __syncwarp();
+    if (ok && lane < (whole ? 4 : 8)) {
+      const int part = lane & 3, hf = lane >> 2;
+      const int inside = p.page_shift >= 0 ? t & (p.page_size - 1) : t % p.page_size;
+      const int64_t row = ((int64_t)page * p.hkv + hk) * p.page_size + inside;
+      const int width = part < 2 ? R::kBytes : 4;
+      const uint8_t* base = part == 0   ? p.k_codes
+                            : part == 1 ? p.v_codes
+                            : part == 2 ? reinterpret_cast<const uint8_t*>(p.k_pairs)
+                                        : reinterpret_cast<const uint8_t*>(p.v_pairs);
+      const uint32_t to = part == 0 ? 0 : part == 1 ? R::kV : part == 2 ? R::kKP : R::kVP;
+      bulk_load(my_ring + st * R::kStage + to + hf * 16 * width, base + row * width, (whole ? kSlab : 16) * width,
+                my_bar + 8 * st);
+    }
+  };
+  int next_page = page_of(v0 + warp);
+#pragma unroll
+  for (int i = 0; i < R::kStages; ++i) {
+    const int v = v0 + warp + i * kWarps;
+    if (v < v1) {
+      fetch(v, i, next_page);
+      next_page = page_of(v + kWarps);
+    }
+  }
 
   // queries as f16, each column divided by the power of two below its largest value (exact, and
   // within range for bf16 queries of any size), with the factor to undo it and the sum over d
@@ -262,8 +344,9 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
     for (int s = 0; s < R::kSteps; ++s)
 #pragma unroll
       for (int pr = 0; pr < 2; ++pr) {
-        const __half* row = q_s[n * 8 + lj] + li * (D / 4);
-        const __half2 h = __halves2half2(row[k_channel<BITS>(s, pr, 0)], row[k_channel<BITS>(s, pr, 1)]);
+        const __half* row = q_s[n * 8 + lj];
+        const __half2 h =
+            __halves2half2(row[k_channel<D, BITS>(li, s, pr, 0)], row[k_channel<D, BITS>(li, s, pr, 1)]);
         qf[n][s][pr] = *reinterpret_cast<const uint32_t*>(&h);
       }
   float mul[NT][2], qsum[NT][2];
@@ -297,22 +380,18 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
   // exponent bits of a float, so that p * scale_v fits f16 whatever the size of the values
   uint32_t vexp = 0x00800000u;
 
-  const int32_t* table = p.table + (int64_t)b * p.table_stride;
-  const int64_t head_row = (int64_t)hk * p.page_size;
-  for (int v = v0 + warp; v < v1; v += kWarps) {
-    const int t0 = (v < rg.first ? v : rg.lo + v - rg.first) * kSlab;
-    // rows of the two 16-key halves of the slab (a page holds a multiple of 16)
-    int64_t row[2];
-    bool have[2];
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int t = t0 + 16 * hf;
-      const int col = t / p.page_size;
-      const int page = t < sq.len && col < p.table_width ? table[col] : -1;
-      have[hf] = page >= 0 && page < p.pages;
-      if (t < sq.len && !have[hf] && lane == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
-      row[hf] = have[hf] ? ((int64_t)page * p.hkv) * p.page_size + head_row + t % p.page_size : 0;
+  bool ok = true;
+  int st = 0;
+  uint32_t phase = 0;
+  int v = v0 + warp;
+  for (; v < v1; v += kWarps) {
+    const int t0 = first_key(v);
+    if (!wait_bounded(my_bar + 8 * st, phase, abort_flag, p.status, kStatusTimeoutProducer)) {
+      ok = false;
+      break;
     }
+    const int have_bits = have_s[warp][st];
+    const uint8_t* slab = ring + (warp * R::kStages + st) * R::kStage;
     float s[2][NT][4];
     float vs[2][2], vz[2][2];
     uint32_t vs_max = 0;
@@ -322,21 +401,29 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[hf][n][e] = 0.f;
+      const bool have = (have_bits >> hf) & 1;
       uint32_t w[2][R::kKWords];
       float ks[2] = {0.f, 0.f}, kz[2] = {0.f, 0.f};
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int t = t0 + 16 * hf + 8 * r + lj;
-        const int64_t at = row[hf] + 8 * r + lj;
+        const int key = 16 * hf + 8 * r + key_of(lj);
         vs[hf][r] = vz[hf][r] = 0.f;
+        const uint8_t* src = slab + key * R::kBytes;
+        if constexpr (R::kKWords >= 4) {
 #pragma unroll
-        for (int i = 0; i < R::kKWords; ++i) w[r][i] = 0;
-        if (have[hf]) {
-          load_words<R::kKWords>(p.k_codes + at * R::kBytes + li * (R::kBytes / 4), w[r]);
-          if (t < sq.len) {
-            Cvt<T>::unpack(p.k_pairs[at], ks[r], kz[r]);
-            Cvt<T>::unpack(p.v_pairs[at], vs[hf][r], vz[hf][r]);
+          for (int i = 0; i < R::kKWords / 4; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + i * 64 + li * 16);
+            w[r][4 * i] = x.x;
+            w[r][4 * i + 1] = x.y;
+            w[r][4 * i + 2] = x.z;
+            w[r][4 * i + 3] = x.w;
           }
+        } else {
+          load_words<R::kKWords>(src + li * 8, w[r]);
+        }
+        if (have && t0 + key < sq.len) {  // what lies behind the sequence may be anything
+          Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kKP)[key], ks[r], kz[r]);
+          Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kVP)[key], vs[hf][r], vz[hf][r]);
         }
         vs_max = max(vs_max, __float_as_uint(vs[hf][r]));
       }
@@ -361,7 +448,7 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
       // logits in log2 units, masks
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int t = t0 + 16 * hf + 8 * r + lj;
+        const int t = t0 + 16 * hf + 8 * r + key_of(lj);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -370,7 +457,7 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
             if (p.softcap > 0.f) x = p.softcap * kLog2e * tanhf(x / p.softcap);
             s[hf][n][2 * r + e] = x;
           }
-        const bool edge = !have[hf] || t0 + kSlab > sq.len || (p.causal && t0 + kSlab - 1 > pos_min) ||
+        const bool edge = !have || t0 + kSlab > sq.len || (p.causal && t0 + kSlab - 1 > pos_min) ||
                           (p.window > 0 && t0 + kSlab > p.sinks &&
                            (t0 < pos_max - p.window || t0 + kSlab - 1 > pos_min + p.window));
         if (edge) {
@@ -378,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              bool keep = have[hf] && t < sq.len && (!p.causal || t <= pos[n][e]);
+              bool keep = have && t < sq.len && (!p.causal || t <= pos[n][e]);
               if (p.window > 0) keep = keep && (abs(t - pos[n][e]) <= p.window || t < p.sinks);
               if (!keep) s[hf][n][2 * r + e] = -INFINITY;
             }
@@ -448,11 +535,9 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
       uint32_t w[4][R::kVWords];  // keys 2i, 2i + 1, 2i + 8, 2i + 9
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int i = 0; i < R::kVWords; ++i) w[r][i] = 0;
-        if (have[hf])
-          load_words<R::kVWords>(p.v_codes + (row[hf] + 2 * li + (r & 1) + 8 * (r >> 1)) * R::kBytes +
-                                     lj * (R::kBytes / 8), w[r]);
+        load_words<R::kVWords>(slab + R::kV + (16 * hf + key_of(2 * li + (r & 1)) + 8 * (r >> 1)) * R::kBytes +
+                                   lj * (R::kBytes / 8),
+                               w[r]);
       }
 #pragma unroll
       for (int i = 0; i < R::kVWords; ++i) {
@@ -479,6 +564,26 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
               mma16816(o[2 * i + h][n], bytes01(x), bytes23(x), bytes01(y), bytes23(y), pf[hf][n][0], pf[hf][n][1]);
           }
         }
+      }
+    }
+    // every lane has read the slab: its place goes to the slab kStages further on
+    __syncwarp();
+    const int ahead = v + R::kStages * kWarps;
+    if (ahead < v1) {
+      fetch(ahead, st, next_page);
+      next_page = page_of(ahead + kWarps);
+    }
+    if (++st == R::kStages) {
+      st = 0;
+      phase ^= 1;
+    }
+  }
+  if (!ok) {  // a wait ran out: let the copies in flight land before the ring goes
+    for (int i = 0; i < R::kStages; ++i) {
+      if (v + i * kWarps < v1) wait_for(my_bar + 8 * st, phase, p.status, kStatusTimeoutDrain);
+      if (++st == R::kStages) {
+        st = 0;
+        phase ^= 1;
       }
     }
   }
@@ -556,38 +661,55 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_kernel(const Params p) {
   }
 }
 
-// -------------------------------------------------------------- join the splits: one warp per (query, head)
+// -------------------------------------------------------------- join the splits
+// `per_row` warps (1, or all of the CTA's when there are many splits) share a (query, head): each adds
+// every per_row-th split, then the warps' sums are added in order.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) fmha_cache_join_kernel(const Params p, int cols) {
+__global__ void __launch_bounds__(kThreads) fmha_cache_join_kernel(const Params p, int cols, int per_row) {
+  constexpr int kPer = D / 32;
+  __shared__ float acc_s[kWarps][D], sum_s[kWarps];
   const int hk = blockIdx.y, b = blockIdx.z;
   const Seq sq = sequence(p, b);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = blockIdx.x * kWarps + warp;
-  if (col >= sq.n * p.group) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % per_row;
+  const int col = blockIdx.x * (kWarps / per_row) + warp / per_row;
+  if (col >= sq.n * p.group) return;  // with per_row = kWarps the whole CTA leaves; else no barrier follows
   const int c0 = col / cols * cols, c1 = min(c0 + cols, sq.n * p.group);
   const Range rg = key_range(p, sq, c0, c1);
   const int used = min(max(1, (rg.count + p.split_slabs - 1) / p.split_slabs), p.splits);
   const int tok = col / p.group, head = hk * p.group + col % p.group;
   const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head, stride = p.tq * p.hq;
   float mx = -INFINITY;
-  for (int s = 0; s < used; ++s) mx = fmaxf(mx, p.part_ml[s * stride + r].x);
-  constexpr int kPer = D / 32;
+  for (int s = lane; s < used; s += 32) mx = fmaxf(mx, p.part_ml[s * stride + r].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float acc[kPer], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  for (int s = 0; s < used; ++s) {
+#pragma unroll 4
+  for (int s = sub; s < used; s += per_row) {
     const float2 ml = p.part_ml[s * stride + r];
     const float a = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
     sum += ml.y * a;
-    const float* src = p.part_o + (s * stride + r) * D + lane * kPer;
+    const float* src = p.part_o + (s * stride + r) * D;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(src[i], a, acc[i]);
+    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(src[lane + 32 * i], a, acc[i]);
+  }
+  if (per_row > 1) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc_s[warp][lane + 32 * i] = acc[i];
+    if (lane == 0) sum_s[warp] = sum;
+    __syncthreads();
+    if (warp > 0) return;
+    for (int w = 1; w < kWarps; ++w) {
+      sum += sum_s[w];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[w][lane + 32 * i];
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* dst = reinterpret_cast<T*>(p.out) + r * D + lane * kPer;
+  T* dst = reinterpret_cast<T*>(p.out) + r * D;
 #pragma unroll
-  for (int i = 0; i < kPer / 2; ++i)
-    reinterpret_cast<uint32_t*>(dst)[i] = Cvt<T>::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  for (int i = 0; i < kPer; ++i) dst[lane + 32 * i] = Cvt<T>::from_f32(acc[i] * inv);
   if (lane == 0) p.lse[(int64_t)head * p.tq + sq.row0 + tok] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
@@ -619,16 +741,31 @@ Plan plan(int64_t b, int64_t hkv, int64_t group, int64_t max_q, int64_t max_k, i
   return pl;
 }
 
+template <typename T, int D, int BITS, int NT>
+int launch_main(const Params& p, const Plan& pl, cudaStream_t s) {
+  auto kern = fmha_cache_kernel<T, D, BITS, NT>;
+  constexpr int kBytes = Row<D, BITS>::kRing;
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) return host::cuda_check(e, "cudaFuncSetAttribute(fmha cache)");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const dim3 grid((unsigned)(pl.tiles * pl.splits), (unsigned)p.hkv, (unsigned)p.b);
+  kern<<<grid, kThreads, kBytes, s>>>(p);
+  return host::cuda_check(cudaGetLastError(), "fmha cache kernel launch");
+}
+
 template <typename T, int D, int BITS>
 int launch(const Params& p, const Plan& pl, cudaStream_t s) {
-  const dim3 grid((unsigned)(pl.tiles * pl.splits), (unsigned)p.hkv, (unsigned)p.b);
-  if (pl.cols == 8) fmha_cache_kernel<T, D, BITS, 1><<<grid, kThreads, 0, s>>>(p);
-  else fmha_cache_kernel<T, D, BITS, 2><<<grid, kThreads, 0, s>>>(p);
-  int rc = host::cuda_check(cudaGetLastError(), "fmha cache kernel launch");
+  int rc = pl.cols == 8 ? launch_main<T, D, BITS, 1>(p, pl, s) : launch_main<T, D, BITS, 2>(p, pl, s);
   if (rc || pl.splits == 1) return rc;
+  const int per_row = pl.splits > 2 * kWarps ? kWarps : 1, rows = kWarps / per_row;
   const int64_t columns = (int64_t)p.max_q * p.group;
-  const dim3 jgrid((unsigned)((columns + kWarps - 1) / kWarps), (unsigned)p.hkv, (unsigned)p.b);
-  fmha_cache_join_kernel<T, D><<<jgrid, kThreads, 0, s>>>(p, pl.cols);
+  const dim3 jgrid((unsigned)((columns + rows - 1) / rows), (unsigned)p.hkv, (unsigned)p.b);
+  fmha_cache_join_kernel<T, D><<<jgrid, kThreads, 0, s>>>(p, pl.cols, per_row);
   return host::cuda_check(cudaGetLastError(), "fmha cache join launch");
 }
 
@@ -720,6 +857,9 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
   p.v_pairs = static_cast<const uint32_t*>(v_pairs);
   p.pages = pages;
   p.page_size = (int)page_size;
+  p.page_shift = -1;
+  for (int i = 4; i <= 20; ++i)
+    if (page_size == (1ll << i)) p.page_shift = i;
   p.table = table;
   p.table_stride = table_stride;
   p.table_width = (int)table_width;

@@ -373,6 +373,7 @@ struct Cvt<__nv_bfloat16> {
     return *reinterpret_cast<uint32_t*>(&v);
   }
   static __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ void unpack(uint32_t v, float& a, float& b) {
     a = __uint_as_float(v << 16);
     b = __uint_as_float(v & 0xFFFF0000u);
@@ -385,6 +386,7 @@ struct Cvt<__half> {
     return *reinterpret_cast<uint32_t*>(&v);
   }
   static __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ void unpack(uint32_t v, float& a, float& b) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
     a = f.x;
