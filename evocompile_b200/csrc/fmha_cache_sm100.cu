@@ -254,6 +254,16 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   const uint32_t my_ring = smem_u32(ring) + warp * (R::kStages * R::kStage);
   const uint32_t my_bar = smem_u32(&bars[warp][0]);
   const bool whole = p.page_size % kSlab == 0;
+  const int copy_width = (lane & 3) < 2 ? R::kBytes : 4;  // bytes of a row of this lane's part
+  const int64_t copy_page = (int64_t)p.hkv * p.page_size * copy_width;
+  const uint8_t* copy_from = ((lane & 3) == 0   ? p.k_codes
+                              : (lane & 3) == 1 ? p.v_codes
+                              : (lane & 3) == 2 ? reinterpret_cast<const uint8_t*>(p.k_pairs)
+                                                : reinterpret_cast<const uint8_t*>(p.v_pairs)) +
+                             (int64_t)hk * p.page_size * copy_width;
+  const uint32_t copy_to = my_ring + ((lane & 3) == 0 ? 0 : (lane & 3) == 1 ? R::kV : (lane & 3) == 2 ? R::kKP : R::kVP) +
+                           (lane >> 2) * 16 * copy_width;
+  const uint32_t copy_bytes = (whole ? kSlab : 16) * copy_width;
   auto first_key = [&](int v) { return (v < rg.first ? v : rg.lo + v - rg.first) * kSlab; };
   auto page_of = [&](int v) {
     const int t = first_key(v) + ((lane >> 2) & 1) * 16;
@@ -273,16 +283,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
     __syncwarp();
     if (ok && lane < (whole ? 4 : 8)) {
-      const int part = lane & 3, hf = lane >> 2;
       const int inside = p.page_shift >= 0 ? t & (p.page_size - 1) : t % p.page_size;
-      const int64_t row = ((int64_t)page * p.hkv + hk) * p.page_size + inside;
-      const int width = part < 2 ? R::kBytes : 4;
-      const uint8_t* base = part == 0   ? p.k_codes
-                            : part == 1 ? p.v_codes
-                            : part == 2 ? reinterpret_cast<const uint8_t*>(p.k_pairs)
-                                        : reinterpret_cast<const uint8_t*>(p.v_pairs);
-      const uint32_t to = part == 0 ? 0 : part == 1 ? R::kV : part == 2 ? R::kKP : R::kVP;
-      bulk_load(my_ring + st * R::kStage + to + hf * 16 * width, base + row * width, (whole ? kSlab : 16) * width,
+      bulk_load(copy_to + st * R::kStage, copy_from + page * copy_page + inside * copy_width, copy_bytes,
                 my_bar + 8 * st);
     }
   };
@@ -392,22 +394,23 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
     const int have_bits = have_s[warp][st];
     const uint8_t* slab = ring + (warp * R::kStages + st) * R::kStage;
+    // whether some key of the slab is hidden from some column (or is not there at all)
+    const bool edge = have_bits != 3 || t0 + kSlab > sq.len || (p.causal && t0 + kSlab - 1 > pos_min) ||
+                      (p.window > 0 && t0 + kSlab > p.sinks &&
+                       (t0 < pos_max - p.window || t0 + kSlab - 1 > pos_min + p.window));
     float s[2][NT][4];
     float vs[2][2], vz[2][2];
-    uint32_t vs_max = 0;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[hf][n][e] = 0.f;
-      const bool have = (have_bits >> hf) & 1;
       uint32_t w[2][R::kKWords];
-      float ks[2] = {0.f, 0.f}, kz[2] = {0.f, 0.f};
+      float ks[2], kz[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int key = 16 * hf + 8 * r + key_of(lj);
-        vs[hf][r] = vz[hf][r] = 0.f;
         const uint8_t* src = slab + key * R::kBytes;
         if constexpr (R::kKWords >= 4) {
 #pragma unroll
@@ -421,11 +424,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
         } else {
           load_words<R::kKWords>(src + li * 8, w[r]);
         }
-        if (have && t0 + key < sq.len) {  // what lies behind the sequence may be anything
-          Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kKP)[key], ks[r], kz[r]);
-          Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kVP)[key], vs[hf][r], vz[hf][r]);
-        }
-        vs_max = max(vs_max, __float_as_uint(vs[hf][r]));
+        Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kKP)[key], ks[r], kz[r]);
+        Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kVP)[key], vs[hf][r], vz[hf][r]);
       }
       // S^T += K q^T
 #pragma unroll
@@ -445,33 +445,41 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
           for (int n = 0; n < NT; ++n) mma16816(s[hf][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
         }
       }
-      // logits in log2 units, masks
+      // logits, in log2 units unless a softcap follows
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int t = t0 + 16 * hf + 8 * r + key_of(lj);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          s[hf][n][x] = fmaf(kz[x >> 1], qsum[n][x & 1], ks[x >> 1] * s[hf][n][x]) * mul[n][x & 1];
+    }
+    if (p.softcap > 0.f) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x = fmaf(kz[r], qsum[n][e], ks[r] * s[hf][n][2 * r + e]) * mul[n][e];
-            if (p.softcap > 0.f) x = p.softcap * kLog2e * tanhf(x / p.softcap);
-            s[hf][n][2 * r + e] = x;
-          }
-        const bool edge = !have || t0 + kSlab > sq.len || (p.causal && t0 + kSlab - 1 > pos_min) ||
-                          (p.window > 0 && t0 + kSlab > p.sinks &&
-                           (t0 < pos_max - p.window || t0 + kSlab - 1 > pos_min + p.window));
-        if (edge) {
+          for (int x = 0; x < 4; ++x) s[hf][n][x] = p.softcap * kLog2e * tanhf(s[hf][n][x] / p.softcap);
+    }
+    if (edge) {  // what lies behind the sequence may be anything, its pairs among it
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int t = t0 + 16 * hf + 8 * r + key_of(lj);
+          const bool there = ((have_bits >> hf) & 1) && t < sq.len;
+          if (!there) vs[hf][r] = vz[hf][r] = 0.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              bool keep = have && t < sq.len && (!p.causal || t <= pos[n][e]);
+              bool keep = there && (!p.causal || t <= pos[n][e]);
               if (p.window > 0) keep = keep && (abs(t - pos[n][e]) <= p.window || t < p.sinks);
               if (!keep) s[hf][n][2 * r + e] = -INFINITY;
             }
         }
-      }
     }
+    uint32_t vs_max = max(max(__float_as_uint(vs[0][0]), __float_as_uint(vs[0][1])),
+                          max(__float_as_uint(vs[1][0]), __float_as_uint(vs[1][1])));
     // running maximum per column and the exponent of the value scales; both move rarely
     bool grow = false;
     float top[NT][2];
@@ -509,6 +517,36 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
     const float vdown = __uint_as_float(0x7f000000u - vexp);  // 1 / 2^(exponent of vexp)
     // probabilities, sums, and P^T as the B operand (rows are keys, columns are queries)
+    float base[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) base[n][e] = m[n][e] == -INFINITY ? 0.f : m[n][e];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          s[hf][n][x] = fast_exp2(s[hf][n][x] - base[n][x & 1]);
+          l[n][x & 1] += s[hf][n][x];
+        }
+    if (edge) {  // a hidden key may have a zero of NaN: it must not meet its probability of 0
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (s[hf][n][x] > 0.f) z[n][x & 1] = fmaf(s[hf][n][x], vz[hf][x >> 1], z[n][x & 1]);
+    } else {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) z[n][x & 1] = fmaf(s[hf][n][x], vz[hf][x >> 1], z[n][x & 1]);
+    }
     uint32_t pf[2][NT][2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
@@ -516,18 +554,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
       for (int r = 0; r < 2; ++r) {
         const float sv = vs[hf][r] * vdown;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float pv[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float mm = m[n][e] == -INFINITY ? 0.f : m[n][e];
-            const float x = fast_exp2(s[hf][n][2 * r + e] - mm);
-            l[n][e] += x;
-            z[n][e] += x > 0.f ? x * vz[hf][r] : 0.f;
-            pv[e] = x * sv;
-          }
-          pf[hf][n][r] = transpose8x8(Cvt<__half>::pack(pv[0], pv[1]));
-        }
+        for (int n = 0; n < NT; ++n)
+          pf[hf][n][r] = transpose8x8(Cvt<__half>::pack(s[hf][n][2 * r] * sv, s[hf][n][2 * r + 1] * sv));
       }
     // O^T += V^T P^T
 #pragma unroll
