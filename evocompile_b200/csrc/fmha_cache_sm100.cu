@@ -4,15 +4,24 @@
 // With K[j] = scale_k[j] c_j + zero_k[j] and V[j] = scale_v[j] e_j + zero_v[j] (c, e: codes):
 //   logit_ij = scale * (scale_k[j] (q_i . c_j) + zero_k[j] sum(q_i))
 //   out_i    = (sum_j (p_ij scale_v[j]) e_j + sum_j p_ij zero_v[j]) / sum_j p_ij
-// so the tensor cores multiply the codes themselves, exact in f16, and the pairs are applied in
-// f32 to the accumulators and probabilities. Nothing dequantised is ever stored.
+// so the tensor cores multiply the codes themselves and the pairs are applied in f32 to the
+// accumulators and probabilities. Nothing dequantised is ever stored.
 //
 // The cache is read once, so the kernel is bound by memory (d * bits / 8 + 4 bytes per row, 2
-// rows per token and kv head), and the work that unpacks 64 codes a clock per SM has to hide
-// behind it. Products run on m16n8k16 (mma.sync) with the codes as the 16-row operand and the
-// query heads of one kv head as the 8-column operand: S^T = K q^T and O^T = V^T P^T. The cache
-// rows come straight from memory in the operand's register layout, and a query group of 8 fills
-// the columns; tcgen05 would want the unpacked codes in shared memory and 128 rows of queries.
+// rows per token and kv head), as long as the work that unpacks the codes hides behind it; that
+// work is what the layout below is about. Products run on mma.sync with the codes as the 16-row
+// operand and the query heads of one kv head as the 8-column operand: S^T = K q^T and
+// O^T = V^T P^T. The codes come straight from memory in the operand's register layout, and a query
+// group of 8 fills the columns; tcgen05 would want the unpacked codes in shared memory and 128
+// rows of queries.
+//   K          m16n8k32 on u8 x s8: bytes of an 8-bit row need no unpacking, and a word of eight
+//              4-bit codes takes three integer instructions. The queries are 21-bit fixed-point
+//              numbers below the column's largest value, in three s8 pieces 2^7 apart (f16 products
+//              would cost five integer and four f16 instructions per word and no less; e4m3, whose
+//              patterns 0 .. 15 are linear too, is emulated for mma.sync on this chip). The sums are
+//              exact integers.
+//   V          m16n8k16 on f16: codes as integers in f16, probabilities times scale_v rounded to f16
+//              (11 bits; the running power of two below keeps them in its range).
 //
 // Columns of a CTA are (new token, query head) pairs of one kv head, kCols at a time. A CTA takes
 // one range of keys (grid.x: column tile, then split); its warps take slabs of 32 keys in turn,
@@ -22,6 +31,8 @@
 // memory system always has several slabs per warp to work on.
 // With more than one split the joined parts go to the workspace and a second kernel adds them,
 // again in a fixed order, so results do not vary from run to run.
+#include <type_traits>
+
 #include "host_common.h"
 #include "sm100_ptx.cuh"
 
@@ -38,6 +49,7 @@ constexpr float kRescale = 8.f;      // log2: the running maximum moves only whe
 
 struct Params {
   int b, hq, hkv, group, max_q;
+  float inv_group;
   int64_t tq;
   const void* q;
   int64_t q_st, q_sh;
@@ -109,7 +121,7 @@ __device__ __forceinline__ Range key_range(const Params& p, const Seq& s, int c0
 // -------------------------------------------------------------- fragments
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -117,7 +129,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -131,19 +143,39 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// C (+)= A B on u8 x s8; the first step of a sum starts from zero.
+__device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], bool first) {
+  if (first)
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "r"(0));
+  else
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
 // Integers as f16: 0x6400 | u is 1024 + u, and a nibble four bits higher adds 16 u.
 constexpr uint32_t kMinus1024 = 0xE400E400u;  // f16 (-1024, -1024)
 constexpr uint32_t kSixteenth = 0x2C002C00u;  // f16 (1/16, 1/16)
 constexpr uint32_t kMinus64 = 0xD400D400u;    // f16 (-64, -64)
 
+// (w & mask) | bits in one three-input logic instruction. It takes a single immediate, so `bits` is
+// kept in a register (opaque to the compiler, which otherwise splits the operation in two: 448
+// instead of 320 integer instructions per slab of 4-bit codes).
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
 // A word of 16-bit halves with four nibbles each -> four f16 pairs, (low half, high half) of
-// nibble 0, 1, 2, 3.
-__device__ __forceinline__ void nibbles(uint32_t w, uint32_t (&f)[4]) {
+// nibble 0, 1, 2, 3. `bits` is 0x64006400.
+__device__ __forceinline__ void nibbles(uint32_t w, uint32_t bits, uint32_t (&f)[4]) {
   const uint32_t s = w >> 8;
-  f[0] = h2_add((w & 0x000F000Fu) | 0x64006400u, kMinus1024);
-  f[1] = h2_fma((w & 0x00F000F0u) | 0x64006400u, kSixteenth, kMinus64);
-  f[2] = h2_add((s & 0x000F000Fu) | 0x64006400u, kMinus1024);
-  f[3] = h2_fma((s & 0x00F000F0u) | 0x64006400u, kSixteenth, kMinus64);
+  f[0] = h2_add(and_or(w, 0x000F000Fu, bits), kMinus1024);
+  f[1] = h2_fma(and_or(w, 0x00F000F0u, bits), kSixteenth, kMinus64);
+  f[2] = h2_add(and_or(s, 0x000F000Fu, bits), kMinus1024);
+  f[3] = h2_fma(and_or(s, 0x00F000F0u, bits), kSixteenth, kMinus64);
 }
 // Bytes 0, 1 and bytes 2, 3 of a word -> two f16 pairs.
 __device__ __forceinline__ uint32_t bytes01(uint32_t w) {
@@ -179,7 +211,8 @@ struct Row {
   static constexpr int kBytes = D * BITS / 8;
   static constexpr int kKWords = kBytes / 16;  // a lane's share of a key row: a quarter, D / 4 channels
   static constexpr int kVWords = kBytes / 32;  // a lane's share of a value row: an eighth, D / 8 channels
-  static constexpr int kSteps = D / 16;        // m16n8k16 steps over the channels of S; m-tiles of O
+  static constexpr int kSteps = D / 32;        // m16n8k32 steps over the channels of S
+  static constexpr int kTiles = D / 16;        // m-tiles of O
   // one slab of the ring: codes of K, of V, pairs of K, of V
   static constexpr int kV = kSlab * kBytes;
   static constexpr int kKP = 2 * kSlab * kBytes;
@@ -199,12 +232,31 @@ template <int D, int BITS>
 __device__ __forceinline__ int k_byte(int li, int i) {
   return Row<D, BITS>::kKWords >= 4 ? (i >> 2) * 64 + li * 16 + (i & 3) * 4 : li * 8 + i * 4;
 }
-// Channel of element e (0, 1: low / high half) of pair `pr` (0, 1) of step s of S: the order in
-// which the unpacking above meets the codes of a lane's words.
+// The queries' operand. Step s of S covers, for each lane quarter li, eight channels in the order in
+// which the codes come out of a lane's words: for 4 bits word s, its low nibbles (even channels) then
+// its high ones; for 8 bits words 2 s and 2 s + 1. A column's pieces are kept in shared memory in that
+// order, eight bytes per (step, li): byte of channel c.
 template <int D, int BITS>
-__device__ __forceinline__ int k_channel(int li, int s, int pr, int e) {
-  if (BITS == 4) return k_byte<D, BITS>(li, s >> 1) * 2 + (s & 1) * 2 + pr + 4 * e;
-  return k_byte<D, BITS>(li, s) + pr * 2 + e;
+__device__ __forceinline__ int query_byte(int c) {
+  if (BITS == 4) {
+    // words of a lane's share: (D = 128) step s of lane li is bytes 16 li + 4 s of the row's 64
+    const int word = c >> 3;  // word of the row
+    const int li = D == 128 ? word >> 2 : word >> 1, s = D == 128 ? word & 3 : word & 1;
+    return (s * 4 + li) * 8 + (c & 1) * 4 + ((c & 7) >> 1);
+  }
+  const int half = c >> 6, li = (c >> 4) & 3, in = c & 15;  // 16 bytes of every 64
+  return ((half * 2 + (in >> 3)) * 4 + li) * 8 + (in & 7);
+}
+
+constexpr int kPieces = 3;
+// One query value, scaled to below 2^7 in its column, as s8 pieces 2^7 apart.
+__device__ __forceinline__ void query_pieces(float x, int8_t (&piece)[kPieces]) {
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const float r = fminf(fmaxf(rintf(x), -127.f), 127.f);
+    piece[i] = (int8_t)r;
+    x = (x - r) * 128.f;
+  }
 }
 
 // -------------------------------------------------------------- main kernel
@@ -212,8 +264,10 @@ template <typename T, int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha_cache_kernel(const Params p) {
   using R = Row<D, BITS>;
   constexpr int kCols = 8 * NT;
-  constexpr int kPitch = D + 4;  // accumulators of one column in shared memory, padded against conflicts
-  __shared__ __align__(16) __half q_s[kCols][D + 8];
+  // accumulators of a warp's columns in shared memory: channel lj (D / 8) + k of a column at k * 8 + lj,
+  // columns D + 4 apart, so that a warp's stores hit every bank once
+  constexpr int kPitch = D + 4;
+  __shared__ __align__(16) int8_t q_s[kPieces][kCols][D];
   __shared__ float q_mul[kCols], q_sum[kCols];
   __shared__ int q_pos[kCols];
   __shared__ float w_max[kWarps][kCols], w_sum[kWarps][kCols], w_zero[kWarps][kCols];
@@ -221,8 +275,10 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   __shared__ int have_s[kWarps][R::kStages];
   __shared__ int abort_s;
   extern __shared__ __align__(16) uint8_t ring[];
-  float(*o_s)[kPitch] = reinterpret_cast<float(*)[kPitch]>(ring);  // after the loop: the ring is done with
-  static_assert(kCols * kPitch * 4 <= R::kRing, "the joined accumulators reuse the ring");
+  // after the loop the ring is done with, and each warp's part takes its accumulators
+  float(*o_s)[kPitch] = reinterpret_cast<float(*)[kPitch]>(ring);
+  constexpr int kWarpRows = R::kStages * R::kStage / (kPitch * 4);
+  static_assert(kCols <= kWarpRows, "a warp's accumulators fit its part of the ring");
 
   const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles;
   const int hk = blockIdx.y, b = blockIdx.z;
@@ -298,58 +354,67 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
   }
 
-  // queries as f16, each column divided by the power of two below its largest value (exact, and
-  // within range for bf16 queries of any size), with the factor to undo it and the sum over d
+  // queries, each column divided by the power of two below its largest value (exact, and any size of
+  // bf16 query comes within range), in pieces; the factor that undoes it and the sum over d
+  const int tok0 = c0 / p.group, rem0 = c0 - tok0 * p.group;
+  auto token_of = [&](int c) { return (int)((rem0 + c + 0.5f) * p.inv_group); };  // relative to tok0
   for (int c = warp; c < kCols; c += kWarps) {
-    const int col = c0 + c;
-    const bool in = col < c1;
-    const int tok = in ? col / p.group : 0;
-    const int head = hk * p.group + (in ? col % p.group : 0);
+    const bool in = c0 + c < c1;
+    const int rel = token_of(c);
+    const int tok = in ? tok0 + rel : tok0;
+    const int head = hk * p.group + (in ? rem0 + c - rel * p.group : 0);
     constexpr int kPer = D / 32;
     float x[kPer];
     float big = 0.f;
     const T* src = reinterpret_cast<const T*>(p.q) + (int64_t)(sq.row0 + tok) * p.q_st + (int64_t)head * p.q_sh +
                    lane * kPer;
+    uint32_t raw[kPer / 2];
+    load_words<kPer / 2>(reinterpret_cast<const uint8_t*>(src), raw);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      x[i] = in ? Cvt<T>::to_f32(src[i]) : 0.f;
-      big = fmaxf(big, fabsf(x[i]));
+    for (int i = 0; i < kPer / 2; ++i) {
+      Cvt<T>::unpack(in ? raw[i] : 0u, x[2 * i], x[2 * i + 1]);
+      big = fmaxf(big, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-    // exponent kept in [-100, 100] so that both factors are normal numbers
+    // largest value into [2^6, 2^7); exponent kept where both factors are normal numbers
+    constexpr int kTop = 6;
     int e = (big > 0.f && big < INFINITY) ? (int)((__float_as_uint(big) >> 23) & 255u) - 127 : 0;
     e = min(max(e, -100), 100);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+    const float down = __uint_as_float((uint32_t)(127 - e + kTop) << 23);
+    const float up = __uint_as_float((uint32_t)(127 + e - kTop) << 23);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      x[i] *= down;
-      sum += x[i];
-      q_s[c][lane * kPer + i] = __float2half_rn(x[i]);
+      const float y = x[i] * down;
+      sum += y;
+      int8_t piece[kPieces];
+      query_pieces(y, piece);
+#pragma unroll
+      for (int k = 0; k < kPieces; ++k) q_s[k][c][query_byte<D, BITS>(lane * kPer + i)] = piece[k];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
-      q_mul[c] = up * p.scale * (p.softcap > 0.f ? 1.f : kLog2e);
-      q_sum[c] = sum;
+      // the integer sums below are in units of 2^-7. A query that is not finite makes its column NaN.
+      q_mul[c] = up * p.scale * (p.softcap > 0.f ? 1.f : kLog2e) * (1.f / 128.f);
+      q_sum[c] = sum * 128.f + (big - big) + (sum - sum);
       q_pos[c] = sq.len - sq.n + tok;
     }
   }
   __syncthreads();
 
   // query fragments (B operand: rows are channels, columns are queries)
-  uint32_t qf[NT][R::kSteps][2];
+  uint32_t qf[kPieces][NT][R::kSteps][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int k = 0; k < kPieces; ++k)
 #pragma unroll
-    for (int s = 0; s < R::kSteps; ++s)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int pr = 0; pr < 2; ++pr) {
-        const __half* row = q_s[n * 8 + lj];
-        const __half2 h =
-            __halves2half2(row[k_channel<D, BITS>(li, s, pr, 0)], row[k_channel<D, BITS>(li, s, pr, 1)]);
-        qf[n][s][pr] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int s = 0; s < R::kSteps; ++s) {
+        const uint2 f = *reinterpret_cast<const uint2*>(&q_s[k][n * 8 + lj][(s * 4 + li) * 8]);
+        qf[k][n][s][0] = f.x;
+        qf[k][n][s][1] = f.y;
       }
   float mul[NT][2], qsum[NT][2];
   int pos[NT][2];
@@ -364,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
   const int pos_min = sq.len - sq.n + c0 / p.group, pos_max = sq.len - sq.n + (c1 - 1) / p.group;
 
-  float o[R::kSteps][NT][4];
+  float o[R::kTiles][NT][4];
   float m[NT][2], l[NT][2], z[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -374,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
       l[n][e] = z[n][e] = 0.f;
     }
 #pragma unroll
-    for (int s = 0; s < R::kSteps; ++s)
+    for (int s = 0; s < R::kTiles; ++s)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[s][n][e] = 0.f;
   }
@@ -382,6 +447,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   // exponent bits of a float, so that p * scale_v fits f16 whatever the size of the values
   uint32_t vexp = 0x00800000u;
 
+  uint32_t bits1024 = 0x64006400u;
+  asm volatile("" : "+r"(bits1024));
   bool ok = true;
   int st = 0;
   uint32_t phase = 0;
@@ -402,10 +469,6 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     float vs[2][2], vz[2][2];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[hf][n][e] = 0.f;
       uint32_t w[2][R::kKWords];
       float ks[2], kz[2];
 #pragma unroll
@@ -427,24 +490,33 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
         Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kKP)[key], ks[r], kz[r]);
         Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kVP)[key], vs[hf][r], vz[hf][r]);
       }
-      // S^T += K q^T
+      // S^T = K q^T, piece by piece
+      int acc[kPieces][NT][4];
 #pragma unroll
-      for (int i = 0; i < R::kKWords; ++i) {
+      for (int i = 0; i < R::kSteps; ++i) {
+        uint32_t a[4];
         if constexpr (BITS == 4) {
-          uint32_t f0[4], f1[4];
-          nibbles(w[0][i], f0);
-          nibbles(w[1][i], f1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma16816(s[hf][n], f0[0], f1[0], f0[1], f1[1], qf[n][2 * i][0], qf[n][2 * i][1]);
-            mma16816(s[hf][n], f0[2], f1[2], f0[3], f1[3], qf[n][2 * i + 1][0], qf[n][2 * i + 1][1]);
-          }
+          a[0] = w[0][i] & 0x0F0F0F0Fu;
+          a[1] = w[1][i] & 0x0F0F0F0Fu;
+          a[2] = (w[0][i] >> 4) & 0x0F0F0F0Fu;
+          a[3] = (w[1][i] >> 4) & 0x0F0F0F0Fu;
         } else {
-          const uint32_t a0 = bytes01(w[0][i]), a1 = bytes01(w[1][i]), a2 = bytes23(w[0][i]), a3 = bytes23(w[1][i]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(s[hf][n], a0, a1, a2, a3, qf[n][i][0], qf[n][i][1]);
+          a[0] = w[0][2 * i];
+          a[1] = w[1][2 * i];
+          a[2] = w[0][2 * i + 1];
+          a[3] = w[1][2 * i + 1];
         }
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16832(acc[k][n], a, qf[k][n][i], i == 0);
       }
+      // at most 128 * 255 * 127 each, so the two larger pieces join as integers
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          s[hf][n][x] = fmaf((float)acc[2][n][x], 1.f / 128.f, (float)(acc[0][n][x] * 128 + acc[1][n][x]));
       // logits, in log2 units unless a softcap follows
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -509,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
           l[n][e] *= alpha;
           z[n][e] *= alpha;
 #pragma unroll
-          for (int st = 0; st < R::kSteps; ++st) {
+          for (int st = 0; st < R::kTiles; ++st) {
             o[st][n][e] *= alpha * vscale;
             o[st][n][2 + e] *= alpha * vscale;
           }
@@ -573,8 +645,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // channels 4 h .. 4 h + 3 of the word
             uint32_t f0[4], f1[4];
-            nibbles(__byte_perm(w[0][i], w[1][i], h ? 0x7632 : 0x5410), f0);
-            nibbles(__byte_perm(w[2][i], w[3][i], h ? 0x7632 : 0x5410), f1);
+            nibbles(__byte_perm(w[0][i], w[1][i], h ? 0x7632 : 0x5410), bits1024, f0);
+            nibbles(__byte_perm(w[2][i], w[3][i], h ? 0x7632 : 0x5410), bits1024, f1);
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -616,6 +688,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
   }
 
+  asm volatile("griddepcontrol.launch_dependents;");  // the join kernel may be set up from here on
   // join the warps: sums over the lanes of a column, a common maximum, then warp after warp
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -643,23 +716,16 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
       for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][n * 8 + li * 2 + e]);
       f[n][e] = m[n][e] == -INFINITY ? 0.f : fast_exp2(m[n][e] - mx) * __uint_as_float(vexp);
     }
-  for (int w = 0; w < kWarps; ++w) {
-    if (warp == w) {
 #pragma unroll
-      for (int st = 0; st < R::kSteps; ++st)
+  for (int st = 0; st < R::kTiles; ++st)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float* at = &o_s[n * 8 + li * 2 + (x & 1)][lj * (D / 8) + 2 * st + (x >> 1)];
-            const float val = o[st][n][x] * f[n][x & 1];
-            *at = w == 0 ? val : *at + val;
-          }
-    }
-    __syncthreads();
-  }
+      for (int x = 0; x < 4; ++x)
+        o_s[warp * kWarpRows + n * 8 + li * 2 + (x & 1)][(2 * st + (x >> 1)) * 8 + lj] = o[st][n][x] * f[n][x & 1];
+  __syncthreads();
   for (int c = warp; c < c1 - c0; c += kWarps) {
-    const int col = c0 + c, tok = col / p.group, head = hk * p.group + col % p.group;
+    const int rel = token_of(c), tok = tok0 + rel, head = hk * p.group + rem0 + c - rel * p.group;
     float mx = -INFINITY, sum = 0.f, zero = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][c]);
@@ -670,19 +736,25 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
       zero += w_zero[w][c] * a;
     }
     constexpr int kPer = D / 32;
+    float acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int ch = lane * kPer + i, at = ch % (D / 8) * 8 + ch / (D / 8);
+      acc[i] = zero;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) acc[i] += o_s[w * kWarpRows + c][at];
+    }
     const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head;
     if (p.splits > 1) {
-      float* dst = p.part_o + ((int64_t)split * p.tq * p.hq + r) * D;
+      float2* dst = reinterpret_cast<float2*>(p.part_o + ((int64_t)split * p.tq * p.hq + r) * D + lane * kPer);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) dst[lane + 32 * i] = o_s[c][lane + 32 * i] + zero;
+      for (int i = 0; i < kPer / 2; ++i) dst[i] = make_float2(acc[2 * i], acc[2 * i + 1]);
       if (lane == 0) p.part_ml[(int64_t)split * p.tq * p.hq + r] = make_float2(mx, sum);
     } else {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays
-      T* dst = reinterpret_cast<T*>(p.out) + r * D;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + r * D + lane * kPer);
 #pragma unroll
-      for (int i = 0; i < kPer / 2; ++i)
-        reinterpret_cast<uint32_t*>(dst)[lane + 32 * i] = Cvt<T>::pack(
-            (o_s[c][2 * (lane + 32 * i)] + zero) * inv, (o_s[c][2 * (lane + 32 * i) + 1] + zero) * inv);
+      for (int i = 0; i < kPer / 2; ++i) dst[i] = Cvt<T>::pack(acc[2 * i] * inv, acc[2 * i + 1] * inv);
       if (lane == 0)
         p.lse[(int64_t)head * p.tq + sq.row0 + tok] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
     }
@@ -690,22 +762,25 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 }
 
 // -------------------------------------------------------------- join the splits
-// `per_row` warps (1, or all of the CTA's when there are many splits) share a (query, head): each adds
-// every per_row-th split, then the warps' sums are added in order.
+// `per_row` of the CTA's 16 warps share a (query, head): each adds every per_row-th split, then the
+// warps' sums are added in order. Launched so that it is resident when the main kernel ends.
+constexpr int kJoinWarps = 16;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) fmha_cache_join_kernel(const Params p, int cols, int per_row) {
+__global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const Params p, int cols, int per_row) {
   constexpr int kPer = D / 32;
-  __shared__ float acc_s[kWarps][D], sum_s[kWarps];
+  __shared__ float acc_s[kJoinWarps][D], sum_s[kJoinWarps];
   const int hk = blockIdx.y, b = blockIdx.z;
   const Seq sq = sequence(p, b);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % per_row;
-  const int col = blockIdx.x * (kWarps / per_row) + warp / per_row;
-  if (col >= sq.n * p.group) return;  // with per_row = kWarps the whole CTA leaves; else no barrier follows
+  const int col = blockIdx.x * (kJoinWarps / per_row) + warp / per_row;
+  const bool in = col < sq.n * p.group;
   const int c0 = col / cols * cols, c1 = min(c0 + cols, sq.n * p.group);
-  const Range rg = key_range(p, sq, c0, c1);
-  const int used = min(max(1, (rg.count + p.split_slabs - 1) / p.split_slabs), p.splits);
+  const Range rg = in ? key_range(p, sq, c0, c1) : Range{0, 0, 0};
+  const int used = in ? min(max(1, (rg.count + p.split_slabs - 1) / p.split_slabs), p.splits) : 0;
   const int tok = col / p.group, head = hk * p.group + col % p.group;
   const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head, stride = p.tq * p.hq;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // all parts are written from here on
   float mx = -INFINITY;
   for (int s = lane; s < used; s += 32) mx = fmaxf(mx, p.part_ml[s * stride + r].x);
 #pragma unroll
@@ -727,13 +802,14 @@ __global__ void __launch_bounds__(kThreads) fmha_cache_join_kernel(const Params 
     for (int i = 0; i < kPer; ++i) acc_s[warp][lane + 32 * i] = acc[i];
     if (lane == 0) sum_s[warp] = sum;
     __syncthreads();
-    if (warp > 0) return;
-    for (int w = 1; w < kWarps; ++w) {
-      sum += sum_s[w];
+    if (sub > 0) return;
+    for (int w = 1; w < per_row; ++w) {
+      sum += sum_s[warp + w];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[w][lane + 32 * i];
+      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[warp + w][lane + 32 * i];
     }
   }
+  if (!in) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* dst = reinterpret_cast<T*>(p.out) + r * D;
 #pragma unroll
@@ -790,11 +866,21 @@ template <typename T, int D, int BITS>
 int launch(const Params& p, const Plan& pl, cudaStream_t s) {
   int rc = pl.cols == 8 ? launch_main<T, D, BITS, 1>(p, pl, s) : launch_main<T, D, BITS, 2>(p, pl, s);
   if (rc || pl.splits == 1) return rc;
-  const int per_row = pl.splits > 2 * kWarps ? kWarps : 1, rows = kWarps / per_row;
+  int per_row = 1;  // about four splits per warp
+  while (per_row < kJoinWarps && per_row * 4 < pl.splits) per_row *= 2;
   const int64_t columns = (int64_t)p.max_q * p.group;
-  const dim3 jgrid((unsigned)((columns + rows - 1) / rows), (unsigned)p.hkv, (unsigned)p.b);
-  fmha_cache_join_kernel<T, D><<<jgrid, kThreads, 0, s>>>(p, pl.cols, per_row);
-  return host::cuda_check(cudaGetLastError(), "fmha cache join launch");
+  const int rows = kJoinWarps / per_row;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((columns + rows - 1) / rows), (unsigned)p.hkv, (unsigned)p.b);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return host::cuda_check(cudaLaunchKernelEx(&cfg, fmha_cache_join_kernel<T, D>, p, pl.cols, per_row),
+                          "fmha cache join launch");
 }
 
 template <typename T>
@@ -858,7 +944,9 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
   if (b == 0 || tq == 0 || max_seqlen_q == 0) return GKO_OK;
   if (!q || !k_codes || !v_codes || !k_pairs || !v_pairs || !table || !seq_lens || !out || !lse)
     return fail(GKO_ERR_INVALID, "fmha over a cache: null pointer argument");
-  const void* ptrs[5] = {k_codes, v_codes, k_pairs, v_pairs, out};
+  if (q_st % 8 || q_sh % 8)
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache needs token / head strides that are multiples of 8");
+  const void* ptrs[6] = {q, k_codes, v_codes, k_pairs, v_pairs, out};
   for (const void* x : ptrs)
     if (!host::aligned16(x)) return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache needs 16-byte aligned tensors");
   const fmha_cache::Plan pl =
@@ -874,6 +962,7 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
   p.hq = (int)hq;
   p.hkv = (int)hkv;
   p.group = (int)(hq / hkv);
+  p.inv_group = 1.f / (float)p.group;
   p.max_q = (int)max_seqlen_q;
   p.tq = tq;
   p.q = q;

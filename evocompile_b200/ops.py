@@ -721,8 +721,7 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
         scale = d ** -0.5
     if max_seqlen_k is None:
         max_seqlen_k = block_table.shape[1] * page_size
-    if q.stride(-1) != 1:
-        q = q.contiguous()
+    q = _bwd_fix(q)
     if out is None:
         out = torch.empty((tq, hq, d), device=dev, dtype=q.dtype)
     elif out.shape != (tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
