@@ -46,6 +46,7 @@ constexpr int kMaxSplitSlabs = 64;   // at most 2048 keys per split, so that one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;      // log2: the running maximum moves only when it grows by more
+constexpr float kNoMax = -1e30f;     // running maximum before any key: finite, so that differences are never NaN
 
 struct Params {
   int b, hq, hkv, group, max_q;
@@ -303,56 +304,70 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   }
   __syncthreads();
 
-  // The ring: lane 4 hf + x issues the copy of part x (codes of K, V, pairs of K, V) of half hf; a page
-  // of a multiple of 32 keys holds a slab whole, and lanes 0 .. 3 copy it at once. Page numbers are
-  // fetched one slab ahead, so the copies never wait for the block table.
+  // The ring. Lane 4 j + x copies part x (codes of K, V, pairs of K, V) of the warp's j-th slab of a
+  // batch of eight; where pages do not hold whole slabs, lane 8 j + 4 hf + x copies that part of half hf
+  // and a batch is four slabs. Addresses are worked out a batch at a time, page numbers fetched a batch
+  // ahead, so a slab costs a handful of instructions and never waits for the block table.
   const int32_t* table = p.table + (int64_t)b * p.table_stride;
   const uint32_t my_ring = smem_u32(ring) + warp * (R::kStages * R::kStage);
   const uint32_t my_bar = smem_u32(&bars[warp][0]);
   const bool whole = p.page_size % kSlab == 0;
-  const int copy_width = (lane & 3) < 2 ? R::kBytes : 4;  // bytes of a row of this lane's part
+  const int lane_shift = whole ? 2 : 3;
+  const int my_slab = lane >> lane_shift, my_part = lane & 3, my_half = whole ? 0 : (lane >> 2) & 1;
+  const int jump = (rg.lo - rg.first) * kSlab;
+  auto first_key = [&](int v) { return v * kSlab + (v < rg.first ? 0 : jump); };
+  const int copy_width = my_part < 2 ? R::kBytes : 4;  // bytes of a row of this lane's part
   const int64_t copy_page = (int64_t)p.hkv * p.page_size * copy_width;
-  const uint8_t* copy_from = ((lane & 3) == 0   ? p.k_codes
-                              : (lane & 3) == 1 ? p.v_codes
-                              : (lane & 3) == 2 ? reinterpret_cast<const uint8_t*>(p.k_pairs)
-                                                : reinterpret_cast<const uint8_t*>(p.v_pairs)) +
+  const uint8_t* copy_from = (my_part == 0   ? p.k_codes
+                              : my_part == 1 ? p.v_codes
+                              : my_part == 2 ? reinterpret_cast<const uint8_t*>(p.k_pairs)
+                                             : reinterpret_cast<const uint8_t*>(p.v_pairs)) +
                              (int64_t)hk * p.page_size * copy_width;
-  const uint32_t copy_to = my_ring + ((lane & 3) == 0 ? 0 : (lane & 3) == 1 ? R::kV : (lane & 3) == 2 ? R::kKP : R::kVP) +
-                           (lane >> 2) * 16 * copy_width;
+  const uint32_t copy_to = my_ring + (my_part == 0 ? 0 : my_part == 1 ? R::kV : my_part == 2 ? R::kKP : R::kVP) +
+                           my_half * 16 * copy_width;
   const uint32_t copy_bytes = (whole ? kSlab : 16) * copy_width;
-  auto first_key = [&](int v) { return (v < rg.first ? v : rg.lo + v - rg.first) * kSlab; };
-  auto page_of = [&](int v) {
-    const int t = first_key(v) + ((lane >> 2) & 1) * 16;
+  auto lookup = [&](int v) {  // page of this lane's slab of the batch that starts at v
+    const int t = first_key(v + my_slab * kWarps) + my_half * 16;
     const int col = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
-    return v < v1 && t < sq.len && col < p.table_width ? table[col] : -1;
+    return v + my_slab * kWarps < v1 && t < sq.len && col < p.table_width ? table[col] : -1;
   };
-  auto fetch = [&](int v, int st, int page) {
-    const int t = first_key(v) + ((lane >> 2) & 1) * 16;
+  const uint8_t* copy_src = nullptr;
+  unsigned good = 0;  // lanes whose copy exists
+  auto plan_batch = [&](int v, int page) {
+    const int t = first_key(v + my_slab * kWarps) + my_half * 16;
     const bool ok = page >= 0 && page < p.pages;
-    if (t < sq.len && !ok && (lane & ~4) == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
-    const unsigned good = __ballot_sync(0xffffffffu, ok);
-    const int have = (good & 1) | ((good >> 3) & 2);
+    if (!ok && v + my_slab * kWarps < v1 && t < sq.len && my_part == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
+    const int inside = p.page_shift >= 0 ? t & (p.page_size - 1) : t % p.page_size;
+    copy_src = copy_from + (ok ? page : 0) * copy_page + inside * copy_width;
+    good = __ballot_sync(0xffffffffu, ok);
+  };
+  int turn = 0;  // the batch's next slab
+  auto fetch = [&](int st) {
+    const unsigned g = good >> (turn << lane_shift);
     if (lane == 0) {
+      const int have = whole ? ((g & 1) ? 3 : 0) : ((g & 1) | ((g >> 3) & 2));
       have_s[warp][st] = have;
-      const int rows = whole ? ((have & 1) ? kSlab : 0) : 16 * ((have & 1) + (have >> 1));
-      mbar_arrive_expect_tx(my_bar + 8 * st, rows * (2 * R::kBytes + 8));
+      mbar_arrive_expect_tx(my_bar + 8 * st, ((have & 1) + (have >> 1)) * 16 * (2 * R::kBytes + 8));
     }
     __syncwarp();
-    if (ok && lane < (whole ? 4 : 8)) {
-      const int inside = p.page_shift >= 0 ? t & (p.page_size - 1) : t % p.page_size;
-      bulk_load(copy_to + st * R::kStage, copy_from + page * copy_page + inside * copy_width, copy_bytes,
-                my_bar + 8 * st);
+    if (my_slab == turn && ((good >> lane) & 1)) bulk_load(copy_to + st * R::kStage, copy_src, copy_bytes, my_bar + 8 * st);
+  };
+  const int batch = 32 >> lane_shift;
+  int ahead = v0 + warp;  // the next slab to fetch
+  plan_batch(ahead, lookup(ahead));
+  int next_page = lookup(ahead + batch * kWarps);
+  auto fetch_next = [&](int st) {
+    fetch(st);
+    ahead += kWarps;
+    if (++turn == batch) {
+      turn = 0;
+      plan_batch(ahead, next_page);
+      next_page = lookup(ahead + batch * kWarps);
     }
   };
-  int next_page = page_of(v0 + warp);
 #pragma unroll
-  for (int i = 0; i < R::kStages; ++i) {
-    const int v = v0 + warp + i * kWarps;
-    if (v < v1) {
-      fetch(v, i, next_page);
-      next_page = page_of(v + kWarps);
-    }
-  }
+  for (int i = 0; i < R::kStages; ++i)
+    if (ahead < v1) fetch_next(i);
 
   // queries, each column divided by the power of two below its largest value (exact, and any size of
   // bf16 query comes within range), in pieces; the factor that undoes it and the sum over d
@@ -435,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      m[n][e] = -INFINITY;
+      m[n][e] = kNoMax;
       l[n][e] = z[n][e] = 0.f;
     }
 #pragma unroll
@@ -449,6 +464,15 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 
   uint32_t bits1024 = 0x64006400u;
   asm volatile("" : "+r"(bits1024));
+  // slabs that every column sees whole: those that end by whole_to and start at or after whole_from, or
+  // end within the sinks
+  int whole_to = sq.len, whole_from = 0, whole_sinks = 0;
+  if (p.causal) whole_to = min(whole_to, pos_min + 1);
+  if (p.window > 0) {
+    whole_sinks = min(whole_to, p.sinks);
+    whole_from = pos_max - p.window;
+    whole_to = (int)min((int64_t)whole_to, (int64_t)pos_min + p.window + 1);
+  }
   bool ok = true;
   int st = 0;
   uint32_t phase = 0;
@@ -462,9 +486,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     const int have_bits = have_s[warp][st];
     const uint8_t* slab = ring + (warp * R::kStages + st) * R::kStage;
     // whether some key of the slab is hidden from some column (or is not there at all)
-    const bool edge = have_bits != 3 || t0 + kSlab > sq.len || (p.causal && t0 + kSlab - 1 > pos_min) ||
-                      (p.window > 0 && t0 + kSlab > p.sinks &&
-                       (t0 < pos_max - p.window || t0 + kSlab - 1 > pos_min + p.window));
+    const bool edge = have_bits != 3 || ((t0 < whole_from || t0 + kSlab > whole_to) && t0 + kSlab > whole_sinks);
     float s[2][NT][4];
     float vs[2][2], vz[2][2];
 #pragma unroll
@@ -550,22 +572,21 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
             }
         }
     }
-    uint32_t vs_max = max(max(__float_as_uint(vs[0][0]), __float_as_uint(vs[0][1])),
-                          max(__float_as_uint(vs[1][0]), __float_as_uint(vs[1][1])));
     // running maximum per column and the exponent of the value scales; both move rarely
-    bool grow = false;
-    float top[NT][2];
+    float top[NT][2], over = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1])) >= __uint_as_float(vexp)
+                                 ? INFINITY : 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[n][e] = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
-        grow |= top[n][e] > m[n][e] + kRescale;
+        top[n][e] = fmaxf(max3f(s[0][n][e], s[0][n][2 + e], s[1][n][e]), s[1][n][2 + e]);
+        over = fmaxf(over, top[n][e] - m[n][e]);
       }
-    vs_max = (__reduce_max_sync(0xffffffffu, vs_max) & 0x7f800000u) + 0x00800000u;
-    if (vs_max > vexp || __any_sync(0xffffffffu, grow)) {
-      // 2^(old exponent - new exponent): 0 when nothing was accumulated yet
-      const uint32_t vnew = max(vexp, vs_max);
+    if (__any_sync(0xffffffffu, over > kRescale)) {
+      // the power of two above the slab's largest value scale
+      const uint32_t vs_max = max(max(__float_as_uint(vs[0][0]), __float_as_uint(vs[0][1])),
+                                  max(__float_as_uint(vs[1][0]), __float_as_uint(vs[1][1])));
+      const uint32_t vnew = max(vexp, (__reduce_max_sync(0xffffffffu, vs_max) & 0x7f800000u) + 0x00800000u);
       const float vscale = __uint_as_float(vexp) / __uint_as_float(vnew);
       vexp = vnew;
 #pragma unroll
@@ -576,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, sh));
           const float mn = x > m[n][e] + kRescale ? x : m[n][e];
-          const float alpha = m[n][e] == mn ? 1.f : fast_exp2(m[n][e] - mn);
+          const float alpha = fast_exp2(m[n][e] - mn);
           m[n][e] = mn;
           l[n][e] *= alpha;
           z[n][e] *= alpha;
@@ -589,18 +610,13 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
     const float vdown = __uint_as_float(0x7f000000u - vexp);  // 1 / 2^(exponent of vexp)
     // probabilities, sums, and P^T as the B operand (rows are keys, columns are queries)
-    float base[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) base[n][e] = m[n][e] == -INFINITY ? 0.f : m[n][e];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          s[hf][n][x] = fast_exp2(s[hf][n][x] - base[n][x & 1]);
+          s[hf][n][x] = fast_exp2(s[hf][n][x] - m[n][x & 1]);
           l[n][x & 1] += s[hf][n][x];
         }
     if (edge) {  // a hidden key may have a zero of NaN: it must not meet its probability of 0
@@ -668,11 +684,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
     // every lane has read the slab: its place goes to the slab kStages further on
     __syncwarp();
-    const int ahead = v + R::kStages * kWarps;
-    if (ahead < v1) {
-      fetch(ahead, st, next_page);
-      next_page = page_of(ahead + kWarps);
-    }
+    if (ahead < v1) fetch_next(st);
     if (++st == R::kStages) {
       st = 0;
       phase ^= 1;
@@ -714,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
       float mx = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][n * 8 + li * 2 + e]);
-      f[n][e] = m[n][e] == -INFINITY ? 0.f : fast_exp2(m[n][e] - mx) * __uint_as_float(vexp);
+      f[n][e] = fast_exp2(m[n][e] - mx) * __uint_as_float(vexp);
     }
 #pragma unroll
   for (int st = 0; st < R::kTiles; ++st)
@@ -731,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][c]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float a = w_max[w][c] == -INFINITY ? 0.f : fast_exp2(w_max[w][c] - mx);
+      const float a = fast_exp2(w_max[w][c] - mx);
       sum += w_sum[w][c] * a;
       zero += w_zero[w][c] * a;
     }
@@ -781,7 +793,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const 
   const int tok = col / p.group, head = hk * p.group + col % p.group;
   const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head, stride = p.tq * p.hq;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // all parts are written from here on
-  float mx = -INFINITY;
+  float mx = kNoMax;
   for (int s = lane; s < used; s += 32) mx = fmaxf(mx, p.part_ml[s * stride + r].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -791,7 +803,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const 
 #pragma unroll 4
   for (int s = sub; s < used; s += per_row) {
     const float2 ml = p.part_ml[s * stride + r];
-    const float a = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
+    const float a = fast_exp2(ml.x - mx);
     sum += ml.y * a;
     const float* src = p.part_o + (s * stride + r) * D;
 #pragma unroll
