@@ -129,7 +129,7 @@ SIGNATURES = {
         _int,
         [_int, _int, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp],
     ),
-    "gko_fmha_cache_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int]),
+    "gko_fmha_cache_workspace_size": (_i64, [_int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int]),
     "gko_fmha_cache_fwd": (
         _int,
         [_int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp,

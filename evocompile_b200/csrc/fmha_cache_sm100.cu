@@ -15,8 +15,8 @@
 // group of 8 fills the columns; tcgen05 would want the unpacked codes in shared memory and 128
 // rows of queries.
 //   K          m16n8k32 on u8 x s8: bytes of an 8-bit row need no unpacking, and a word of eight
-//              4-bit codes takes three integer instructions. The queries are 21-bit fixed-point
-//              numbers below the column's largest value, in three s8 pieces 2^7 apart (f16 products
+//              4-bit codes takes three integer instructions. The queries are fixed-point numbers, 20 bits
+//              (21 for 8-bit codes) below the column's largest value, in three s8 pieces 2^7 apart (f16 products
 //              would cost five integer and four f16 instructions per word and no less; e4m3, whose
 //              patterns 0 .. 15 are linear too, is emulated for mma.sync on this chip). The sums are
 //              exact integers.
@@ -219,7 +219,7 @@ struct Row {
   static constexpr int kKP = 2 * kSlab * kBytes;
   static constexpr int kVP = kKP + kSlab * 4;
   static constexpr int kStage = kVP + kSlab * 4;
-  static constexpr int kStages = kStage > 8192 ? 2 : 3;
+  static constexpr int kStages = kStage > 4096 ? 2 : 3;
   static constexpr int kRing = kWarps * kStages * kStage;
 };
 
@@ -250,7 +250,7 @@ __device__ __forceinline__ int query_byte(int c) {
 }
 
 constexpr int kPieces = 3;
-// One query value, scaled to below 2^7 in its column, as s8 pieces 2^7 apart.
+// One query value, scaled to below 2^7 (2^6 for 4-bit codes) in its column, as s8 pieces 2^7 apart.
 __device__ __forceinline__ void query_pieces(float x, int8_t (&piece)[kPieces]) {
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   // accumulators of a warp's columns in shared memory: channel lj (D / 8) + k of a column at k * 8 + lj,
   // columns D + 4 apart, so that a warp's stores hit every bank once
   constexpr int kPitch = D + 4;
-  __shared__ __align__(16) int8_t q_s[kPieces][kCols][D];
+  constexpr int kQPitch = D + 32;  // a warp reads 8 bytes of eight columns at a time: no bank twice
+  __shared__ __align__(16) int8_t q_s[kPieces][kCols][kQPitch];
   __shared__ float q_mul[kCols], q_sum[kCols];
   __shared__ int q_pos[kCols];
   __shared__ float w_max[kWarps][kCols], w_sum[kWarps][kCols], w_zero[kWarps][kCols];
@@ -392,8 +393,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-    // largest value into [2^6, 2^7); exponent kept where both factors are normal numbers
-    constexpr int kTop = 6;
+    // largest value into [2^top, 2^(top + 1)); exponent kept where both factors are normal numbers
+    constexpr int kTop = BITS == 4 ? 5 : 6;
     int e = (big > 0.f && big < INFINITY) ? (int)((__float_as_uint(big) >> 23) & 255u) - 127 : 0;
     e = min(max(e, -100), 100);
     const float down = __uint_as_float((uint32_t)(127 - e + kTop) << 23);
@@ -411,26 +412,18 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
-      // the integer sums below are in units of 2^-7. A query that is not finite makes its column NaN.
-      q_mul[c] = up * p.scale * (p.softcap > 0.f ? 1.f : kLog2e) * (1.f / 128.f);
-      q_sum[c] = sum * 128.f + (big - big) + (sum - sum);
+      // the sums below are in units of 2^-14 (4 bits) or 2^-7. A query that is not finite makes its column NaN.
+      constexpr float kUnits = BITS == 4 ? 16384.f : 128.f;
+      q_mul[c] = up * p.scale * (p.softcap > 0.f ? 1.f : kLog2e) * (1.f / kUnits);
+      q_sum[c] = sum * kUnits + (big - big) + (sum - sum);
       q_pos[c] = sq.len - sq.n + tok;
     }
   }
   __syncthreads();
 
-  // query fragments (B operand: rows are channels, columns are queries)
-  uint32_t qf[kPieces][NT][R::kSteps][2];
-#pragma unroll
-  for (int k = 0; k < kPieces; ++k)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int s = 0; s < R::kSteps; ++s) {
-        const uint2 f = *reinterpret_cast<const uint2*>(&q_s[k][n * 8 + lj][(s * 4 + li) * 8]);
-        qf[k][n][s][0] = f.x;
-        qf[k][n][s][1] = f.y;
-      }
+  // query fragments (B operand: rows are channels, columns are queries) are read from shared memory step
+  // by step: 24 registers held across the loop would spill others
+  uint32_t q_at = smem_u32(&q_s[0][lj][li * 8]);
   float mul[NT][2], qsum[NT][2];
   int pos[NT][2];
 #pragma unroll
@@ -488,11 +481,10 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     // whether some key of the slab is hidden from some column (or is not there at all)
     const bool edge = have_bits != 3 || ((t0 < whole_from || t0 + kSlab > whole_to) && t0 + kSlab > whole_sinks);
     float s[2][NT][4];
-    float vs[2][2], vz[2][2];
+    float vs[2][2], vz[2][2], ks[2][2], kz[2][2];
+    uint32_t w[2][2][R::kKWords];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      uint32_t w[2][R::kKWords];
-      float ks[2], kz[2];
+    for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int key = 16 * hf + 8 * r + key_of(lj);
@@ -501,50 +493,72 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 #pragma unroll
           for (int i = 0; i < R::kKWords / 4; ++i) {
             const uint4 x = *reinterpret_cast<const uint4*>(src + i * 64 + li * 16);
-            w[r][4 * i] = x.x;
-            w[r][4 * i + 1] = x.y;
-            w[r][4 * i + 2] = x.z;
-            w[r][4 * i + 3] = x.w;
+            w[hf][r][4 * i] = x.x;
+            w[hf][r][4 * i + 1] = x.y;
+            w[hf][r][4 * i + 2] = x.z;
+            w[hf][r][4 * i + 3] = x.w;
           }
         } else {
-          load_words<R::kKWords>(src + li * 8, w[r]);
+          load_words<R::kKWords>(src + li * 8, w[hf][r]);
         }
-        Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kKP)[key], ks[r], kz[r]);
-        Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kVP)[key], vs[hf][r], vz[hf][r]);
       }
-      // S^T = K q^T, piece by piece
-      int acc[kPieces][NT][4];
+    // S^T = K q^T, piece by piece
+    {
+      int acc[kPieces][2][NT][4];
+      asm volatile("" : "+r"(q_at));  // keeps the fragments from being held across slabs
 #pragma unroll
       for (int i = 0; i < R::kSteps; ++i) {
-        uint32_t a[4];
-        if constexpr (BITS == 4) {
-          a[0] = w[0][i] & 0x0F0F0F0Fu;
-          a[1] = w[1][i] & 0x0F0F0F0Fu;
-          a[2] = (w[0][i] >> 4) & 0x0F0F0F0Fu;
-          a[3] = (w[1][i] >> 4) & 0x0F0F0F0Fu;
-        } else {
-          a[0] = w[0][2 * i];
-          a[1] = w[1][2 * i];
-          a[2] = w[0][2 * i + 1];
-          a[3] = w[1][2 * i + 1];
+        uint32_t a[2][4];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if constexpr (BITS == 4) {
+            a[hf][0] = w[hf][0][i] & 0x0F0F0F0Fu;
+            a[hf][1] = w[hf][1][i] & 0x0F0F0F0Fu;
+            a[hf][2] = (w[hf][0][i] >> 4) & 0x0F0F0F0Fu;
+            a[hf][3] = (w[hf][1][i] >> 4) & 0x0F0F0F0Fu;
+          } else {
+            a[hf][0] = w[hf][0][2 * i];
+            a[hf][1] = w[hf][1][2 * i];
+            a[hf][2] = w[hf][0][2 * i + 1];
+            a[hf][3] = w[hf][1][2 * i + 1];
+          }
         }
 #pragma unroll
         for (int k = 0; k < kPieces; ++k)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16832(acc[k][n], a, qf[k][n][i], i == 0);
+          for (int n = 0; n < NT; ++n) {
+            uint32_t f[2];
+            ld_shared_v2(q_at + (k * kCols + n * 8) * kQPitch + i * 32, f[0], f[1]);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) mma16832(acc[k][hf][n], a[hf], f, i == 0);
+          }
       }
-      // at most 128 * 255 * 127 each, so the two larger pieces join as integers
+      // 4 bits: at most 128 * 15 * (64 * 2^14 + 127 * 2^7 + 127) < 2^31, so all pieces join as integers;
+      // 8 bits: at most 128 * 255 * 127 each, and the two larger ones do
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            s[hf][n][x] = BITS == 4 ? (float)((acc[0][hf][n][x] * 128 + acc[1][hf][n][x]) * 128 + acc[2][hf][n][x])
+                                    : fmaf((float)acc[2][hf][n][x], 1.f / 128.f,
+                                           (float)(acc[0][hf][n][x] * 128 + acc[1][hf][n][x]));
+    }
+    // logits, in log2 units unless a softcap follows
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int key = 16 * hf + 8 * r + key_of(lj);
+        Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kKP)[key], ks[hf][r], kz[hf][r]);
+        Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(slab + R::kVP)[key], vs[hf][r], vz[hf][r]);
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          s[hf][n][x] = fmaf((float)acc[2][n][x], 1.f / 128.f, (float)(acc[0][n][x] * 128 + acc[1][n][x]));
-      // logits, in log2 units unless a softcap follows
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          s[hf][n][x] = fmaf(kz[x >> 1], qsum[n][x & 1], ks[x >> 1] * s[hf][n][x]) * mul[n][x & 1];
+          s[hf][n][x] = fmaf(kz[hf][x >> 1], qsum[n][x & 1], ks[hf][x >> 1] * s[hf][n][x]) * mul[n][x & 1];
     }
     if (p.softcap > 0.f) {
 #pragma unroll
@@ -834,9 +848,9 @@ struct Plan {
   int cols, tiles, splits, split_slabs;
 };
 
-// Columns per CTA, column tiles and key splits. Splits fill four CTAs on every SM, with at least
+// Columns per CTA, column tiles and key splits. Splits fill the CTAs that every SM holds, with at least
 // a slab for each warp and at most kMaxSplitSlabs slabs each.
-Plan plan(int64_t b, int64_t hkv, int64_t group, int64_t max_q, int64_t max_k, int window, int sinks) {
+Plan plan(int bits, int64_t b, int64_t hkv, int64_t group, int64_t max_q, int64_t max_k, int window, int sinks) {
   Plan pl;
   const int64_t columns = max_q * group;
   pl.cols = columns <= 8 ? 8 : 16;
@@ -847,7 +861,7 @@ Plan plan(int64_t b, int64_t hkv, int64_t group, int64_t max_q, int64_t max_k, i
     if (span < keys) keys = span;
   }
   const int64_t slabs = (keys + kSlab - 1) / kSlab > 0 ? (keys + kSlab - 1) / kSlab : 1;
-  const int64_t ctas = b * hkv * pl.tiles, slots = 4 * (int64_t)host::sm_count();
+  const int64_t ctas = b * hkv * pl.tiles, slots = (pl.cols > 8 ? 2 : bits == 4 ? 4 : 3) * (int64_t)host::sm_count();
   int64_t want = (slots + ctas - 1) / ctas;
   int64_t per = (slabs + want - 1) / want;
   if (per < kWarps) per = kWarps;
@@ -923,11 +937,11 @@ int check_sizes(int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq, int64
 using namespace gko;
 using gko::host::fail;
 
-extern "C" int64_t gko_fmha_cache_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+extern "C" int64_t gko_fmha_cache_workspace_size(int bits, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
                                                  int64_t max_seqlen_q, int64_t max_seqlen_k, int window, int sinks) {
-  if (fmha_cache::check_sizes(b, hq, hkv, d, tq, max_seqlen_q, max_seqlen_k, window, sinks)) return -1;
+  if ((bits != 4 && bits != 8) || fmha_cache::check_sizes(b, hq, hkv, d, tq, max_seqlen_q, max_seqlen_k, window, sinks)) return -1;
   if (b == 0 || tq == 0 || max_seqlen_q == 0) return 0;
-  const fmha_cache::Plan pl = fmha_cache::plan(b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
+  const fmha_cache::Plan pl = fmha_cache::plan(bits, b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
   return pl.splits > 1 ? pl.splits * tq * hq * (d * 4 + 8) : 0;
 }
 
@@ -962,7 +976,7 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
   for (const void* x : ptrs)
     if (!host::aligned16(x)) return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache needs 16-byte aligned tensors");
   const fmha_cache::Plan pl =
-      fmha_cache::plan(b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
+      fmha_cache::plan(bits, b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
   const int64_t need = pl.splits > 1 ? pl.splits * tq * hq * (d * 4 + 8) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need || !host::aligned16(workspace)))
     return fail(GKO_ERR_INVALID, "fmha over a cache needs a 16-byte aligned workspace of %lld bytes (got %lld)",

@@ -730,7 +730,7 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
     seq_lens = seq_lens.contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
-        ws_bytes = lib.gko_fmha_cache_workspace_size(b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k),
+        ws_bytes = lib.gko_fmha_cache_workspace_size(bits, b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k),
                                                      int(window or 0), int(sinks or 0))
         if ws_bytes < 0:
             _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_cache_workspace_size")

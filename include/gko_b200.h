@@ -378,7 +378,7 @@ int gko_kv_cache_read(int dtype, int bits, int64_t b, int64_t hkv, int64_t d, in
  * is cut to it. The result does not vary from run to run. workspace: 16-byte aligned device memory of
  * gko_fmha_cache_workspace_size bytes (may be 0; -1: sizes out of range), overwritten by the call.
  */
-int64_t gko_fmha_cache_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
+int64_t gko_fmha_cache_workspace_size(int bits, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
                                       int64_t max_seqlen_q, int64_t max_seqlen_k, int window, int sinks);
 int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
                        int64_t max_seqlen_q, int64_t max_seqlen_k, const void* q, int64_t q_st, int64_t q_sh,

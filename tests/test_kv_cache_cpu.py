@@ -78,13 +78,14 @@ def test_nothing_to_do(lib):
 def test_workspace_rule(lib):
     """Nothing when the keys fit one split; refused sizes give -1; a window bounds what a long cache needs."""
     size = lib.gko_fmha_cache_workspace_size
-    assert size(1, 8, 8, 128, 1, 1, 100, 0, 0) == 0
-    long_ = size(1, 8, 8, 128, 1, 1, 100000, 0, 0)
+    assert size(4, 1, 8, 8, 128, 1, 1, 100, 0, 0) == 0
+    long_ = size(4, 1, 8, 8, 128, 1, 1, 100000, 0, 0)
     assert long_ > 0 and long_ % (8 * (128 * 4 + 8)) == 0
-    assert size(1, 8, 8, 128, 1, 1, 100000, 64, 4) <= size(1, 8, 8, 128, 1, 1, 400, 0, 0)
-    assert size(0, 8, 8, 128, 0, 1, 100000, 0, 0) == 0
-    assert size(1, 8, 3, 128, 1, 1, 100, 0, 0) == -1
-    assert size(1, 8, 8, 100, 1, 1, 100, 0, 0) == -1
+    assert size(4, 1, 8, 8, 128, 1, 1, 100000, 64, 4) <= size(4, 1, 8, 8, 128, 1, 1, 400, 0, 0)
+    assert size(4, 0, 8, 8, 128, 0, 1, 100000, 0, 0) == 0
+    assert size(4, 1, 8, 3, 128, 1, 1, 100, 0, 0) == -1
+    assert size(4, 1, 8, 8, 100, 1, 1, 100, 0, 0) == -1
+    assert size(5, 1, 8, 8, 128, 1, 1, 100, 0, 0) == -1
 
 
 def test_fake_shapes():
