@@ -15,6 +15,8 @@
 // byte i), pairs [pages, kv heads, page, 2]; the rows of one page and head are contiguous, which
 // is what the attention over the cache reads in one bulk copy. Both kernels are bound by memory:
 // a row costs 2 d bytes on one side and d * bits / 8 + 4 on the other.
+#include <type_traits>
+
 #include "host_common.h"
 #include "sm100_ptx.cuh"
 
@@ -30,6 +32,7 @@ struct Params {
   void* k_pairs;
   void* v_pairs;
   int64_t pages, page_size;
+  int page_shift;  // log2 of the page size, -1 when it is not a power of two
   int64_t tokens;  // write: new tokens; read: packed tokens of the destination
   int hkv;
   const int64_t* slots;  // write
@@ -70,6 +73,21 @@ __device__ __forceinline__ uint32_t as_word(P p) {
 // -------------------------------------------------------------- write
 // kLanes = d / 8 lanes share a row, eight values (16 bytes) each. Minimum and maximum travel
 // together as one packed pair (min x, min -x), NaN kept, so a row needs log2(kLanes) shuffles.
+//
+// (x - zero) / scale is rounded to an integer without a division per value: t = (x - zero) * (1 / scale)
+// is off by less than 2^-14 (three f32 roundings of numbers up to 255), so its nearest integer is the
+// quotient's unless t is that near to a half; then the exact residual a - (c + 1/2) scale, of which one
+// fused multiply-add gives the sign, decides, and a true tie goes to the even code. Adding 1.5 * 2^23
+// rounds to an integer and leaves it in the low bits.
+constexpr float kRound = 12582912.f;
+
+__device__ __forceinline__ float settle(float a, float t, float scale) {
+  const float c = floorf(t);
+  const float r = fmaf(-(c + 0.5f), scale, a);
+  if (r != 0.f) return r > 0.f ? c + 1.f : c;
+  return c + (float)((int)c & 1);
+}
+
 template <typename T, int BITS, int kLanes>
 __device__ __forceinline__ void quantise_row(const uint4& raw, uint8_t* codes, T* pair, int part, bool store) {
   using P = typename Pair<T>::P;
@@ -87,24 +105,37 @@ __device__ __forceinline__ void quantise_row(const uint4& raw, uint8_t* codes, T
   float scale = Cvt<T>::to_f32(Pair<T>::up((high - low) / kTop));
   scale = fmaxf(scale, Pair<T>::kFloor);
   const bool fine = fabsf(low) < INFINITY && fabsf(high) < INFINITY && scale < INFINITY;
+  const float inv = 1.f / scale;
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  uint32_t q[8];
+  float x[8], q[8], far = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float x, y;
-    Cvt<T>::unpack(w[i], x, y);
-    q[2 * i] = fine ? (uint32_t)fminf(rintf((x - low) / scale), kTop) : 0u;
-    q[2 * i + 1] = fine ? (uint32_t)fminf(rintf((y - low) / scale), kTop) : 0u;
+  for (int i = 0; i < 4; ++i) Cvt<T>::unpack(w[i], x[2 * i], x[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = (x[i] - low) * inv;
+    q[i] = (t + kRound) - kRound;
+    far = fmaxf(far, fabsf(t - q[i]));
+  }
+  if (far > 0.5f - 1e-4f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = (x[i] - low) * inv;
+      if (fabsf(t - q[i]) > 0.5f - 1e-4f) q[i] = settle(x[i] - low, t, scale);
+    }
   }
   if (!store) return;
-  if constexpr (BITS == 4) {
-    uint32_t p = 0;
+  uint32_t u[8];
+  if constexpr (BITS == 4) {  // two codes make a byte, still as a float
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p |= q[i] << (4 * i);
-    reinterpret_cast<uint32_t*>(codes)[part] = p;
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(q[2 * i + 1], 16.f, q[2 * i]) + kRound);
+    const uint32_t word = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    reinterpret_cast<uint32_t*>(codes)[part] = fine ? word : 0u;
   } else {
-    reinterpret_cast<uint2*>(codes)[part] =
-        make_uint2(q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24, q[4] | q[5] << 8 | q[6] << 16 | q[7] << 24);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(q[i] + kRound);
+    const uint32_t lo = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    const uint32_t hi = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
+    reinterpret_cast<uint2*>(codes)[part] = fine ? make_uint2(lo, hi) : make_uint2(0u, 0u);
   }
   if (part == 0) {
     const float s = fine ? scale : 0.f, z = fine ? low : __int_as_float(0x7fc00000);
@@ -112,107 +143,156 @@ __device__ __forceinline__ void quantise_row(const uint4& raw, uint8_t* codes, T
   }
 }
 
+// One row of K and of V per group of lanes. A warp whose rows all lie past the end still runs: the
+// shuffles need every lane.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(256) kv_write_kernel(const Params p) {
   constexpr int kLanes = D / 8;
   constexpr int kRowBytes = D * BITS / 8;
   const int part = threadIdx.x % kLanes;
-  const int64_t rows = p.tokens * p.hkv;
-  const int64_t groups = (int64_t)gridDim.x * (256 / kLanes);
-  const int64_t limit = p.pages * p.page_size;
-  // every lane of a warp runs the same number of rounds: the shuffles need all of them
-  const int64_t first = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  const int64_t rounds = (rows + groups - 1) / groups;
-  for (int64_t n = 0; n < rounds; ++n) {
-    const int64_t r = first + n * groups;
-    const bool in = r < rows;
-    const int64_t t = in ? r / p.hkv : 0;
-    const int h = in ? (int)(r % p.hkv) : 0;
-    const int64_t slot = in ? p.slots[t] : -1;
-    const bool store = slot >= 0 && slot < limit;
-    if (slot >= limit && part == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
-    uint4 kx = make_uint4(0, 0, 0, 0), vx = make_uint4(0, 0, 0, 0);
-    if (store) {
-      kx = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh + part * 8);
-      vx = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + t * p.v_st + h * p.v_sh + part * 8);
-    }
-    const int64_t row = store ? ((slot / p.page_size) * p.hkv + h) * p.page_size + slot % p.page_size : 0;
-    quantise_row<T, BITS, kLanes>(kx, p.k_codes + row * kRowBytes, reinterpret_cast<T*>(p.k_pairs) + row * 2, part,
-                                  store);
-    quantise_row<T, BITS, kLanes>(vx, p.v_codes + row * kRowBytes, reinterpret_cast<T*>(p.v_pairs) + row * 2, part,
-                                  store);
-  }
+  const unsigned r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const bool in = r < (unsigned)(p.tokens * p.hkv);
+  const unsigned t = in ? r / (unsigned)p.hkv : 0u;
+  const int h = in ? (int)(r - t * (unsigned)p.hkv) : 0;
+  const int64_t slot = in ? p.slots[t] : -1;
+  const uint4 kx = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh + part * 8);
+  const uint4 vx = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + t * p.v_st + h * p.v_sh + part * 8);
+  const bool past = slot >= p.pages * p.page_size;
+  if (past && part == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
+  const bool store = slot >= 0 && !past;
+  const int64_t page = !store ? 0 : p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
+  const int64_t row = (page * p.hkv + h) * p.page_size + (store ? slot - page * p.page_size : 0);
+  quantise_row<T, BITS, kLanes>(kx, p.k_codes + row * kRowBytes, reinterpret_cast<T*>(p.k_pairs) + row * 2, part, store);
+  quantise_row<T, BITS, kLanes>(vx, p.v_codes + row * kRowBytes, reinterpret_cast<T*>(p.v_pairs) + row * 2, part, store);
 }
 
 // -------------------------------------------------------------- read
-// Eight codes -> eight values of the element type. A code (at most 8 bits) times a scale (at
-// most 11) is exact in f32, so the value is rounded once in the sum and once to the type.
+// Codes become integers in the element type and then code * scale + zero in one packed fused
+// multiply-add, so a value is rounded once. As f16, 0x6400 | u is 1024 + u (u below 1024); as bf16,
+// 0x4300 | u is 128 + u for u below 128, and bytes go through their two nibbles.
+template <typename T>
+struct Code;
+template <>
+struct Code<__half> {
+  static constexpr uint32_t kBits = 0x64006400u;
+  static constexpr float kBias = 1024.f;
+};
+template <>
+struct Code<__nv_bfloat16> {
+  static constexpr uint32_t kBits = 0x43004300u;
+  static constexpr float kBias = 128.f;
+};
+
+template <typename T, typename P = typename Pair<T>::P>
+__device__ __forceinline__ P both_of(float x) {
+  P r;
+  r.x = r.y = Cvt<T>::from_f32(x);
+  return r;
+}
+
+// Nibble `at` of each 16-bit half of w, as a pair of integers.
+template <typename T>
+__device__ __forceinline__ typename Pair<T>::P nibble_pair(uint32_t w, int at) {
+  using P = typename Pair<T>::P;
+  return __hsub2(as_pair<P>(((w >> (4 * at)) & 0x000F000Fu) | Code<T>::kBits), both_of<T>(Code<T>::kBias));
+}
+
+// Eight codes (a word of nibbles, or two of bytes) -> eight values.
 template <typename T, int BITS>
-__device__ __forceinline__ uint4 expand8(uint2 c, float s, float z) {
-  float f[8];
+__device__ __forceinline__ uint4 expand8(const uint32_t* c, typename Pair<T>::P s, typename Pair<T>::P z) {
+  using P = typename Pair<T>::P;
+  uint32_t v[4];
+  if constexpr (BITS == 4) {
+    // nibble n of the low half and of the high half are channels n and n + 4
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = BITS == 4 ? (c.x >> (4 * i)) & 15u : ((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 255u;
-    f[i] = fmaf((float)u, s, z);
+    for (int n = 0; n < 4; ++n) v[n] = as_word(__hfma2(nibble_pair<T>(c[0], n), s, z));
+    return make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410), __byte_perm(v[0], v[1], 0x7632),
+                      __byte_perm(v[2], v[3], 0x7632));
   }
-  return make_uint4(Cvt<T>::pack(f[0], f[1]), Cvt<T>::pack(f[2], f[3]), Cvt<T>::pack(f[4], f[5]),
-                    Cvt<T>::pack(f[6], f[7]));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = __byte_perm(c[i >> 1], 0u, i & 1 ? 0x4342 : 0x4140);  // two bytes, one in each half
+    P u;
+    if constexpr (std::is_same<T, __half>::value)
+      u = __hsub2(as_pair<P>(w | Code<T>::kBits), both_of<T>(Code<T>::kBias));
+    else  // 16 high + low, at most 255: exact
+      u = __hfma2(nibble_pair<T>(w, 1), both_of<T>(16.f), nibble_pair<T>(w, 0));
+    v[i] = as_word(__hfma2(u, s, z));
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-template <int BITS>
-__device__ __forceinline__ uint2 load_codes8(const uint8_t* row, int part) {
-  if constexpr (BITS == 4) return make_uint2(reinterpret_cast<const uint32_t*>(row)[part], 0u);
-  return reinterpret_cast<const uint2*>(row)[part];
-}
-
-// d / 8 lanes share a token and walk its heads; the token's sequence is found once by bisection.
+// d / 16 lanes share a token and walk its heads, 16 channels each; the token's sequence is found once by
+// bisection. Neighbouring lanes swap halves, so that each store of the warp writes whole sectors.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
-  constexpr int kLanes = D / 8;
+  using P = typename Pair<T>::P;
+  constexpr int kLanes = D / 16;
   constexpr int kRowBytes = D * BITS / 8;
+  constexpr int kWords = 2 * BITS / 4;  // of codes per lane
   const int part = threadIdx.x % kLanes;
   const int64_t t = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  if (t >= p.tokens) return;
   int lo = 0, hi = p.b;  // the first sequence whose end is past t
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (p.cu[mid + 1] > t) hi = mid;
     else lo = mid + 1;
   }
-  if (lo >= p.b || p.cu[lo] > t) return;  // behind the last sequence: left as it is
-  const int64_t pos = t - p.cu[lo];
-  const int64_t col = pos / p.page_size;
-  const int64_t page = col < p.table_width ? p.table[lo * p.table_stride + col] : -1;
-  if (page < 0 || page >= p.pages) {
+  // behind the last sequence: left as it is
+  bool live = t < p.tokens && lo < p.b && p.cu[lo] <= t;
+  const int pos = live ? (int)t - p.cu[lo] : 0;
+  const int col = p.page_shift >= 0 ? pos >> p.page_shift : pos / (int)p.page_size;
+  const int64_t page = live && col < p.table_width ? p.table[lo * p.table_stride + col] : -1;
+  if (live && (page < 0 || page >= p.pages)) {
     if (part == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
-    return;
+    live = false;
   }
-  const int64_t row0 = page * p.hkv * p.page_size + pos % p.page_size;
+  const int64_t row0 = live ? page * p.hkv * p.page_size + (pos - col * (int)p.page_size) : 0;
+  const bool odd = part & 1;
+  uint4* k_to = reinterpret_cast<uint4*>(p.k_out) + t * p.hkv * (D / 8) + (part & ~1) * 2 + odd;
+  uint4* v_to = reinterpret_cast<uint4*>(p.v_out) + t * p.hkv * (D / 8) + (part & ~1) * 2 + odd;
+  auto give = [&](const uint32_t (&c)[kWords], uint32_t pair, uint4* to) {
+    const P sz = as_pair<P>(pair);
+    P s, z;
+    s.x = s.y = sz.x;
+    z.x = z.y = sz.y;
+    const uint4 a = expand8<T, BITS>(c, s, z), b = expand8<T, BITS>(c + kWords / 2, s, z);
+    // the even lane writes the first half of its 16 channels and the first of the odd lane's, and so on
+    const uint4 keep = odd ? b : a, pass = odd ? a : b;
+    uint4 got;
+    got.x = __shfl_xor_sync(0xffffffffu, pass.x, 1);
+    got.y = __shfl_xor_sync(0xffffffffu, pass.y, 1);
+    got.z = __shfl_xor_sync(0xffffffffu, pass.z, 1);
+    got.w = __shfl_xor_sync(0xffffffffu, pass.w, 1);
+    if (live) {
+      to[0] = odd ? got : keep;
+      to[2] = odd ? keep : got;
+    }
+  };
 #pragma unroll 4
   for (int h = 0; h < p.hkv; ++h) {
     const int64_t row = row0 + h * p.page_size;
-    const uint2 kc = load_codes8<BITS>(p.k_codes + row * kRowBytes, part);
-    const uint2 vc = load_codes8<BITS>(p.v_codes + row * kRowBytes, part);
-    float ks, kz, vs, vz;
-    Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(p.k_pairs)[row], ks, kz);
-    Cvt<T>::unpack(reinterpret_cast<const uint32_t*>(p.v_pairs)[row], vs, vz);
-    const int64_t at = (t * p.hkv + h) * kLanes + part;
-    reinterpret_cast<uint4*>(p.k_out)[at] = expand8<T, BITS>(kc, ks, kz);
-    reinterpret_cast<uint4*>(p.v_out)[at] = expand8<T, BITS>(vc, vs, vz);
+    uint32_t kc[kWords], vc[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords / 2; ++i) {
+      const uint2 a = reinterpret_cast<const uint2*>(p.k_codes + row * kRowBytes)[part * (kWords / 2) + i];
+      const uint2 b = reinterpret_cast<const uint2*>(p.v_codes + row * kRowBytes)[part * (kWords / 2) + i];
+      kc[2 * i] = a.x;
+      kc[2 * i + 1] = a.y;
+      vc[2 * i] = b.x;
+      vc[2 * i + 1] = b.y;
+    }
+    give(kc, reinterpret_cast<const uint32_t*>(p.k_pairs)[row], k_to + (int64_t)h * (D / 8));
+    give(vc, reinterpret_cast<const uint32_t*>(p.v_pairs)[row], v_to + (int64_t)h * (D / 8));
   }
 }
 
 template <typename T, int D, int BITS>
 int launch(const Params& p, bool write, cudaStream_t s) {
-  const int64_t rows = write ? p.tokens * p.hkv : p.tokens;
-  int64_t blocks = (rows + 256 / (D / 8) - 1) / (256 / (D / 8));
-  if (write) {
-    const int64_t cap = (int64_t)host::sm_count() * 8;
-    if (blocks > cap) blocks = cap;
-    kv_write_kernel<T, D, BITS><<<(unsigned)blocks, 256, 0, s>>>(p);
-  } else {
-    kv_read_kernel<T, D, BITS><<<(unsigned)blocks, 256, 0, s>>>(p);
-  }
+  const int64_t rows = write ? p.tokens * p.hkv : p.tokens, per = 256 / (write ? D / 8 : D / 16);
+  const unsigned blocks = (unsigned)((rows + per - 1) / per);
+  if (write) kv_write_kernel<T, D, BITS><<<blocks, 256, 0, s>>>(p);
+  else kv_read_kernel<T, D, BITS><<<blocks, 256, 0, s>>>(p);
   return host::cuda_check(cudaGetLastError(), write ? "kv cache write launch" : "kv cache read launch");
 }
 
@@ -220,6 +300,12 @@ template <typename T>
 int dispatch(int d, int bits, const Params& p, bool write, cudaStream_t s) {
   if (d == 64) return bits == 4 ? launch<T, 64, 4>(p, write, s) : launch<T, 64, 8>(p, write, s);
   return bits == 4 ? launch<T, 128, 4>(p, write, s) : launch<T, 128, 8>(p, write, s);
+}
+
+int shift_of(int64_t page_size) {
+  for (int i = 4; i <= 20; ++i)
+    if (page_size == (1ll << i)) return i;
+  return -1;
 }
 
 int check(const char* what, int dtype, int bits, int64_t tokens, int64_t hkv, int64_t d, int64_t pages,
@@ -234,7 +320,7 @@ int check(const char* what, int dtype, int bits, int64_t tokens, int64_t hkv, in
   if (page_size <= 0 || page_size % 16 || page_size > (1 << 20))
     return fail(GKO_ERR_UNSUPPORTED, "%s: the page size must be a multiple of 16 up to 2^20 tokens, got %lld", what,
                 (long long)page_size);
-  if (tokens >= (1ll << 31) || hkv > 65535 || pages >= (1ll << 31))
+  if (tokens * hkv >= (1ll << 31) || hkv > 65535 || tokens >= (1ll << 31) || pages >= (1ll << 31))
     return fail(GKO_ERR_UNSUPPORTED, "%s: sizes out of range", what);
   return GKO_OK;
 }
@@ -272,6 +358,7 @@ extern "C" int gko_kv_cache_write(int dtype, int bits, int64_t tokens, int64_t h
   p.v_pairs = v_pairs;
   p.pages = pages;
   p.page_size = page_size;
+  p.page_shift = kv::shift_of(page_size);
   p.tokens = tokens;
   p.hkv = (int)hkv;
   p.slots = slots;
@@ -303,6 +390,7 @@ extern "C" int gko_kv_cache_read(int dtype, int bits, int64_t b, int64_t hkv, in
   p.v_pairs = const_cast<void*>(v_pairs);
   p.pages = pages;
   p.page_size = page_size;
+  p.page_shift = kv::shift_of(page_size);
   p.tokens = tokens;
   p.hkv = (int)hkv;
   p.table = table;
