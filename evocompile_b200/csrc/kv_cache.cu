@@ -32,7 +32,8 @@ struct Params {
   void* k_pairs;
   void* v_pairs;
   int64_t pages, page_size;
-  int page_shift;  // log2 of the page size, -1 when it is not a power of two
+  int page_shift, head_shift;  // log2 of the page size and of the kv heads, -1 when not a power of two
+  int side_shift;              // read: log2 of the heads of a token taken side by side
   int64_t tokens;  // write: new tokens; read: packed tokens of the destination
   int hkv;
   const int64_t* slots;  // write
@@ -71,11 +72,13 @@ __device__ __forceinline__ uint32_t as_word(P p) {
 }
 
 // -------------------------------------------------------------- write
-// kLanes = d / 8 lanes share a row, eight values (16 bytes) each. Minimum and maximum travel
-// together as one packed pair (min x, min -x), NaN kept, so a row needs log2(kLanes) shuffles.
+// d / 16 lanes share a row: 16 values each, two pieces of eight (16 bytes) half a row apart, so that a
+// warp's loads and stores are contiguous. Minimum and maximum travel together as one packed pair
+// (min x, min -x), NaN kept, so a row needs log2(d / 16) shuffles. What a row needs once (the scale's
+// division) is repeated by its lanes; with eight values a lane it was a third of the instructions.
 //
 // (x - zero) / scale is rounded to an integer without a division per value: t = (x - zero) * (1 / scale)
-// is off by less than 2^-14 (three f32 roundings of numbers up to 255), so its nearest integer is the
+// is off by less than 2^-14 (four f32 roundings of numbers up to 255), so its nearest integer is the
 // quotient's unless t is that near to a half; then the exact residual a - (c + 1/2) scale, of which one
 // fused multiply-add gives the sign, decides, and a true tie goes to the even code. Adding 1.5 * 2^23
 // rounds to an integer and leaves it in the low bits.
@@ -88,13 +91,53 @@ __device__ __forceinline__ float settle(float a, float t, float scale) {
   return c + (float)((int)c & 1);
 }
 
+// Eight of a lane's values as codes: a word of nibbles, or two of bytes.
+template <typename T, int BITS>
+__device__ __forceinline__ uint2 quantise8(const uint4& raw, float low, float scale, float inv) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float x[8], q[8], far = 0.f;
+  const uint64_t minus_low = f2pack(-low, -low), inv2 = f2pack(inv, inv), one = f2pack(-1.f, -1.f);
+  const uint64_t up2 = f2pack(kRound, kRound), down2 = f2pack(-kRound, -kRound);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    Cvt<T>::unpack(w[i], x[2 * i], x[2 * i + 1]);
+    const uint64_t t = mul2(add2(f2pack(x[2 * i], x[2 * i + 1]), minus_low), inv2);
+    const uint64_t c = add2(add2(t, up2), down2);
+    float d0, d1;
+    f2unpack(fma2(c, one, t), d0, d1);
+    f2unpack(c, q[2 * i], q[2 * i + 1]);
+    far = max3f(far, fabsf(d0), fabsf(d1));
+  }
+  if (far > 0.5f - 1e-4f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = (x[i] - low) * inv;
+      if (fabsf(t - q[i]) > 0.5f - 1e-4f) q[i] = settle(x[i] - low, t, scale);
+    }
+  }
+  uint32_t u[8];
+  if constexpr (BITS == 4) {  // two codes make a byte, still as a float
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(q[2 * i + 1], 16.f, q[2 * i]) + kRound);
+    return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410), 0u);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(q[i] + kRound);
+  return make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+}
+
 template <typename T, int BITS, int kLanes>
-__device__ __forceinline__ void quantise_row(const uint4& raw, uint8_t* codes, T* pair, int part, bool store) {
+__device__ __forceinline__ void quantise_row(const uint4 (&raw)[2], uint8_t* codes, T* pair, int part, bool store) {
   using P = typename Pair<T>::P;
   constexpr float kTop = BITS == 4 ? 15.f : 255.f;
-  const P a = as_pair<P>(raw.x), b = as_pair<P>(raw.y), c = as_pair<P>(raw.z), d = as_pair<P>(raw.w);
-  const P lo2 = __hmin2_nan(__hmin2_nan(a, b), __hmin2_nan(c, d));
-  const P hi2 = __hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d));
+  P lo2 = as_pair<P>(raw[0].x), hi2 = lo2;
+  const uint32_t rest[7] = {raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    lo2 = __hmin2_nan(lo2, as_pair<P>(rest[i]));
+    hi2 = __hmax2_nan(hi2, as_pair<P>(rest[i]));
+  }
   P both;
   both.x = __hmin_nan(lo2.x, lo2.y);
   both.y = __hneg(__hmax_nan(hi2.x, hi2.y));
@@ -105,39 +148,15 @@ __device__ __forceinline__ void quantise_row(const uint4& raw, uint8_t* codes, T
   float scale = Cvt<T>::to_f32(Pair<T>::up((high - low) / kTop));
   scale = fmaxf(scale, Pair<T>::kFloor);
   const bool fine = fabsf(low) < INFINITY && fabsf(high) < INFINITY && scale < INFINITY;
-  const float inv = 1.f / scale;
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  float x[8], q[8], far = 0.f;
+  const float inv = __fdividef(1.f, scale);  // within two units of the last place
 #pragma unroll
-  for (int i = 0; i < 4; ++i) Cvt<T>::unpack(w[i], x[2 * i], x[2 * i + 1]);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = (x[i] - low) * inv;
-    q[i] = (t + kRound) - kRound;
-    far = fmaxf(far, fabsf(t - q[i]));
+  for (int i = 0; i < 2; ++i) {
+    const uint2 w = quantise8<T, BITS>(raw[i], low, scale, inv);
+    if (!store) continue;
+    if constexpr (BITS == 4) reinterpret_cast<uint32_t*>(codes)[i * kLanes + part] = fine ? w.x : 0u;
+    else reinterpret_cast<uint2*>(codes)[i * kLanes + part] = fine ? w : make_uint2(0u, 0u);
   }
-  if (far > 0.5f - 1e-4f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float t = (x[i] - low) * inv;
-      if (fabsf(t - q[i]) > 0.5f - 1e-4f) q[i] = settle(x[i] - low, t, scale);
-    }
-  }
-  if (!store) return;
-  uint32_t u[8];
-  if constexpr (BITS == 4) {  // two codes make a byte, still as a float
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(q[2 * i + 1], 16.f, q[2 * i]) + kRound);
-    const uint32_t word = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
-    reinterpret_cast<uint32_t*>(codes)[part] = fine ? word : 0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(q[i] + kRound);
-    const uint32_t lo = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
-    const uint32_t hi = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
-    reinterpret_cast<uint2*>(codes)[part] = fine ? make_uint2(lo, hi) : make_uint2(0u, 0u);
-  }
-  if (part == 0) {
+  if (store && part == 0) {
     const float s = fine ? scale : 0.f, z = fine ? low : __int_as_float(0x7fc00000);
     *reinterpret_cast<uint32_t*>(pair) = Cvt<T>::pack(s, z);
   }
@@ -147,16 +166,18 @@ __device__ __forceinline__ void quantise_row(const uint4& raw, uint8_t* codes, T
 // shuffles need every lane.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(256) kv_write_kernel(const Params p) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   constexpr int kRowBytes = D * BITS / 8;
   const int part = threadIdx.x % kLanes;
   const unsigned r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const bool in = r < (unsigned)(p.tokens * p.hkv);
-  const unsigned t = in ? r / (unsigned)p.hkv : 0u;
+  const unsigned t = !in ? 0u : p.head_shift >= 0 ? r >> p.head_shift : r / (unsigned)p.hkv;
   const int h = in ? (int)(r - t * (unsigned)p.hkv) : 0;
   const int64_t slot = in ? p.slots[t] : -1;
-  const uint4 kx = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh + part * 8);
-  const uint4 vx = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + t * p.v_st + h * p.v_sh + part * 8);
+  const uint4* k = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + t * p.k_st + h * p.k_sh);
+  const uint4* v = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + t * p.v_st + h * p.v_sh);
+  const uint4 kx[2] = {k[part], k[kLanes + part]};
+  const uint4 vx[2] = {v[part], v[kLanes + part]};
   const bool past = slot >= p.pages * p.page_size;
   if (past && part == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
   const bool store = slot >= 0 && !past;
@@ -222,16 +243,18 @@ __device__ __forceinline__ uint4 expand8(const uint32_t* c, typename Pair<T>::P 
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// d / 16 lanes share a token and walk its heads, 16 channels each; the token's sequence is found once by
+// d / 16 lanes share a row, 16 channels each, and neighbouring groups of lanes take up to four heads of one
+// token (their rows are adjacent in the output) and walk the others; the token's sequence is found by
 // bisection. Neighbouring lanes swap halves, so that each store of the warp writes whole sectors.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
   using P = typename Pair<T>::P;
   constexpr int kLanes = D / 16;
   constexpr int kRowBytes = D * BITS / 8;
-  constexpr int kWords = 2 * BITS / 4;  // of codes per lane
+  constexpr int kWords = 2 * BITS / 4;  // of codes per lane and row
   const int part = threadIdx.x % kLanes;
-  const int64_t t = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const unsigned group = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const int64_t t = group >> p.side_shift;
   int lo = 0, hi = p.b;  // the first sequence whose end is past t
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -249,6 +272,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
   }
   const int64_t row0 = live ? page * p.hkv * p.page_size + (pos - col * (int)p.page_size) : 0;
   const bool odd = part & 1;
+  // groups of a warp may walk different numbers of heads: a swap names its own group's lanes
+  const unsigned lanes = ((1u << kLanes) - 1u) << (threadIdx.x % 32 / kLanes * kLanes);
   uint4* k_to = reinterpret_cast<uint4*>(p.k_out) + t * p.hkv * (D / 8) + (part & ~1) * 2 + odd;
   uint4* v_to = reinterpret_cast<uint4*>(p.v_out) + t * p.hkv * (D / 8) + (part & ~1) * 2 + odd;
   auto give = [&](const uint32_t (&c)[kWords], uint32_t pair, uint4* to) {
@@ -260,17 +285,18 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
     // the even lane writes the first half of its 16 channels and the first of the odd lane's, and so on
     const uint4 keep = odd ? b : a, pass = odd ? a : b;
     uint4 got;
-    got.x = __shfl_xor_sync(0xffffffffu, pass.x, 1);
-    got.y = __shfl_xor_sync(0xffffffffu, pass.y, 1);
-    got.z = __shfl_xor_sync(0xffffffffu, pass.z, 1);
-    got.w = __shfl_xor_sync(0xffffffffu, pass.w, 1);
+    got.x = __shfl_xor_sync(lanes, pass.x, 1);
+    got.y = __shfl_xor_sync(lanes, pass.y, 1);
+    got.z = __shfl_xor_sync(lanes, pass.z, 1);
+    got.w = __shfl_xor_sync(lanes, pass.w, 1);
     if (live) {
-      to[0] = odd ? got : keep;
-      to[2] = odd ? keep : got;
+      // written once, and more than the L2 holds when it matters: first to leave it
+      __stcs(to, odd ? got : keep);
+      __stcs(to + 2, odd ? keep : got);
     }
   };
-#pragma unroll 4
-  for (int h = 0; h < p.hkv; ++h) {
+#pragma unroll 2
+  for (int h = group & ((1 << p.side_shift) - 1); h < p.hkv; h += 1 << p.side_shift) {
     const int64_t row = row0 + h * p.page_size;
     uint32_t kc[kWords], vc[kWords];
 #pragma unroll
@@ -289,7 +315,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
 
 template <typename T, int D, int BITS>
 int launch(const Params& p, bool write, cudaStream_t s) {
-  const int64_t rows = write ? p.tokens * p.hkv : p.tokens, per = 256 / (write ? D / 8 : D / 16);
+  const int64_t rows = write ? p.tokens * p.hkv : p.tokens << p.side_shift, per = 256 / (D / 16);
   const unsigned blocks = (unsigned)((rows + per - 1) / per);
   if (write) kv_write_kernel<T, D, BITS><<<blocks, 256, 0, s>>>(p);
   else kv_read_kernel<T, D, BITS><<<blocks, 256, 0, s>>>(p);
@@ -302,9 +328,9 @@ int dispatch(int d, int bits, const Params& p, bool write, cudaStream_t s) {
   return bits == 4 ? launch<T, 128, 4>(p, write, s) : launch<T, 128, 8>(p, write, s);
 }
 
-int shift_of(int64_t page_size) {
-  for (int i = 4; i <= 20; ++i)
-    if (page_size == (1ll << i)) return i;
+int shift_of(int64_t n) {
+  for (int i = 0; i <= 20; ++i)
+    if (n == (1ll << i)) return i;
   return -1;
 }
 
@@ -359,6 +385,7 @@ extern "C" int gko_kv_cache_write(int dtype, int bits, int64_t tokens, int64_t h
   p.pages = pages;
   p.page_size = page_size;
   p.page_shift = kv::shift_of(page_size);
+  p.head_shift = kv::shift_of(hkv);
   p.tokens = tokens;
   p.hkv = (int)hkv;
   p.slots = slots;
@@ -391,11 +418,13 @@ extern "C" int gko_kv_cache_read(int dtype, int bits, int64_t b, int64_t hkv, in
   p.pages = pages;
   p.page_size = page_size;
   p.page_shift = kv::shift_of(page_size);
+  p.head_shift = kv::shift_of(hkv);
   p.tokens = tokens;
   p.hkv = (int)hkv;
   p.table = table;
   p.table_stride = table_stride;
   p.table_width = table_width;
+  p.side_shift = hkv >= 4 ? 2 : hkv >= 2 ? 1 : 0;
   p.cu = cu_seqlens;
   p.b = (int)b;
   p.k_out = k;
