@@ -18,7 +18,10 @@
 // With a window and sinks (leading keys that stay visible) the key tiles that hold sinks are seen by
 // every query, the others by a window of them. A sink tile's queries are split over several CTAs of
 // about a window tile's work each, first in the grid; their dk / dv parts go to the workspace in f32 and
-// a fourth kernel adds them in a fixed order.
+// a fourth kernel adds them in a fixed order. There (no bias, no softcap) dq = scale dS k also takes its keys
+// minus one vector per kv head, about their mean: each row of dS sums to zero, so the product is the same, but
+// the roundings of dS and of delta, which do not, no longer meet the keys' common part (keys with channels of
+// their own mean, |mean| about |deviation|: error of dq 0.0050 to 0.0026 in bf16).
 //
 // The main kernel is laid out around two costs of B200: shared-memory bandwidth
 // (about 128 B per clock per SM, which limits MMAs that read both operands from shared
@@ -81,6 +84,7 @@ struct Params {
   int sink_tiles;  // 128-key tiles that hold sinks (0: no tile is split)
   int pieces;      // CTAs that share a sink tile's query blocks
   int piece;       // query blocks each takes
+  const float* centre;  // kWindow: [batch x kv head][D], taken off the keys in dq
   float* parts;    // pieces > 1: [batch x kv head][sink tile][piece][dk, dv][128][D]
   const void* bias;
   int bias_mode, bias_dtype, bias_z;
@@ -118,6 +122,12 @@ struct RowParams {
   float scale;
   const int* cu_q;
   int total_q;  // varlen: packed query tokens
+  // kWindow: the keys and where the vector taken off them goes
+  const void* k;
+  int64_t k_sz, k_sh, k_ss;
+  int sk, group, total_k;
+  const int* cu_k;
+  float* centre;
 };
 
 // Rows [row0, row0 + len) of sequence b (varlen), clamped to the packed tokens [0, total):
@@ -469,6 +479,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tmem_st32(tm_row + kTmK + c * 32, w);
       }
+      if constexpr (MODE == kWindow) {
+        // from here on the shared-memory tile serves dq alone: the same row minus the centre
+        const float4* centre = reinterpret_cast<const float4*>(p.centre + (int64_t)bh * D);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint4* at = reinterpret_cast<uint4*>(sgen + L::kK + r * 128 + c * L::kChunkKV + ((i ^ (r & 7)) << 4));
+            const uint4 x = *at;
+            const float4 m0 = __ldg(centre + c * 16 + i * 2), m1 = __ldg(centre + c * 16 + i * 2 + 1);
+            float a[8];
+            Cvt<T>::unpack(x.x, a[0], a[1]);
+            Cvt<T>::unpack(x.y, a[2], a[3]);
+            Cvt<T>::unpack(x.z, a[4], a[5]);
+            Cvt<T>::unpack(x.w, a[6], a[7]);
+            *at = make_uint4(Cvt<T>::pack(a[0] - m0.x, a[1] - m0.y), Cvt<T>::pack(a[2] - m0.z, a[3] - m0.w),
+                             Cvt<T>::pack(a[4] - m1.x, a[5] - m1.y), Cvt<T>::pack(a[6] - m1.z, a[7] - m1.w));
+          }
+        fence_proxy_async_smem();
+      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -707,7 +737,7 @@ __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = Cvt<T>::to_f32(e[i]);
 }
 
-template <typename T, int D, bool VARLEN>
+template <typename T, int D, bool VARLEN, bool CENTRE>
 __global__ void __launch_bounds__(256) fmha_bwd_prep_kernel(const RowParams p) {
   const int bh = (int)blockIdx.y + (int)blockIdx.z * (int)gridDim.y;
   if (bh >= p.zh) return;
@@ -722,6 +752,30 @@ __global__ void __launch_bounds__(256) fmha_bwd_prep_kernel(const RowParams p) {
   }
   if (jb * kBM >= len_q) return;
   const int64_t tile = (VARLEN ? (int64_t)h : (int64_t)bh) * p.tiles_per_head + base + jb;
+  if constexpr (CENTRE) {
+    if (jb == 0 && h % p.group == 0) {
+      // mean of 64 keys of the head, evenly spread: any vector is right, a near one makes dq exact
+      __shared__ float sums[256];
+      int row_k0 = 0, len_k = p.sk;
+      if constexpr (VARLEN) varlen_rows(p.cu_k, zb, p.total_k, row_k0, len_k);
+      const int hk = h / p.group, d = threadIdx.x % D, g = threadIdx.x / D;
+      const T* k = reinterpret_cast<const T*>(p.k) + (VARLEN ? (int64_t)row_k0 * p.k_ss : (int64_t)zb * p.k_sz) +
+                   (int64_t)hk * p.k_sh + d;
+      float sum = 0.f;
+      if (len_k > 0)
+  #pragma unroll 8
+        for (int j = g; j < 64; j += 256 / D) {
+          const float x = Cvt<T>::to_f32(k[(int64_t)((int64_t)j * len_k >> 6) * p.k_ss]);
+          sum += fabsf(x) < 256.f ? x : 0.f;  // leaves out NaN, and what could overflow the type
+        }
+      sums[threadIdx.x] = sum;
+      __syncthreads();
+      if (threadIdx.x < D) {
+        for (int i = 1; i < 256 / D; ++i) sum += sums[threadIdx.x + i * D];
+        p.centre[((int64_t)zb * (p.hq / p.group) + hk) * D + d] = sum * (1.f / 64.f);
+      }
+    }
+  }
   // zero this block's dq accumulator
   uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + tile * (kBM * D));
   for (int i = threadIdx.x; i < kBM * D / 4; i += 256) acc[i] = make_uint4(0, 0, 0, 0);
@@ -837,10 +891,10 @@ constexpr int kMaxWindow = (1 << 30) - 1024;  // wider ones hide nothing; positi
 // window tile (at least 8), without more CTAs than two per SM, which also bounds the workspace.
 struct SinkPlan {
   int tiles, pieces, piece;
-  int64_t part_floats;
+  int64_t part_floats, centre_floats;
 };
 SinkPlan sink_plan(int64_t zh_kv, int64_t max_q, int64_t max_k, int64_t d, int causal, int window, int sinks) {
-  SinkPlan s{0, 1, 0, 0};
+  SinkPlan s{0, 1, 0, 0, 0};
   if (window <= 0 || sinks <= 0 || max_q <= 0 || max_k <= 0 || zh_kv <= 0) return s;
   const int64_t keys = sinks < max_k ? sinks : max_k;
   s.tiles = (int)((keys + kBN - 1) / kBN);
@@ -851,6 +905,7 @@ SinkPlan sink_plan(int64_t zh_kv, int64_t max_q, int64_t max_k, int64_t d, int c
   if (piece * most < blocks) piece = (blocks + most - 1) / most;
   s.pieces = (int)((blocks + piece - 1) / piece);
   s.piece = (int)piece;
+  s.centre_floats = zh_kv * d;
   if (s.pieces > 1) s.part_floats = zh_kv * s.tiles * s.pieces * 2 * kBN * d;
   return s;
 }
@@ -889,7 +944,8 @@ int run_all(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
             const Params& p, const RowParams& rp, int q_blocks, int kv_tiles, int mode, cudaStream_t s) {
   const dim3 rgrid = grid_of(q_blocks, rp.zh);
   if (q_blocks > 0) {
-    fmha_bwd_prep_kernel<T, D, VARLEN><<<rgrid, 256, 0, s>>>(rp);
+    if (rp.centre) fmha_bwd_prep_kernel<T, D, VARLEN, true><<<rgrid, 256, 0, s>>>(rp);
+    else fmha_bwd_prep_kernel<T, D, VARLEN, false><<<rgrid, 256, 0, s>>>(rp);
     int rc = host::cuda_check(cudaGetLastError(), "fmha bwd prep launch");
     if (rc) return rc;
   }
@@ -977,7 +1033,7 @@ extern "C" int64_t gko_fmha_sinks_bwd_workspace_size(int64_t batch, int64_t hq, 
   if (base < 0 || hkv <= 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || window < 0 || sinks < 0) return -1;
   const fmha_bwd::SinkPlan sp =
       fmha_bwd::sink_plan(batch * hkv, varlen ? max_seqlen_q : sq_or_tq, max_seqlen_k, d, causal, window, sinks);
-  return base + sp.part_floats * 4;
+  return base + (sp.part_floats + sp.centre_floats) * 4;
 }
 
 extern "C" int gko_fmha_sinks_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv, int64_t sq, int64_t sk, int64_t d,
@@ -1110,6 +1166,16 @@ extern "C" int gko_fmha_sinks_bwd(int dtype, int64_t z, int64_t hq, int64_t hkv,
   rp.dq_ss = dqs[2];
   rp.scale = scale;
   const int mode = fmha_bwd::mode_of(bias_mode != GKO_BIAS_NONE, softcap, window, p.sinks);
+  if (mode == fmha_bwd::kWindow) {
+    rp.k = k;
+    rp.k_sz = ks[0];
+    rp.k_sh = ks[1];
+    rp.k_ss = ks[2];
+    rp.sk = (int)sk;
+    rp.group = p.group;
+    rp.centre = p.parts + sp.part_floats;
+    p.centre = rp.centre;
+  }
   const int q_blocks = (int)((sq + fmha_bwd::kBM - 1) / fmha_bwd::kBM);
   const int kv_tiles = (int)((sk + fmha_bwd::kBN - 1) / fmha_bwd::kBN);
   return fmha_bwd::dispatch<false>(dtype, (int)d, tq, tk, tv, tdo, p, rp, q_blocks, kv_tiles, mode,
@@ -1236,6 +1302,16 @@ extern "C" int gko_fmha_sinks_varlen_bwd(int dtype, int64_t b, int64_t hq, int64
   rp.cu_q = cu_q;
   rp.total_q = (int)tq;
   const int mode = fmha_bwd::mode_of(false, softcap, window, p.sinks);
+  if (mode == fmha_bwd::kWindow) {
+    rp.k = k;
+    rp.k_sh = k_sh;
+    rp.k_ss = k_st;
+    rp.group = p.group;
+    rp.cu_k = cu_k;
+    rp.total_k = (int)tk;
+    rp.centre = p.parts + sp.part_floats;
+    p.centre = rp.centre;
+  }
   const int q_blocks = (int)((max_seqlen_q + fmha_bwd::kBM - 1) / fmha_bwd::kBM);
   const int kv_tiles = (int)((max_seqlen_k + fmha_bwd::kBN - 1) / fmha_bwd::kBN);
   return fmha_bwd::dispatch<true>(dtype, (int)d, mq, mk, mv, mdo, p, rp, q_blocks, kv_tiles, mode,

@@ -16,6 +16,7 @@ import torch
 from . import _lib
 
 _I64x4 = ctypes.c_int64 * 4
+_NO_STRIDES = _I64x4(0, 0, 0, 0)
 
 
 # Addresses go to the library as plain integers (its arguments are declared void pointers); None is NULL.
@@ -353,6 +354,15 @@ def _bias_layout(q, k, attn_bias):
     )
 
 
+def _bwd_fix(t):
+    """Unit d stride, other strides multiples of 8 elements, 16-byte aligned (else a contiguous copy)."""
+    *outer, last = t.stride()
+    low = t.data_ptr() >> 1  # in 2-byte elements: 16-byte alignment and multiples of 8 elements are one test
+    for s in outer:
+        low |= s
+    return t.contiguous() if last != 1 or low & 7 else t
+
+
 def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.0, out=None, sinks=0):
     """Fused attention forward -> (out [z, hq, sq, d], lse f32 [z * hq, sq]).
 
@@ -378,25 +388,23 @@ def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.
         scale = d ** -0.5
     dt = _lib.dtype_code(q.dtype)
 
-    def _fix(t):
-        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
-            return t.contiguous()
-        return t
-
-    q, k, v = _fix(q), _fix(k), _fix(v)
+    q, k, v = _bwd_fix(q), _bwd_fix(k), _bwd_fix(v)
     bias_t, mode, bstr, nb = _bias_layout(q, k, attn_bias)
+    ostr = None  # contiguous
     if out is None:
-        out = torch.empty((z, hq, sq, d), device=dev, dtype=q.dtype)
+        out = q.new_empty((z, hq, sq, d))
     elif out.shape != (z, hq, sq, d) or out.dtype != q.dtype or out.device != dev:
         raise RuntimeError(f"fmha: out must be [{z}, {hq}, {sq}, {d}] {q.dtype} on {dev}")
-    lse = torch.empty((z * hq, sq), device=dev, dtype=torch.float32)
+    else:
+        ostr = _I64x4(*out.stride())
+    lse = q.new_empty((z * hq, sq), dtype=torch.float32)
     if z and hq and sq:
         with _lib.on_device(dev):
             rc = _lib.load().gko_fmha_sinks_fwd(
                 dt, z, hq, hkv, sq, sk, d,
                 _ptr(q), _I64x4(*q.stride()), _ptr(k), _I64x4(*k.stride()), _ptr(v), _I64x4(*v.stride()),
                 _ptr(bias_t), mode, _lib.dtype_code(bias_t.dtype) if bias_t is not None else 0,
-                _I64x4(*bstr), nb, _I64x4(*out.stride()), float(scale), int(bool(causal)), int(window or 0),
+                _I64x4(*bstr) if mode else _NO_STRIDES, nb, ostr, float(scale), int(bool(causal)), int(window or 0),
                 float(softcap or 0.0), int(sinks or 0),
                 _ptr(out), _ptr(lse), _status_ptr(dev), _stream(dev),
             )
@@ -430,12 +438,7 @@ def fmha_varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqle
         scale = d ** -0.5
     b = cu_seqlens_q.numel() - 1
 
-    def _fix(t):
-        if t.stride(-1) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-            return t.contiguous()
-        return t
-
-    q, k, v = _fix(q), _fix(k), _fix(v)
+    q, k, v = _bwd_fix(q), _bwd_fix(k), _bwd_fix(v)
     cq = cu_seqlens_q.contiguous()
     ck = cu_seqlens_k.contiguous()
     out = torch.empty((tq, hq, d), device=dev, dtype=q.dtype)
@@ -450,13 +453,6 @@ def fmha_varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqle
             )
         _lib.check(rc, "gko_fmha_varlen_fwd")
     return out, lse
-
-
-def _bwd_fix(t):
-    """Unit d stride, other strides multiples of 8 elements, 16-byte aligned (else a contiguous copy)."""
-    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
-        return t.contiguous()
-    return t
 
 
 def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0, softcap=0.0, sinks=0):
@@ -485,9 +481,9 @@ def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0,
     q, k, v, out, dout = (_bwd_fix(t) for t in (q, k, v, out, dout))
     lse = lse.contiguous()
     bias_t, mode, bstr, nb = _bias_layout(q, k, attn_bias)
-    dq = torch.empty((z, hq, sq, d), device=dev, dtype=q.dtype)
-    dk = torch.empty((z, hkv, sk, d), device=dev, dtype=k.dtype)
-    dv = torch.empty((z, hkv, sk, d), device=dev, dtype=v.dtype)
+    dq = q.new_empty((z, hq, sq, d))
+    dk = k.new_empty((z, hkv, sk, d))
+    dv = v.new_empty((z, hkv, sk, d))
     if z and hq and (sq or sk):
         lib = _lib.load()
         with _lib.on_device(dev):
@@ -500,8 +496,9 @@ def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0,
                 dt, z, hq, hkv, sq, sk, d,
                 _ptr(q), _I64x4(*q.stride()), _ptr(k), _I64x4(*k.stride()), _ptr(v), _I64x4(*v.stride()),
                 _ptr(bias_t), mode, _lib.dtype_code(bias_t.dtype) if bias_t is not None else 0,
-                _I64x4(*bstr), nb, _ptr(out), _I64x4(*out.stride()), _ptr(dout), _I64x4(*dout.stride()),
-                _ptr(lse), float(scale), int(bool(causal)), int(window or 0), float(softcap or 0.0), int(sinks or 0),
+                _I64x4(*bstr) if mode else _NO_STRIDES, nb, _ptr(out), _I64x4(*out.stride()), _ptr(dout),
+                _I64x4(*dout.stride()), _ptr(lse), float(scale), int(bool(causal)), int(window or 0),
+                float(softcap or 0.0), int(sinks or 0),
                 _ptr(dq), _I64x4(*dq.stride()), _ptr(dk), _I64x4(*dk.stride()), _ptr(dv), _I64x4(*dv.stride()),
                 _ptr(ws), ws_bytes, _status_ptr(dev), _stream(dev),
             )
@@ -669,7 +666,7 @@ def kv_cache_read(cache, block_table, cu_seqlens, tokens, head_dim, out=None):
     b = cu_seqlens.shape[0] - 1
     block_table = _check_table("kv_cache_read", block_table, b, f"cu_seqlens of {b} sequences")
     if out is None:
-        out = tuple(torch.empty((tokens, hkv, d), device=dev, dtype=kp.dtype) for _ in range(2))
+        out = kp.new_empty((tokens, hkv, d)), kp.new_empty((tokens, hkv, d))
     for t in out:
         if t.shape != (tokens, hkv, d) or t.dtype != kp.dtype or not t.is_contiguous():
             raise RuntimeError(f"kv_cache_read: out must be two contiguous [{tokens}, {hkv}, {d}] {kp.dtype} tensors")
@@ -723,10 +720,10 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
         max_seqlen_k = block_table.shape[1] * page_size
     q = _bwd_fix(q)
     if out is None:
-        out = torch.empty((tq, hq, d), device=dev, dtype=q.dtype)
+        out = q.new_empty((tq, hq, d))
     elif out.shape != (tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
         raise RuntimeError(f"fmha_cache: out must be a contiguous [{tq}, {hq}, {d}] {q.dtype} tensor")
-    lse = torch.empty((hq, tq), device=dev, dtype=torch.float32)
+    lse = q.new_empty((hq, tq), dtype=torch.float32)
     seq_lens = seq_lens.contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
@@ -734,7 +731,7 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
                                                      int(window or 0), int(sinks or 0))
         if ws_bytes < 0:
             _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_cache_workspace_size")
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+        ws = kc.new_empty(ws_bytes) if ws_bytes else None
         rc = lib.gko_fmha_cache_fwd(
             dt, bits, b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k), _ptr(q), q.stride(0), q.stride(1),
             _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), pages, page_size, _ptr(block_table), block_table.stride(0),

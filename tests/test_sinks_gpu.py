@@ -5,7 +5,9 @@ Tolerances, element by element, from the arithmetic (u: half a step of the eleme
 
 * out: each probability is rounded to the type (u p, or 2^-25 where f16 underflows), the sum once more;
 * delta = sum(out dout) inherits out's error; dS = P (dP - delta) is rounded to the type;
-* dq, dk, dv: sums of those with exact factors, rounded once;
+* dq, dk, dv: sums of those with exact factors, rounded once. The keys of dq may be less one vector c of about their
+  mean, rounded to the type (rows of dS sum to zero): then dS's error meets |k - c| <= |k| + |c|, and each key's
+  rounding adds u |dS| (|k| + |c|); c is a mean of keys, taken here as at most twice the mean of |k|;
 * every output has a last rounding of its own: f16 holds multiples of 2^-24 below 2^-14, so one that small is off
   by up to 2^-25 whatever its size.
 """
@@ -51,7 +53,7 @@ def _head(q, k, v, dout, scale, causal, window, softcap, sinks, bias, dtype):
     e_ds = (u + 3 * e) * ds.abs() + p * (e_delta + d * 2.0 ** -24 * (dout.abs() @ v.abs().T)) + 2.0 ** -25 * (p > 0)
     e_p = (u + 3 * e) * p + 2.0 ** -25 * (p > 0)
     dq, dk, dv = scale * ds @ k, scale * ds.T @ q, p.T @ dout
-    t_dq = abs(scale) * e_ds @ k.abs() + u * dq.abs()
+    t_dq = abs(scale) * (e_ds + u * ds.abs()) @ (k.abs() + 2 * k.abs().mean(0)) + u * dq.abs()
     t_dk = abs(scale) * e_ds.T @ q.abs()
     t_dv = e_p.T @ dout.abs()
     return (out, lse, dq, dk, dv), (t_out, e + 2.0 ** -21 + 2.0 ** -22 * lse.abs(), t_dq, t_dk, t_dv)
