@@ -24,13 +24,14 @@
 //              (11 bits; the running power of two below keeps them in its range).
 //
 // Columns of a CTA are (new token, query head) pairs of one kv head, kCols at a time. A CTA takes
-// one range of keys (grid.x: column tile, then split); its warps take slabs of 32 keys in turn,
+// one range of the keys of one column tile, kv head and sequence; its warps take slabs of 32 keys in turn,
 // each with its own running maximum, sum and accumulators, and join at the end in a fixed order.
 // Every warp keeps a ring of slabs in flight for itself (bulk copies of codes and pairs into shared
 // memory, completing on an mbarrier of the warp), so the loop has no barrier between warps and the
 // memory system always has several slabs per warp to work on.
-// With more than one split the joined parts go to the workspace and a second kernel adds them,
-// again in a fixed order, so results do not vary from run to run.
+// A tile whose keys are split goes to the workspace in parts and a second kernel adds them, again in
+// a fixed order, so results do not vary from run to run. Splits follow the lengths on the device (see
+// `place`): sequences of 512 to 8192 tokens are shared out as evenly as one of 131072.
 #include <type_traits>
 
 #include "host_common.h"
@@ -42,7 +43,7 @@ namespace fmha_cache {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kSlab = 32;            // keys a warp takes at a time
-constexpr int kMaxSplitSlabs = 64;   // at most 2048 keys per split, so that one long sequence spreads
+constexpr int kMinSplit = 32, kMaxSplit = 256;  // slabs per split of a fixed grid
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;      // log2: the running maximum moves only when it grows by more
@@ -67,11 +68,15 @@ struct Params {
   const int32_t* cu_q;  // NULL: one new token per sequence
   float scale, softcap;
   int causal, window, sinks;
-  int tiles, splits, split_slabs;
+  int tiles;            // column tiles of the longest query range
+  int cols;             // columns of a tile
+  int slots;            // > 0: CTAs to share the work over, by the lengths; 0: a fixed grid of
+  int splits;           //   splits of
+  int split_slabs;      //   slabs each
   void* out;
   float* lse;
-  float* part_o;   // [splits][tq * hq][d]
-  float2* part_ml;  // [splits][tq * hq] (maximum in log2 units, sum)
+  float* part_o;    // [part][cols][d]
+  float2* part_ml;  // [part][cols] (maximum in log2 units, sum)
   unsigned* status;
 };
 
@@ -90,10 +95,7 @@ __device__ __forceinline__ Seq sequence(const Params& p, int b) {
     s.row0 = b;
     s.n = b < p.tq ? 1 : 0;
   }
-  const int64_t cap = (int64_t)p.table_width * p.page_size;
-  const int64_t len = p.lens[b];
-  s.len = (int)min(max(len, (int64_t)0), cap);
-  if (len > cap && threadIdx.x == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
+  s.len = (int)min(max((int64_t)p.lens[b], (int64_t)0), (int64_t)p.table_width * p.page_size);
   return s;
 }
 
@@ -117,6 +119,71 @@ __device__ __forceinline__ Range key_range(const Params& p, const Seq& s, int c0
   const int end = hi > 0 ? (hi + kSlab - 1) / kSlab : 0;
   r.count = r.first + max(0, end - r.lo);
   return r;
+}
+
+// -------------------------------------------------------------- who does what
+// One CTA's share: split `split` of `splits` of a column tile, `per` slabs each; its part of the
+// workspace is part0 + split * stride.
+struct Place {
+  int b, hk, tile, split, splits, per, stride;
+  int64_t part0;
+};
+
+// Even sharing over p.slots CTAs, for up to 32 sequences: lane b of every warp weighs sequence b by the
+// slabs that one of its tiles can see at most, times its tiles and kv heads. `per` is chosen so that the
+// full splits and the begun ones together come to about the slots (a tile begins half a split on
+// average), never more than slots + tiles. With id >= 0 finds the share of CTA id of the main kernel, else
+// that of sequence `of_b` (split and tile unset). Every warp works it out for itself, without a barrier:
+// the lengths are needed before anything else anyway, and the rest is a few shuffles.
+__device__ __forceinline__ bool place(const Params& p, int id, int of_b, Place& w) {
+  const int lane = threadIdx.x & 31;
+  int tiles = 0, slabs = 0;
+  if (lane < p.b) {
+    const Seq s = sequence(p, lane);
+    tiles = min((s.n * p.group + p.cols - 1) / p.cols, p.tiles);
+    slabs = (s.len + kSlab - 1) / kSlab;
+    if (p.window > 0) {
+      const int64_t span = (int64_t)p.window * (p.causal ? 1 : 2) + p.cols / p.group + 2;
+      slabs = (int)min((int64_t)slabs, span / kSlab + 2 + (p.sinks + kSlab - 1) / kSlab);
+    }
+  }
+  // in slabs of one kv head; as a float: a split may be a little longer or shorter, the same for everyone
+  const float total = (float)__reduce_add_sync(0xffffffffu, (unsigned)min((int64_t)slabs * tiles, (int64_t)1 << 26));
+  const int all = (int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * p.hkv;
+  const int room = max(p.slots - min(all, p.slots) / 2, 1);
+  const int want = (int)ceilf(total * (float)p.hkv / (float)room);
+  const int per = max((want + kWarps - 1) / kWarps * kWarps, kWarps);
+  const int splits = max(1, (slabs + per - 1) / per), mine = splits * tiles * p.hkv;
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  before -= mine;
+  const unsigned hit = __ballot_sync(0xffffffffu, id >= 0 ? id >= before && id < before + mine : lane == of_b);
+  if (hit == 0) return false;
+  const int b = __ffs(hit) - 1;
+  const int base = __shfl_sync(0xffffffffu, before, b);
+  w.b = b;
+  w.splits = __shfl_sync(0xffffffffu, splits, b);
+  w.stride = __shfl_sync(0xffffffffu, tiles, b);
+  w.per = per;
+  w.hk = w.tile = w.split = 0;
+  w.part0 = base;
+  if (id >= 0) {
+    const int rest = (id - base) / w.stride;
+    w.tile = id - base - rest * w.stride;
+    w.hk = rest / w.splits;
+    w.split = rest - w.hk * w.splits;
+    w.part0 = base + w.hk * w.splits * w.stride + w.tile;
+  }
+  return true;
+}
+
+// How many of a tile's splits hold keys (at least one: an empty row is written too).
+__device__ __forceinline__ int splits_used(const Place& w, const Range& rg) {
+  return min(max(1, (rg.count + w.per - 1) / w.per), w.splits);
 }
 
 // -------------------------------------------------------------- fragments
@@ -282,25 +349,35 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   constexpr int kWarpRows = R::kStages * R::kStage / (kPitch * 4);
   static_assert(kCols <= kWarpRows, "a warp's accumulators fit its part of the ring");
 
-  const int tile = blockIdx.x % p.tiles, split = blockIdx.x / p.tiles;
-  const int hk = blockIdx.y, b = blockIdx.z;
+  Place w;
+  if (p.slots > 0) {
+    if (!place(p, (int)blockIdx.x, 0, w)) return;
+  } else {
+    const int tile = blockIdx.x % p.tiles;
+    w = Place{(int)blockIdx.z, (int)blockIdx.y, tile, (int)blockIdx.x / p.tiles, p.splits, p.split_slabs, p.tiles,
+              ((int64_t)blockIdx.z * p.hkv + blockIdx.y) * p.splits * p.tiles + tile};
+  }
+  const int tile = w.tile, split = w.split, hk = w.hk, b = w.b;
   const Seq sq = sequence(p, b);
+  if (threadIdx.x == 0 && sq.len < p.lens[b] && p.status) atomicOr(p.status, kStatusBadIndex);
   const int c0 = tile * kCols;
   const int c1 = min(c0 + kCols, sq.n * p.group);
   if (c0 >= c1) return;
   const Range rg = key_range(p, sq, c0, c1);
-  const int v0 = split * p.split_slabs;
+  const int v0 = split * w.per;
   // the last split takes whatever is left, should a sequence be longer than the caller's bound
-  const int v1 = split == p.splits - 1 ? rg.count : min(rg.count, v0 + p.split_slabs);
+  const int v1 = split == w.splits - 1 ? rg.count : min(rg.count, v0 + w.per);
   if (v0 >= v1 && split > 0) return;
+  // part of the workspace, -1 when this CTA holds the whole tile; kept in shared memory over the loop
+  __shared__ int64_t part_s;
+  if (threadIdx.x == 0) part_s = splits_used(w, rg) == 1 ? -1 : w.part0 + (int64_t)split * w.stride;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int li = lane & 3, lj = lane >> 2;
   volatile int* abort_flag = &abort_s;
   if (threadIdx.x == 0) {
     abort_s = 0;
-    for (int w = 0; w < kWarps; ++w)
-      for (int i = 0; i < R::kStages; ++i) mbar_init(smem_u32(&bars[w][i]), 1);
+    for (int i = 0; i < kWarps * R::kStages; ++i) mbar_init(smem_u32(&bars[0][i]), 1);
     fence_mbar_init();
   }
   __syncthreads();
@@ -482,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     const bool edge = have_bits != 3 || ((t0 < whole_from || t0 + kSlab > whole_to) && t0 + kSlab > whole_sinks);
     float s[2][NT][4];
     float vs[2][2], vz[2][2], ks[2][2], kz[2][2];
-    uint32_t w[2][2][R::kKWords];
+    uint32_t kw[2][2][R::kKWords];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -493,13 +570,13 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 #pragma unroll
           for (int i = 0; i < R::kKWords / 4; ++i) {
             const uint4 x = *reinterpret_cast<const uint4*>(src + i * 64 + li * 16);
-            w[hf][r][4 * i] = x.x;
-            w[hf][r][4 * i + 1] = x.y;
-            w[hf][r][4 * i + 2] = x.z;
-            w[hf][r][4 * i + 3] = x.w;
+            kw[hf][r][4 * i] = x.x;
+            kw[hf][r][4 * i + 1] = x.y;
+            kw[hf][r][4 * i + 2] = x.z;
+            kw[hf][r][4 * i + 3] = x.w;
           }
         } else {
-          load_words<R::kKWords>(src + li * 8, w[hf][r]);
+          load_words<R::kKWords>(src + li * 8, kw[hf][r]);
         }
       }
     // S^T = K q^T, piece by piece
@@ -512,15 +589,15 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           if constexpr (BITS == 4) {
-            a[hf][0] = w[hf][0][i] & 0x0F0F0F0Fu;
-            a[hf][1] = w[hf][1][i] & 0x0F0F0F0Fu;
-            a[hf][2] = (w[hf][0][i] >> 4) & 0x0F0F0F0Fu;
-            a[hf][3] = (w[hf][1][i] >> 4) & 0x0F0F0F0Fu;
+            a[hf][0] = kw[hf][0][i] & 0x0F0F0F0Fu;
+            a[hf][1] = kw[hf][1][i] & 0x0F0F0F0Fu;
+            a[hf][2] = (kw[hf][0][i] >> 4) & 0x0F0F0F0Fu;
+            a[hf][3] = (kw[hf][1][i] >> 4) & 0x0F0F0F0Fu;
           } else {
-            a[hf][0] = w[hf][0][2 * i];
-            a[hf][1] = w[hf][1][2 * i];
-            a[hf][2] = w[hf][0][2 * i + 1];
-            a[hf][3] = w[hf][1][2 * i + 1];
+            a[hf][0] = kw[hf][0][2 * i];
+            a[hf][1] = kw[hf][1][2 * i];
+            a[hf][2] = kw[hf][0][2 * i + 1];
+            a[hf][3] = kw[hf][1][2 * i + 1];
           }
         }
 #pragma unroll
@@ -662,12 +739,12 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     // O^T += V^T P^T
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      uint32_t w[4][R::kVWords];  // keys 2i, 2i + 1, 2i + 8, 2i + 9
+      uint32_t vw[4][R::kVWords];  // keys 2i, 2i + 1, 2i + 8, 2i + 9
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         load_words<R::kVWords>(slab + R::kV + (16 * hf + key_of(2 * li + (r & 1)) + 8 * (r >> 1)) * R::kBytes +
                                    lj * (R::kBytes / 8),
-                               w[r]);
+                               vw[r]);
       }
 #pragma unroll
       for (int i = 0; i < R::kVWords; ++i) {
@@ -675,8 +752,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // channels 4 h .. 4 h + 3 of the word
             uint32_t f0[4], f1[4];
-            nibbles(__byte_perm(w[0][i], w[1][i], h ? 0x7632 : 0x5410), bits1024, f0);
-            nibbles(__byte_perm(w[2][i], w[3][i], h ? 0x7632 : 0x5410), bits1024, f1);
+            nibbles(__byte_perm(vw[0][i], vw[1][i], h ? 0x7632 : 0x5410), bits1024, f0);
+            nibbles(__byte_perm(vw[2][i], vw[3][i], h ? 0x7632 : 0x5410), bits1024, f1);
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -687,8 +764,8 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {  // channels 2 h, 2 h + 1 of the word
-            const uint32_t x = __byte_perm(w[0][i], w[1][i], h ? 0x7362 : 0x5140);
-            const uint32_t y = __byte_perm(w[2][i], w[3][i], h ? 0x7362 : 0x5140);
+            const uint32_t x = __byte_perm(vw[0][i], vw[1][i], h ? 0x7362 : 0x5140);
+            const uint32_t y = __byte_perm(vw[2][i], vw[3][i], h ? 0x7362 : 0x5140);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               mma16816(o[2 * i + h][n], bytes01(x), bytes23(x), bytes01(y), bytes23(y), pf[hf][n][0], pf[hf][n][1]);
@@ -739,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     for (int e = 0; e < 2; ++e) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][n * 8 + li * 2 + e]);
+      for (int i = 0; i < kWarps; ++i) mx = fmaxf(mx, w_max[i][n * 8 + li * 2 + e]);
       f[n][e] = fast_exp2(m[n][e] - mx) * __uint_as_float(vexp);
     }
 #pragma unroll
@@ -754,12 +831,12 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     const int rel = token_of(c), tok = tok0 + rel, head = hk * p.group + rem0 + c - rel * p.group;
     float mx = -INFINITY, sum = 0.f, zero = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, w_max[w][c]);
+    for (int i = 0; i < kWarps; ++i) mx = fmaxf(mx, w_max[i][c]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float a = fast_exp2(w_max[w][c] - mx);
-      sum += w_sum[w][c] * a;
-      zero += w_zero[w][c] * a;
+    for (int i = 0; i < kWarps; ++i) {
+      const float a = fast_exp2(w_max[i][c] - mx);
+      sum += w_sum[i][c] * a;
+      zero += w_zero[i][c] * a;
     }
     constexpr int kPer = D / 32;
     float acc[kPer];
@@ -768,14 +845,15 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
       const int ch = lane * kPer + i, at = ch % (D / 8) * 8 + ch / (D / 8);
       acc[i] = zero;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) acc[i] += o_s[w * kWarpRows + c][at];
+      for (int j = 0; j < kWarps; ++j) acc[i] += o_s[j * kWarpRows + c][at];
     }
     const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head;
-    if (p.splits > 1) {
-      float2* dst = reinterpret_cast<float2*>(p.part_o + ((int64_t)split * p.tq * p.hq + r) * D + lane * kPer);
+    if (part_s >= 0) {
+      const int64_t at = part_s * kCols + c;
+      float2* dst = reinterpret_cast<float2*>(p.part_o + at * D + lane * kPer);
 #pragma unroll
       for (int i = 0; i < kPer / 2; ++i) dst[i] = make_float2(acc[2 * i], acc[2 * i + 1]);
-      if (lane == 0) p.part_ml[(int64_t)split * p.tq * p.hq + r] = make_float2(mx, sum);
+      if (lane == 0) p.part_ml[at] = make_float2(mx, sum);
     } else {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;  // NaN stays
       uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + r * D + lane * kPer);
@@ -793,22 +871,31 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
 constexpr int kJoinWarps = 16;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const Params p, int cols, int per_row) {
+__global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const Params p, int per_row) {
   constexpr int kPer = D / 32;
   __shared__ float acc_s[kJoinWarps][D], sum_s[kJoinWarps];
   const int hk = blockIdx.y, b = blockIdx.z;
+  Place w;
+  if (p.slots > 0) {
+    place(p, -1, b, w);
+    w.part0 += (int64_t)hk * w.splits * w.stride;
+  } else {
+    w = Place{b, hk, 0, 0, p.splits, p.split_slabs, p.tiles, ((int64_t)b * p.hkv + hk) * p.splits * p.tiles};
+  }
   const Seq sq = sequence(p, b);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % per_row;
   const int col = blockIdx.x * (kJoinWarps / per_row) + warp / per_row;
   const bool in = col < sq.n * p.group;
-  const int c0 = col / cols * cols, c1 = min(c0 + cols, sq.n * p.group);
+  const int tile = col / p.cols, c0 = tile * p.cols, c1 = min(c0 + p.cols, sq.n * p.group);
   const Range rg = in ? key_range(p, sq, c0, c1) : Range{0, 0, 0};
-  const int used = in ? min(max(1, (rg.count + p.split_slabs - 1) / p.split_slabs), p.splits) : 0;
+  int used = in ? splits_used(w, rg) : 0;
+  if (used == 1) used = 0;  // written by the main kernel
   const int tok = col / p.group, head = hk * p.group + col % p.group;
-  const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head, stride = p.tq * p.hq;
+  const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head;
+  const int64_t first = (w.part0 + tile) * p.cols + col - c0, stride = (int64_t)w.stride * p.cols;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // all parts are written from here on
   float mx = kNoMax;
-  for (int s = lane; s < used; s += 32) mx = fmaxf(mx, p.part_ml[s * stride + r].x);
+  for (int s = lane; s < used; s += 32) mx = fmaxf(mx, p.part_ml[first + s * stride].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float acc[kPer], sum = 0.f;
@@ -816,10 +903,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const 
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int s = sub; s < used; s += per_row) {
-    const float2 ml = p.part_ml[s * stride + r];
+    const float2 ml = p.part_ml[first + s * stride];
     const float a = fast_exp2(ml.x - mx);
     sum += ml.y * a;
-    const float* src = p.part_o + (s * stride + r) * D;
+    const float* src = p.part_o + (first + s * stride) * D;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) acc[i] = fmaf(src[lane + 32 * i], a, acc[i]);
   }
@@ -829,13 +916,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const 
     if (lane == 0) sum_s[warp] = sum;
     __syncthreads();
     if (sub > 0) return;
-    for (int w = 1; w < per_row; ++w) {
-      sum += sum_s[warp + w];
+    for (int j = 1; j < per_row; ++j) {
+      sum += sum_s[warp + j];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[warp + w][lane + 32 * i];
+      for (int i = 0; i < kPer; ++i) acc[i] += acc_s[warp + j][lane + 32 * i];
     }
   }
-  if (!in) return;
+  if (used == 0) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* dst = reinterpret_cast<T*>(p.out) + r * D;
 #pragma unroll
@@ -845,13 +932,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const 
 
 // -------------------------------------------------------------- host side
 struct Plan {
-  int cols, tiles, splits, split_slabs;
+  int cols, tiles, slots, splits, split_slabs, likely;
+  int64_t parts;  // of the workspace
 };
 
-// Columns per CTA, column tiles and key splits. Splits fill the CTAs that every SM holds, with at least
-// a slab for each warp and at most kMaxSplitSlabs slabs each.
+// Columns per CTA, column tiles and how the keys are split:
+//   one slab per warp or less at the caller's bound: not at all (one kernel, no workspace);
+//   2 to 32 sequences with tiles for a quarter of the CTAs that the SMs hold, and 16 slabs or more for each
+//     of those: evenly over them, by the lengths on the device (16 sequences of 512 to 8192 tokens, 4 bits,
+//     GPU time: 35 us, by the caller's bound 39; working it out costs 1.3 us, so 7 sequences of 1 to 5000
+//     tokens with a window of 1000 take 14.8 against 13.6 us and stay with the next rule);
+//   few tiles otherwise: by the bound, so that the longest sequences fill those CTAs once;
+//   many tiles: so that they would fill them three times, for the tiles balance one another and a CTA costs
+//     about 5 us besides its keys (64 sequences of 8192 tokens, 4 bits: splits of 16, 32, 64 and 256 slabs
+//     196, 161, 146 and 161 us).
 Plan plan(int bits, int64_t b, int64_t hkv, int64_t group, int64_t max_q, int64_t max_k, int window, int sinks) {
-  Plan pl;
+  Plan pl{};
   const int64_t columns = max_q * group;
   pl.cols = columns <= 8 ? 8 : 16;
   pl.tiles = (int)((columns + pl.cols - 1) / pl.cols);
@@ -860,14 +956,27 @@ Plan plan(int bits, int64_t b, int64_t hkv, int64_t group, int64_t max_q, int64_
     const int64_t span = 2 * (int64_t)window + max_q + (int64_t)sinks + 3 * kSlab;
     if (span < keys) keys = span;
   }
-  const int64_t slabs = (keys + kSlab - 1) / kSlab > 0 ? (keys + kSlab - 1) / kSlab : 1;
-  const int64_t ctas = b * hkv * pl.tiles, slots = (pl.cols > 8 ? 2 : bits == 4 ? 4 : 3) * (int64_t)host::sm_count();
-  int64_t want = (slots + ctas - 1) / ctas;
-  int64_t per = (slabs + want - 1) / want;
-  if (per < kWarps) per = kWarps;
-  if (per > kMaxSplitSlabs) per = kMaxSplitSlabs;
-  pl.split_slabs = (int)per;
-  pl.splits = (int)((slabs + per - 1) / per);
+  const int64_t slabs = (keys + kSlab - 1) / kSlab;
+  const int64_t tiles = b * hkv * pl.tiles;
+  const int64_t slots = (pl.cols > 8 ? 2 : bits == 4 ? 4 : 3) * (int64_t)host::sm_count();
+  pl.splits = 1;
+  pl.split_slabs = 1 << 26;
+  if (slabs <= kWarps) return pl;
+  const bool few = tiles <= slots / 4;
+  if (!few || b == 1 || b > 32 || tiles * slabs < 16 * slots) {
+    int64_t per = tiles * slabs / (3 * slots);
+    per = per < kMinSplit ? kMinSplit : per > kMaxSplit ? kMaxSplit : per;
+    pl.splits = (int)(few ? (slots + tiles - 1) / tiles : (slabs + per - 1) / per);
+    const int64_t even = (slabs + pl.splits - 1) / pl.splits;
+    pl.split_slabs = (int)((even + kWarps - 1) / kWarps * kWarps);
+    pl.splits = pl.likely = (int)((slabs + pl.split_slabs - 1) / pl.split_slabs);
+    if (pl.splits > 1) pl.parts = tiles * pl.splits;
+    return pl;
+  }
+  pl.slots = (int)slots;
+  pl.likely = (int)((slots + tiles - 1) / tiles);
+  if (pl.likely > (slabs + kWarps - 1) / kWarps) pl.likely = (int)((slabs + kWarps - 1) / kWarps);
+  pl.parts = slots + tiles;
   return pl;
 }
 
@@ -883,7 +992,8 @@ int launch_main(const Params& p, const Plan& pl, cudaStream_t s) {
     if (e != cudaSuccess) return host::cuda_check(e, "cudaFuncSetAttribute(fmha cache)");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const dim3 grid((unsigned)(pl.tiles * pl.splits), (unsigned)p.hkv, (unsigned)p.b);
+  const dim3 grid = pl.slots > 0 ? dim3((unsigned)pl.parts)
+                                 : dim3((unsigned)(pl.tiles * pl.splits), (unsigned)p.hkv, (unsigned)p.b);
   kern<<<grid, kThreads, kBytes, s>>>(p);
   return host::cuda_check(cudaGetLastError(), "fmha cache kernel launch");
 }
@@ -891,9 +1001,9 @@ int launch_main(const Params& p, const Plan& pl, cudaStream_t s) {
 template <typename T, int D, int BITS>
 int launch(const Params& p, const Plan& pl, cudaStream_t s) {
   int rc = pl.cols == 8 ? launch_main<T, D, BITS, 1>(p, pl, s) : launch_main<T, D, BITS, 2>(p, pl, s);
-  if (rc || pl.splits == 1) return rc;
+  if (rc || pl.parts == 0) return rc;
   int per_row = 1;  // about four splits per warp
-  while (per_row < kJoinWarps && per_row * 4 < pl.splits) per_row *= 2;
+  while (per_row < kJoinWarps && per_row * 4 < pl.likely) per_row *= 2;
   const int64_t columns = (int64_t)p.max_q * p.group;
   const int rows = kJoinWarps / per_row;
   cudaLaunchConfig_t cfg{};
@@ -905,7 +1015,7 @@ int launch(const Params& p, const Plan& pl, cudaStream_t s) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  return host::cuda_check(cudaLaunchKernelEx(&cfg, fmha_cache_join_kernel<T, D>, p, pl.cols, per_row),
+  return host::cuda_check(cudaLaunchKernelEx(&cfg, fmha_cache_join_kernel<T, D>, p, per_row),
                           "fmha cache join launch");
 }
 
@@ -942,7 +1052,7 @@ extern "C" int64_t gko_fmha_cache_workspace_size(int bits, int64_t b, int64_t hq
   if ((bits != 4 && bits != 8) || fmha_cache::check_sizes(b, hq, hkv, d, tq, max_seqlen_q, max_seqlen_k, window, sinks)) return -1;
   if (b == 0 || tq == 0 || max_seqlen_q == 0) return 0;
   const fmha_cache::Plan pl = fmha_cache::plan(bits, b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
-  return pl.splits > 1 ? pl.splits * tq * hq * (d * 4 + 8) : 0;
+  return pl.parts * pl.cols * (d * 4 + 8);
 }
 
 extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
@@ -977,11 +1087,11 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
     if (!host::aligned16(x)) return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache needs 16-byte aligned tensors");
   const fmha_cache::Plan pl =
       fmha_cache::plan(bits, b, hkv, hq / hkv, max_seqlen_q, max_seqlen_k, window, sinks);
-  const int64_t need = pl.splits > 1 ? pl.splits * tq * hq * (d * 4 + 8) : 0;
+  const int64_t need = pl.parts * pl.cols * (d * 4 + 8);
   if (need > 0 && (!workspace || workspace_bytes < need || !host::aligned16(workspace)))
     return fail(GKO_ERR_INVALID, "fmha over a cache needs a 16-byte aligned workspace of %lld bytes (got %lld)",
                 (long long)need, (long long)workspace_bytes);
-  if ((int64_t)pl.tiles * pl.splits >= (1ll << 31))
+  if ((int64_t)pl.tiles * pl.splits >= (1ll << 31) || pl.parts >= (1ll << 31))
     return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: sizes out of range");
   fmha_cache::Params p{};
   p.b = (int)b;
@@ -1014,12 +1124,14 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
   p.window = window;
   p.sinks = window > 0 ? sinks : 0;
   p.tiles = pl.tiles;
+  p.cols = pl.cols;
+  p.slots = pl.slots;
   p.splits = pl.splits;
   p.split_slabs = pl.split_slabs;
   p.out = out;
   p.lse = lse;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + (int64_t)pl.splits * tq * hq * d);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + pl.parts * pl.cols * d);
   p.status = status;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == GKO_BF16 ? fmha_cache::dispatch<__nv_bfloat16>((int)d, bits, p, pl, s)

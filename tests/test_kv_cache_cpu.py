@@ -76,13 +76,21 @@ def test_nothing_to_do(lib):
 
 
 def test_workspace_rule(lib):
-    """Nothing when the keys fit one split; refused sizes give -1; a window bounds what a long cache needs."""
+    """Nothing when the keys fit one round of a CTA's warps; else a part (8 columns of d sums, a maximum and a sum)
+    for each split: of one sequence, over the 4 (8 bits: 3) CTAs of 148 SMs; of several, one for each of those CTAs
+    and each column tile, whatever the lengths; of many tiles, splits of 32 to 256 slabs. Refused sizes give -1."""
     size = lib.gko_fmha_cache_workspace_size
+    part = 8 * (128 * 4 + 8)
     assert size(4, 1, 8, 8, 128, 1, 1, 100, 0, 0) == 0
-    long_ = size(4, 1, 8, 8, 128, 1, 1, 100000, 0, 0)
-    assert long_ > 0 and long_ % (8 * (128 * 4 + 8)) == 0
-    assert size(4, 1, 8, 8, 128, 1, 1, 100000, 64, 4) <= size(4, 1, 8, 8, 128, 1, 1, 400, 0, 0)
+    assert size(4, 1, 8, 8, 128, 1, 1, 131072, 0, 0) == 74 * 8 * part
+    assert size(8, 1, 8, 8, 128, 1, 1, 131072, 0, 0) == 54 * 8 * part
+    assert size(4, 1, 8, 8, 128, 1, 1, 512, 0, 0) == 4 * 8 * part
+    assert size(4, 16, 64, 8, 128, 16, 1, 8192, 0, 0) == (4 * 148 + 128) * part
+    assert size(4, 1, 8, 8, 128, 1, 1, 100000, 10, 4) == 0
     assert size(4, 0, 8, 8, 128, 0, 1, 100000, 0, 0) == 0
+    assert size(4, 1000, 8, 8, 128, 1000, 1, 4000, 0, 0) == 0  # many tiles: only sequences past 8192 keys are split
+    assert size(4, 1000, 8, 8, 128, 1000, 1, 9000, 0, 0) == 2 * 8000 * part
+    assert size(4, 64, 64, 8, 128, 64, 1, 8192, 0, 0) == 4 * 512 * part
     assert size(4, 1, 8, 3, 128, 1, 1, 100, 0, 0) == -1
     assert size(4, 1, 8, 8, 100, 1, 1, 100, 0, 0) == -1
     assert size(5, 1, 8, 8, 128, 1, 1, 100, 0, 0) == -1
