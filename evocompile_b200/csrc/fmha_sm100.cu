@@ -45,6 +45,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleThreshold = 8.f;  // log2 units
+constexpr int kFewSinks = 32;             // sinks of a tile that takes part with 32 keys only
 constexpr int kMaxWindow = (1 << 30) - 1024;  // wider ones hide nothing; position + window stays an int
 // K tiles are double or triple buffered (V always double): the S MMA of the next key tile
 // waits on K, so a deeper K ring hides more TMA latency when shared memory allows it.
@@ -105,7 +106,8 @@ __device__ __forceinline__ float bias_value(const Params& p, int z, int h, int q
 // What the softmax of a kernel handles: kPlain an optional causal mask; kExtra also bias, softcap and
 // windows, element by element; kWindow a window with sinks and a positive scale, the scale folded into
 // the exponent as in kPlain and masks only on the key tiles that cross the edge of what a warp's rows
-// see.
+// see. Up to 32 sinks, ahead of the window, cost a quarter of a key tile: S has 32 columns, P V two steps
+// (4096 tokens, 64 heads, window 1024: 196 us with a whole tile, see the table for now).
 enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
 
 template <typename T, int D, bool VARLEN, int MODE>
@@ -148,6 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // query tile below that of the second only where it leaves the first nothing else, so the tiles of
   // both together are [0, sk) and [lo, hi) with lo >= sk.
   int lo_t[kQTiles], hi_t[kQTiles], sk_t[kQTiles];
+  bool few_t[kQTiles];  // the one sink tile has few sinks and no key of the window
 #pragma unroll
   for (int t = 0; t < kQTiles; ++t) {
     const int mt = m0 + t * kBM;
@@ -158,6 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       k_hi = min(k_hi, mt + kBM + p.window);
     }
     sk_t[t] = 0;
+    few_t[t] = false;
     if (mt >= len_q || k_hi <= k_lo) {
       lo_t[t] = hi_t[t] = 0;
     } else {
@@ -168,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (p.sinks > 0 && mt < len_q) {
         const int end = min(min(p.sinks, len_k), p.causal ? mt + kBM : len_k);
         sk_t[t] = (end + kBN - 1) / kBN;
+        few_t[t] = MODE == kWindow && p.sinks <= kFewSinks && k_lo >= kBN;
         lo_t[t] = max(lo_t[t], sk_t[t]);
         hi_t[t] = max(hi_t[t], lo_t[t]);
       }
@@ -282,14 +287,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && n_tiles > 0) {
       bool ok = wait_bounded(bar_q, 0, abort_flag, p.status, kStatusTimeoutMma);
+      auto few = [&](int t, int j) { return MODE == kWindow && few_t[t] && j < sk_t[t]; };
       auto issue_s = [&](int t, int u) {
+        const uint32_t idesc =
+            few(t, tile_at(u)) ? make_idesc_f16(kBF16, kBM, kFewSinks, false, false) : kIdescS;
         const uint32_t k_addr = sb + L::kK0 + (u % kKStages) * L::kTile;
         const uint32_t q_addr = sb + L::kQ + t * L::kTile;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (kk >> 2) * L::kChunk + (kk & 3) * 32;
           mma_f16_ss(tmem_base + t * kBN, make_sdesc_sw128(q_addr + off, 16, 1024),
-                     make_sdesc_sw128(k_addr + off, 16, 1024), kIdescS, kk > 0 ? 1u : 0u);
+                     make_sdesc_sw128(k_addr + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
         }
         mma_commit(bar_sfull + 8 * t);
       };
@@ -302,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k4 = 0; k4 < kBN / 32; ++k4) {
           const int kk = half * (kBN / 32) + k4;
+          if (kk >= kFewSinks / 16 && few(t, tile_at(u))) continue;
           mma_f16_ts(o_tmem, p_tmem + kk * 8, make_sdesc_sw128(v_addr + kk * 16 * 128, L::kChunk, 1024),
                      kIdescO, (!first || kk > 0) ? 1u : 0u);
         }
@@ -392,6 +401,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
+      if constexpr (MODE == kWindow) {
+        if (i < jsk && (t ? few_t[1] : few_t[0])) {  // the first tile: nothing to rescale yet
+          uint32_t su[kFewSinks];
+          tmem_ld32p(s_tmem, su);
+          tmem_wait_ld();
+          const int sink = min(min(p.sinks, len_k), p.causal ? qi + 1 : len_k);
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < kFewSinks; ++c) {
+            su[c] = c < sink ? su[c] : 0xff800000u;
+            top = fmaxf(top, __uint_as_float(su[c]));
+          }
+          m_run = top * p.scale_log2;
+          const float nm = (m_run == -INFINITY) ? 0.f : -m_run;
+          uint32_t pk[kFewSinks / 2];
+#pragma unroll
+          for (int c = 0; c < kFewSinks / 2; ++c) {
+            const float a = fast_exp2(fmaf(__uint_as_float(su[2 * c]), p.scale_log2, nm));
+            const float b = fast_exp2(fmaf(__uint_as_float(su[2 * c + 1]), p.scale_log2, nm));
+            l_run += a + b;
+            pk[c] = Cvt<T>::pack(a, b);
+          }
+          tmem_st16(s_tmem, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar_pfull + 16 * t);
+            mbar_arrive(bar_pfull + 16 * t + 8);
+          }
+          continue;
+        }
+      }
       float s[kBN];
       {
         uint32_t su[kBN];
@@ -424,15 +466,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rw = mt + quarter * 32;
         const int last_w = min(len_k - 1, p.causal ? rw : rw + p.window);
         const int sink_w = min(min(p.sinks, len_k), p.causal ? rw + 1 : len_k);
-        if (kbase + kBN > sink_w && (kbase + kBN - 1 > last_w || kbase < rw + 31 - p.window)) {
+        const bool late = kbase + kBN - 1 > last_w, early = kbase < rw + 31 - p.window;
+        if (kbase + kBN > sink_w && (late || early)) {
           const int last = min(len_k - 1, p.causal ? qi : qi + p.window) - kbase;
-          const int sink = min(min(p.sinks, len_k), p.causal ? qi + 1 : len_k) - kbase;
-          // [first, last] as one unsigned comparison; an empty range starts past the tile
-          const int first = last >= qi - p.window - kbase ? qi - p.window - kbase : kBN;
-          const unsigned span = last >= first ? (unsigned)(last - first) : 0u;
+          const int first = qi - p.window - kbase;
+          if (kbase < sink_w || (late && early)) {
+            const int sink = min(min(p.sinks, len_k), p.causal ? qi + 1 : len_k) - kbase;
+            // [first, last] as one unsigned comparison; an empty range starts past the tile
+            const int from = last >= first ? first : kBN;
+            const unsigned span = last >= from ? (unsigned)(last - from) : 0u;
 #pragma unroll
-          for (int c = 0; c < kBN; ++c)
-            s[c] = ((unsigned)(c - first) <= span || c < sink) ? s[c] : -INFINITY;
+            for (int c = 0; c < kBN; ++c)
+              s[c] = ((unsigned)(c - from) <= span || c < sink) ? s[c] : -INFINITY;
+          } else if (late) {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c) s[c] = (c <= last) ? s[c] : -INFINITY;
+          } else {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c) s[c] = (c >= first) ? s[c] : -INFINITY;
+          }
         }
         kmul = p.scale_log2;
       } else {
