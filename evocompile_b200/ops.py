@@ -9,6 +9,7 @@ them falls back to another implementation.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -30,6 +31,16 @@ def _status_ptr(dev):
 
 def _stream(dev):
     return _lib.stream_ptr(dev)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, device, *sizes):
+    """Bytes that the library's ``name`` asks for ``sizes`` on ``device`` (an index; it must be current: the answer
+    goes by its SMs). A pure function of its arguments, so a decode loop asks once."""
+    n = getattr(_lib.load(), name)(*sizes)
+    if n < 0:
+        _lib.check(_lib.ERR_UNSUPPORTED, name)
+    return n
 
 
 def _byte_range(t):
@@ -487,11 +498,9 @@ def fmha_bwd(q, k, v, attn_bias, out, lse, dout, scale=None, causal=0, window=0,
     if z and hq and (sq or sk):
         lib = _lib.load()
         with _lib.on_device(dev):
-            ws_bytes = lib.gko_fmha_sinks_bwd_workspace_size(z, hq, hkv, sq, sq, sk, d, int(bool(causal)),
-                                                             int(window or 0), int(sinks or 0), 0)
-            if ws_bytes < 0:
-                _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_bwd_workspace_size")
-            ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
+            ws_bytes = _workspace_bytes("gko_fmha_sinks_bwd_workspace_size", dev.index, z, hq, hkv, sq, sq, sk, d,
+                                        int(bool(causal)), int(window or 0), int(sinks or 0), 0)
+            ws = q.new_empty(max(ws_bytes // 2, 8))
             rc = lib.gko_fmha_sinks_bwd(
                 dt, z, hq, hkv, sq, sk, d,
                 _ptr(q), _I64x4(*q.stride()), _ptr(k), _I64x4(*k.stride()), _ptr(v), _I64x4(*v.stride()),
@@ -540,11 +549,10 @@ def fmha_varlen_bwd(q, k, v, out, lse, dout, cu_seqlens_q, cu_seqlens_k, max_seq
     if b and hq and (tq or tk):
         lib = _lib.load()
         with _lib.on_device(dev):
-            ws_bytes = lib.gko_fmha_sinks_bwd_workspace_size(b, hq, hkv, tq, int(max_seqlen_q), int(max_seqlen_k), d,
-                                                             int(bool(causal)), int(window or 0), int(sinks or 0), 1)
-            if ws_bytes < 0:
-                _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_bwd_workspace_size")
-            ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
+            ws_bytes = _workspace_bytes("gko_fmha_sinks_bwd_workspace_size", dev.index, b, hq, hkv, tq,
+                                        int(max_seqlen_q), int(max_seqlen_k), d, int(bool(causal)), int(window or 0),
+                                        int(sinks or 0), 1)
+            ws = q.new_empty(max(ws_bytes // 2, 8))
             rc = lib.gko_fmha_sinks_varlen_bwd(
                 _lib.dtype_code(q.dtype), b, hq, hkv, d, tq, tk, int(max_seqlen_q), int(max_seqlen_k),
                 _ptr(q), q.stride(0), q.stride(1), _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0),
@@ -588,19 +596,20 @@ def kv_cache_alloc(pages, page_size, kv_heads, head_dim, bits=4, dtype=torch.bfl
     return KVCache(codes(), codes(), pairs(), pairs())
 
 
-def _cache_layout(name, cache, hkv=None, d=None, dtype=None):
-    """(dtype code, bits, kv heads, d) of a cache whose four tensors fit together and, where given, k and v."""
+def _cache_layout(name, cache, hkv=None, dtype=None):
+    """Type code of a cache whose four tensors fit together and, where given, its kv heads and element type."""
     kc, vc, kp, vp = cache
-    if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or kc.dim() != 4 or kc.shape != vc.shape:
+    codes, pairs = kc.shape, kp.shape
+    if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or len(codes) != 4 or vc.shape != codes:
         raise RuntimeError(f"{name}: codes must be two uint8 [pages, kv heads, page, bytes] tensors of one shape")
-    if kp.shape != (*kc.shape[:3], 2) or vp.shape != kp.shape or kp.dtype != vp.dtype:
+    if pairs[:3] != codes[:3] or pairs[3:] != (2,) or vp.shape != pairs or kp.dtype != vp.dtype:
         raise RuntimeError(f"{name}: pairs must be two [pages, kv heads, page, 2] tensors of one type")
     if not (kc.is_contiguous() and vc.is_contiguous() and kp.is_contiguous() and vp.is_contiguous()):
         raise RuntimeError(f"{name}: the cache's tensors must be contiguous")
     if dtype is not None and kp.dtype != dtype:
         raise RuntimeError(f"{name}: the cache holds {kp.dtype}, got {dtype}")
-    if hkv is not None and kc.shape[1] != hkv:
-        raise RuntimeError(f"{name}: the cache has {kc.shape[1]} kv heads, got {hkv}")
+    if hkv is not None and codes[1] != hkv:
+        raise RuntimeError(f"{name}: the cache has {codes[1]} kv heads, got {hkv}")
     return _lib.dtype_code(kp.dtype)
 
 
@@ -625,7 +634,7 @@ def kv_cache_write(k, v, cache, slots):
     if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
         raise RuntimeError("kv_cache_write: k and v must be two [tokens, kv heads, d] tensors of one type")
     t, hkv, d = k.shape
-    dt = _cache_layout("kv_cache_write", cache, hkv, d, k.dtype)
+    dt = _cache_layout("kv_cache_write", cache, hkv, k.dtype)
     bits = _cache_bits("kv_cache_write", kc.shape[3], d)
     if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != t:
         raise RuntimeError(f"kv_cache_write: slots must be int64 [{t}], got {slots.dtype} {tuple(slots.shape)}")
@@ -699,7 +708,7 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
     if q.dim() != 3:
         raise RuntimeError("fmha_cache: q must be 3-D [tokens, heads, d]")
     tq, hq, d = q.shape
-    dt = _cache_layout("fmha_cache", cache, None, None, q.dtype)
+    dt = _cache_layout("fmha_cache", cache, None, q.dtype)
     pages, hkv, page_size, row = kc.shape
     bits = _cache_bits("fmha_cache", row, d)
     if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1:
@@ -727,10 +736,8 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
     seq_lens = seq_lens.contiguous()
     lib = _lib.load()
     with _lib.on_device(dev):
-        ws_bytes = lib.gko_fmha_cache_workspace_size(bits, b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k),
-                                                     int(window or 0), int(sinks or 0))
-        if ws_bytes < 0:
-            _lib.check(_lib.ERR_UNSUPPORTED, "gko_fmha_cache_workspace_size")
+        ws_bytes = _workspace_bytes("gko_fmha_cache_workspace_size", dev.index, bits, b, hq, hkv, d, tq,
+                                    int(max_seqlen_q), int(max_seqlen_k), int(window or 0), int(sinks or 0))
         ws = kc.new_empty(ws_bytes) if ws_bytes else None
         rc = lib.gko_fmha_cache_fwd(
             dt, bits, b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k), _ptr(q), q.stride(0), q.stride(1),
