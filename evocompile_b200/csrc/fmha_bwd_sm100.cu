@@ -20,8 +20,10 @@
 // about a window tile's work each, first in the grid; their dk / dv parts go to the workspace in f32 and
 // a fourth kernel adds them in a fixed order. There (no bias, no softcap) dq = scale dS k also takes its keys
 // minus one vector per kv head, about their mean: each row of dS sums to zero, so the product is the same, but
-// the roundings of dS and of delta, which do not, no longer meet the keys' common part (keys with channels of
-// their own mean, |mean| about |deviation|: error of dq 0.0050 to 0.0026 in bf16).
+// the roundings of dS and of delta, which do not, no longer meet the keys' common part (keys whose channels have
+// means of 1.5 deviations: relative error of dq 0.0050 to 0.0029 in bf16).
+// 4096 tokens, 32 / 8 heads of 128, window 512, 4 sinks: 223 us at the main loop's rate, about 2.3 us for each of a
+// CTA's 44 steps; the sinks' pieces are 48 of its 296 CTAs.
 //
 // The main kernel is laid out around two costs of B200: shared-memory bandwidth
 // (about 128 B per clock per SM, which limits MMAs that read both operands from shared

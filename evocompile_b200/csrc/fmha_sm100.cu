@@ -62,7 +62,8 @@ constexpr int kKStages = GKO_FMHA_K_STAGES;
 struct Params {
   int hq, hkv, group;  // group = hq / hkv
   int sq, sk;          // dense: per-batch lengths; varlen: unused
-  int q_tiles;         // 256-row query blocks along the query axis (grid.x)
+  int q_tiles;         // query blocks along the query axis (grid.x)
+  int half;            // kWindow: query blocks of 128 rows, the second tile unused (else 256 rows)
   int zh;              // batch (or sequences) x query heads
   float scale, scale_log2, softcap;
   int causal, window, sinks;  // sinks: leading keys that the window does not hide (0 without a window)
@@ -106,8 +107,11 @@ __device__ __forceinline__ float bias_value(const Params& p, int z, int h, int q
 // What the softmax of a kernel handles: kPlain an optional causal mask; kExtra also bias, softcap and
 // windows, element by element; kWindow a window with sinks and a positive scale, the scale folded into
 // the exponent as in kPlain and masks only on the key tiles that cross the edge of what a warp's rows
-// see. Up to 32 sinks, ahead of the window, cost a quarter of a key tile: S has 32 columns, P V two steps
-// (4096 tokens, 64 heads, window 1024: 196 us with a whole tile, see the table for now).
+// see. Up to 32 sinks, ahead of the window, cost a quarter of a key tile: S has 32 columns, P V two steps.
+// Bound by the chain S -> softmax -> P -> P V of each key tile, as kPlain is (its rate on dense causal
+// attention, 0.9 PFLOP/s, is what the tiles here run at too); the window leaves 9 to 10 tiles per block.
+// 4096 tokens, 64 / 8 heads of 128, window 1024, 4 sinks: 179 us, 0.68 PFLOP/s of visible pairs (196 us with a
+// whole tile for the sinks and one mask for every edge); kExtra takes some ten times as long.
 enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
 
 template <typename T, int D, bool VARLEN, int MODE>
@@ -128,7 +132,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h = bh % p.hq;
   const int zb = bh / p.hq;  // batch (dense) or sequence (varlen)
   const int qb = p.q_tiles - 1 - (int)blockIdx.x;
-  const int m0 = qb * kBlockM;
+  const bool half = MODE == kWindow && p.half;
+  const int m0 = qb * (half ? kBM : kBlockM);
   int len_q, len_k, row_q0, row_k0;
   if constexpr (VARLEN) {
     row_q0 = p.cu_q[zb];
@@ -162,14 +167,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     sk_t[t] = 0;
     few_t[t] = false;
-    if (mt >= len_q || k_hi <= k_lo) {
+    const bool idle = mt >= len_q || (half && t > 0);
+    if (idle || k_hi <= k_lo) {
       lo_t[t] = hi_t[t] = 0;
     } else {
       lo_t[t] = k_lo / kBN;
       hi_t[t] = (k_hi + kBN - 1) / kBN;
     }
     if constexpr (MODE != kPlain) {
-      if (p.sinks > 0 && mt < len_q) {
+      if (p.sinks > 0 && !idle) {
         const int end = min(min(p.sinks, len_k), p.causal ? mt + kBM : len_k);
         sk_t[t] = (end + kBN - 1) / kBN;
         few_t[t] = MODE == kWindow && p.sinks <= kFewSinks && k_lo >= kBN;
@@ -566,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
     }
     // varlen: rows outside [0, total_q) (cu_seqlens past the packed tokens) are never written
-    const bool write = qi < len_q && (!VARLEN || (row_q0 >= 0 && row_q0 + qi < p.total_q));
+    const bool write = qi < len_q && !(half && t > 0) && (!VARLEN || (row_q0 >= 0 && row_q0 + qi < p.total_q));
     T* orow;
     if constexpr (VARLEN)
       orow = reinterpret_cast<T*>(p.out) + ((int64_t)(row_q0 + qi) * p.hq + h) * D;
@@ -652,6 +658,13 @@ int mode_of(bool bias, float softcap, int window, int sinks, float scale) {
   if (window > 0) return sinks > 0 && scale > 0.f ? kWindow : kExtra;
   return kPlain;
 }
+
+// Whether windows with sinks take query blocks of 128 rows: where blocks of 256 would leave half of the
+// SMs idle. A lone tile cannot hide its softmax behind another's products, but the CTAs run side by side
+// (2 x 8 heads, 1000 queries, 1777 keys, window 300 both ways: 27.6 us with 256 rows, 21.9 with 128; 12 heads,
+// 513 tokens, window 128: 11.6 and 8.5 us). With more blocks than that 256 rows are faster: K and V are
+// fetched half as often.
+bool half_blocks(int mode, int64_t blocks) { return mode == kWindow && 2 * blocks <= host::sm_count(); }
 
 // Grid: query blocks along x, (batch, head) pairs along y (and z beyond 65535).
 dim3 grid_of(int q_blocks, int zh) {
@@ -780,6 +793,8 @@ extern "C" int gko_fmha_sinks_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv,
   p.status = status;
   const int mode = fmha::mode_of(bias_mode != GKO_BIAS_NONE, softcap, window, p.sinks, scale);
   p.zh = (int)(z * hq);
+  p.half = fmha::half_blocks(mode, (int64_t)p.q_tiles * p.zh);
+  if (p.half) p.q_tiles = (int)((sq + fmha::kBM - 1) / fmha::kBM);
   const dim3 grid = fmha::grid_of(p.q_tiles, p.zh);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, false>((int)d, mode, tq, tk, tv, p, grid, s);
@@ -848,6 +863,8 @@ extern "C" int gko_fmha_sinks_varlen_fwd(int dtype, int64_t b, int64_t hq, int64
   p.status = status;
   const int mode = fmha::mode_of(false, softcap, window, p.sinks, scale);
   p.zh = (int)(b * hq);
+  p.half = fmha::half_blocks(mode, (int64_t)p.q_tiles * p.zh);
+  if (p.half) p.q_tiles = (int)((max_seqlen_q + fmha::kBM - 1) / fmha::kBM);
   const dim3 grid = fmha::grid_of(p.q_tiles, p.zh);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, true>((int)d, mode, mq, mk, mv, p, grid, s);

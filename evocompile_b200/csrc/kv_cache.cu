@@ -13,8 +13,13 @@
 //
 // Codes are [pages, kv heads, page, d * bits / 8] bytes (4 bits: channel 2i in the low half of
 // byte i), pairs [pages, kv heads, page, 2]; the rows of one page and head are contiguous, which
-// is what the attention over the cache reads in one bulk copy. Both kernels are bound by memory:
-// a row costs 2 d bytes on one side and d * bits / 8 + 4 on the other.
+// is what the attention over the cache reads in one bulk copy. A row costs 2 d bytes on one side and
+// d * bits / 8 + 4 on the other, and both kernels are meant to be bound by that. Measured, 8 heads of 128:
+//   read, 16 sequences, 70 k tokens, 4 bits   78 us, 5.25 TB/s (80 % of a copy's rate; three of four bytes
+//                                             are written); 108 us with one value at a time in f32
+//   write, 16 k tokens, f16, 8 bits           about 20 us, 5 TB/s, issue slots three quarters full;
+//                                             some 40 us with a division per value and eight values a lane
+//   write and read back of those              37 us
 #include <type_traits>
 
 #include "host_common.h"
