@@ -1045,7 +1045,7 @@ int check_sizes(int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq, int64
                 (long long)hkv);
   if (b < 0 || tq < 0 || max_q < 0 || max_k < 0 || window < 0 || sinks < 0)
     return fail(GKO_ERR_INVALID, "fmha over a cache: negative size, window or sinks");
-  if (b > 65535 || hkv > 65535 || tq * hq >= (1ll << 31) || max_q * (hq / hkv) >= (1 << 24) || max_k > (1 << 30) ||
+  if (b > 65535 || hkv > 65535 || tq * hq >= (1ll << 31) || hq / hkv > 65536 || max_q * (hq / hkv) >= (1 << 24) || max_k > (1 << 30) ||
       window > (1 << 30) || sinks > (1 << 30))
     return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: sizes out of range");
   return GKO_OK;
@@ -1088,7 +1088,7 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
   if (table_width * page_size >= (1ll << 31) || pages >= (1ll << 31))
     return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: a sequence may hold fewer than 2^31 tokens");
   if (b == 0 || tq == 0 || max_seqlen_q == 0) return GKO_OK;
-  if (!q || !k_codes || !v_codes || !k_pairs || !v_pairs || !table || !seq_lens || !out || !lse)
+  if (!q || !k_codes || !v_codes || !k_pairs || !v_pairs || (!table && table_width > 0) || !seq_lens || !out || !lse)
     return fail(GKO_ERR_INVALID, "fmha over a cache: null pointer argument");
   if (q_st % 8 || q_sh % 8)
     return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache needs token / head strides that are multiples of 8");

@@ -42,6 +42,9 @@ bool encode_tmap(CUtensorMap* map, int dtype, int rank, const void* base, const 
 // Checks that a pointer is 16-byte aligned.
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Checks that a pointer is 32-byte aligned (the widest global store).
+inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
+
 inline int cuda_check(cudaError_t e, const char* what) {
   if (e != cudaSuccess) return fail(GKO_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return GKO_OK;

@@ -15,11 +15,11 @@
 // byte i), pairs [pages, kv heads, page, 2]; the rows of one page and head are contiguous, which
 // is what the attention over the cache reads in one bulk copy. A row costs 2 d bytes on one side and
 // d * bits / 8 + 4 on the other, and both kernels are meant to be bound by that. Measured, 8 heads of 128:
-//   read, 16 sequences, 70 k tokens, 4 bits   78 us, 5.25 TB/s (80 % of a copy's rate; three of four bytes
-//                                             are written); 108 us with one value at a time in f32
+//   read, 16 sequences, 70 k tokens, 4 bits   68 us, 6.0 TB/s (92 % of a copy's rate); 108 us with one value
+//                                             at a time in f32
 //   write, 16 k tokens, f16, 8 bits           about 20 us, 5 TB/s, issue slots three quarters full;
 //                                             some 40 us with a division per value and eight values a lane
-//   write and read back of those              37 us
+//   write and read back of those              36 us
 #include <type_traits>
 
 #include "host_common.h"
@@ -250,7 +250,8 @@ __device__ __forceinline__ uint4 expand8(const uint32_t* c, typename Pair<T>::P 
 
 // d / 16 lanes share a row, 16 channels each, and neighbouring groups of lanes take up to four heads of one
 // token (their rows are adjacent in the output) and walk the others; the token's sequence is found by
-// bisection. Neighbouring lanes swap halves, so that each store of the warp writes whole sectors.
+// bisection. A lane's 16 values leave in one 32-byte store, a whole sector (as two 16-byte stores, with
+// neighbours swapping halves to fill sectors, 70 k tokens took 78 us instead of 68).
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
   using P = typename Pair<T>::P;
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
     else lo = mid + 1;
   }
   // behind the last sequence: left as it is
-  bool live = t < p.tokens && lo < p.b && p.cu[lo] <= t;
+  bool live = t < p.tokens && lo < p.b && p.cu[lo] <= t && p.cu[lo] >= 0;
   const int pos = live ? (int)t - p.cu[lo] : 0;
   const int col = p.page_shift >= 0 ? pos >> p.page_shift : pos / (int)p.page_size;
   const int64_t page = live && col < p.table_width ? p.table[lo * p.table_stride + col] : -1;
@@ -276,29 +277,16 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const Params p) {
     live = false;
   }
   const int64_t row0 = live ? page * p.hkv * p.page_size + (pos - col * (int)p.page_size) : 0;
-  const bool odd = part & 1;
-  // groups of a warp may walk different numbers of heads: a swap names its own group's lanes
-  const unsigned lanes = ((1u << kLanes) - 1u) << (threadIdx.x % 32 / kLanes * kLanes);
-  uint4* k_to = reinterpret_cast<uint4*>(p.k_out) + t * p.hkv * (D / 8) + (part & ~1) * 2 + odd;
-  uint4* v_to = reinterpret_cast<uint4*>(p.v_out) + t * p.hkv * (D / 8) + (part & ~1) * 2 + odd;
+  uint4* k_to = reinterpret_cast<uint4*>(p.k_out) + t * p.hkv * (D / 8) + part * 2;
+  uint4* v_to = reinterpret_cast<uint4*>(p.v_out) + t * p.hkv * (D / 8) + part * 2;
   auto give = [&](const uint32_t (&c)[kWords], uint32_t pair, uint4* to) {
     const P sz = as_pair<P>(pair);
     P s, z;
     s.x = s.y = sz.x;
     z.x = z.y = sz.y;
     const uint4 a = expand8<T, BITS>(c, s, z), b = expand8<T, BITS>(c + kWords / 2, s, z);
-    // the even lane writes the first half of its 16 channels and the first of the odd lane's, and so on
-    const uint4 keep = odd ? b : a, pass = odd ? a : b;
-    uint4 got;
-    got.x = __shfl_xor_sync(lanes, pass.x, 1);
-    got.y = __shfl_xor_sync(lanes, pass.y, 1);
-    got.z = __shfl_xor_sync(lanes, pass.z, 1);
-    got.w = __shfl_xor_sync(lanes, pass.w, 1);
-    if (live) {
-      // written once, and more than the L2 holds when it matters: first to leave it
-      __stcs(to, odd ? got : keep);
-      __stcs(to + 2, odd ? keep : got);
-    }
+    // written once, and more than the L2 holds when it matters: first to leave it
+    if (live) st_global_cs_v8(to, a, b);
   };
 #pragma unroll 2
   for (int h = group & ((1 << p.side_shift) - 1); h < p.hkv; h += 1 << p.side_shift) {
@@ -410,11 +398,13 @@ extern "C" int gko_kv_cache_read(int dtype, int bits, int64_t b, int64_t hkv, in
   if (b < 0 || b >= (1ll << 31) || table_width < 0 || table_stride < 0)
     return fail(GKO_ERR_INVALID, "kv cache read: bad sizes");
   if (b == 0 || tokens == 0) return GKO_OK;
-  if (!k_codes || !v_codes || !k_pairs || !v_pairs || !table || !cu_seqlens || !k || !v)
+  if (!k_codes || !v_codes || !k_pairs || !v_pairs || (!table && table_width > 0) || !cu_seqlens || !k || !v)
     return fail(GKO_ERR_INVALID, "kv cache read: null pointer argument");
   const void* ptrs[6] = {k, v, k_codes, v_codes, k_pairs, v_pairs};
   for (const void* x : ptrs)
     if (!host::aligned16(x)) return fail(GKO_ERR_UNSUPPORTED, "kv cache read needs 16-byte aligned tensors");
+  if (!host::aligned32(k) || !host::aligned32(v))
+    return fail(GKO_ERR_UNSUPPORTED, "kv cache read needs 32-byte aligned k and v");
   kv::Params p{};
   p.k_codes = static_cast<uint8_t*>(const_cast<void*>(k_codes));
   p.v_codes = static_cast<uint8_t*>(const_cast<void*>(v_codes));

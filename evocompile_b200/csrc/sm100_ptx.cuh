@@ -411,6 +411,12 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   return v;
 }
 
+// 32 bytes, one L2 sector, in one store (32-byte aligned), first to leave the L2.
+__device__ __forceinline__ void st_global_cs_v8(void* dst, const uint4& a, const uint4& b) {
+  asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(a.x), "r"(a.y),
+               "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
 // ---------------------------------------------------------------- cross-GPU reductions (NVLink)
 // dst[0..8) += v (8 packed bf16 / f16) on every GPU bound to the NVLink multicast address
 // `mc`: one in-switch reduction (NVLS) per 16 bytes.

@@ -354,7 +354,7 @@ int gko_linear_allreduce(int dtype, int64_t m, int64_t n, int64_t k, const void*
  *
  * gko_kv_cache_read: token i of sequence s is at place i % page_size of page table[s, i / page_size]
  * (row stride table_stride, table_width columns). Sequence s goes to rows [cu_seqlens[s],
- * cu_seqlens[s + 1]) of the contiguous k and v [tokens, hkv, d]; rows of no sequence, and rows whose
+ * cu_seqlens[s + 1]) of the contiguous, 32-byte aligned k and v [tokens, hkv, d]; rows of no sequence, and rows whose
  * page is outside [0, pages) or the table (GKO_STATUS_BAD_INDEX), are left as they were.
  */
 int gko_kv_cache_write(int dtype, int bits, int64_t tokens, int64_t hkv, int64_t d, const void* k, int64_t k_st,

@@ -47,6 +47,7 @@ def _attend(lib, dtype=_lib.BF16, bits=4, b=2, hq=4, hkv=2, d=64, tq=2, max_q=1,
     (_read, dict(b=-1), _lib.ERR_INVALID, "bad sizes"),
     (_read, dict(table=0), _lib.ERR_INVALID, "null"),
     (_read, dict(out=(1 << 20) + 2), _lib.ERR_UNSUPPORTED, "16-byte"),
+    (_read, dict(out=(1 << 20) + 16), _lib.ERR_UNSUPPORTED, "32-byte"),
     (_attend, dict(dtype=_lib.F32), _lib.ERR_UNSUPPORTED, "float16 and bfloat16"),
     (_attend, dict(bits=16), _lib.ERR_UNSUPPORTED, "4 or 8 bits"),
     (_attend, dict(d=256), _lib.ERR_UNSUPPORTED, "head dim"),

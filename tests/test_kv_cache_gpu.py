@@ -291,6 +291,49 @@ def test_attend_bad_values_and_pages():
     assert _same(got, base)
 
 
+def test_empty_tables():
+    """No sequence has a token yet: a block table of no columns, rows of zeros and -inf, nothing read back."""
+    cache = ops.kv_cache_alloc(2, 16, 2, 64, 4)
+    q = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=DEV)
+    table, lens = torch.empty(3, 0, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    out, lse = ops.fmha_cache_fwd(q, cache, table, lens)
+    assert not out.any() and (lse == -float("inf")).all()
+    back = tuple(torch.full((2, 2, 64), 7.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ops.kv_cache_read(cache, table, torch.zeros(4, dtype=torch.int32, device=DEV), 2, 64, out=back)
+    ops.kv_cache_write(q[:0, :2], q[:0, :2], cache, torch.empty(0, dtype=torch.int64, device=DEV))
+    _status_clear()
+    assert (back[0] == 7.0).all() and (back[1] == 7.0).all()
+
+
+def test_many_sequences():
+    """More than 32 sequences, and more column tiles than CTAs: the fixed splits."""
+    gen = torch.Generator().manual_seed(31)
+    lens = torch.randint(0, 700, (40,), generator=gen).tolist()
+    lens[7] = 9000
+    _attend(gen, lens, [1] * 40, 32, 8, 8, 64, 4, torch.bfloat16)
+    _attend(gen, lens[:20], [9] * 20, 32, 32, 2, 64, 8, torch.float16, window=200, sinks=3)
+
+
+def test_two_streams_at_once():
+    """Two calls in flight on two streams, each with its own workspace, equal the calls made alone."""
+    gen = torch.Generator().manual_seed(32)
+    lens = [3000, 40, 900]
+    cache, table = _cache(gen, lens, 64, 2, 128, 4, torch.bfloat16)
+    cache, table, ln = _to(cache), table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    qs = [_rows(gen, 3, 8, 128, dtype=torch.bfloat16).to(DEV) for _ in range(2)]
+    alone = [ops.fmha_cache_fwd(q, cache, table, ln) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.fmha_cache_fwd(qs[i], cache, table, ln))
+    _status_clear()
+    for i in range(2):
+        assert all(_same(o, alone[i][0]) and _same(l, alone[i][1]) for o, l in got[i])
+
+
 def test_attend_rows_of_no_sequence_and_strides():
     """q as a column range of a projection output; rows behind the last sequence keep what out had."""
     gen = torch.Generator().manual_seed(14)
