@@ -167,6 +167,28 @@ def load():
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The compiled tensor-level host code (binding/gko_torch.cpp), loaded once; it links the same library."""
+    global _binding
+    if _binding is None:
+        load()
+        try:
+            from . import _gko_torch
+        except ImportError as e:
+            raise RuntimeError("evocompile_b200/_gko_torch.so is not built; run `python -m evocompile_b200.build` "
+                               f"(the operators have no fallback implementation): {e}") from None
+        _binding = _gko_torch
+    return _binding
+
+
+def status_address(t: torch.Tensor) -> int:
+    """Address of the status word of ``t``'s device, 0 for a tensor that is on none (it is refused further on)."""
+    return status_word(t.device).data_ptr() if t.is_cuda else 0
+
+
 def last_error() -> str:
     msg = load().gko_last_error()
     return msg.decode() if msg else ""

@@ -1,0 +1,309 @@
+// Tensor-level host code of the cache operators and of windowed attention with sinks, compiled: argument
+// checks, output and workspace allocation and the call of the C ABI on the current stream, and the
+// attention's gradient as a C++ autograd node. What evocompile_b200/ops.py does in Python for the other
+// operators; here because one new token per sequence is answered in less time than Python and ctypes need
+// to ask for it (host time per call: a cache attention 28 us in Python, a training step of 333 tokens, whose
+// backward runs on autograd's own thread, 178 us).
+#include <torch/extension.h>
+
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <cmath>
+#include <stdexcept>
+#include <string>
+#include <tuple>
+
+#include "../../include/gko_b200.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+[[noreturn]] void refuse(const std::string& text) { throw std::runtime_error(text); }
+
+void check(int rc, const char* what) {
+  if (rc == GKO_OK) return;
+  const char* kind = rc == GKO_ERR_INVALID       ? "invalid argument"
+                     : rc == GKO_ERR_UNSUPPORTED ? "unsupported input"
+                                                 : "CUDA error";
+  refuse(std::string(what) + ": " + kind + ": " + gko_last_error());
+}
+
+// The operands' device is made current for the call; launches go to torch's current stream on it.
+struct OnDevice {
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit OnDevice(const Tensor& t)
+      : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+
+template <typename... Ts>
+void same_device(const Tensor& first, const Ts&... rest) {
+  auto one = [&](const Tensor& t) {
+    if (!t.is_cuda())
+      refuse("gko fused operators run only on CUDA tensors (sm_100a); got a tensor on " + t.device().str() +
+             " — there is no CPU fallback");
+    if (t.device() != first.device())
+      refuse("operands on different devices: " + first.device().str() + " and " + t.device().str());
+  };
+  one(first);
+  (one(rest), ...);
+}
+
+int dtype_code(at::ScalarType t) {
+  if (t == at::kBFloat16) return GKO_BF16;
+  if (t == at::kHalf) return GKO_F16;
+  refuse(std::string("unsupported dtype ") + c10::toString(t) + "; attention and the cache take float16 or bfloat16");
+}
+
+// Unit stride along the last dimension, the others multiples of 8 elements, 16-byte aligned; else a copy.
+Tensor fixed(const Tensor& t) {
+  const auto s = t.strides();
+  int64_t low = static_cast<int64_t>(reinterpret_cast<uintptr_t>(t.data_ptr()) >> 1);
+  for (size_t i = 0; i + 1 < s.size(); ++i) low |= s[i];
+  return s.back() != 1 || (low & 7) ? t.contiguous() : t;
+}
+
+unsigned* status_word(int64_t address) { return reinterpret_cast<unsigned*>(address); }
+
+// ---------------------------------------------------------------- cache
+struct Cache {
+  const Tensor &kc, &vc, &kp, &vp;
+  int dtype, bits;
+  int64_t pages, hkv, page, d;
+  Cache(const char* name, const Tensor& k_codes, const Tensor& v_codes, const Tensor& k_pairs, const Tensor& v_pairs,
+        int64_t head_dim)
+      : kc(k_codes), vc(v_codes), kp(k_pairs), vp(v_pairs), d(head_dim) {
+    const std::string n(name);
+    if (kc.scalar_type() != at::kByte || vc.scalar_type() != at::kByte || kc.dim() != 4 || kc.sizes() != vc.sizes())
+      refuse(n + ": codes must be two uint8 [pages, kv heads, page, bytes] tensors of one shape");
+    if (kp.dim() != 4 || kp.sizes().slice(0, 3) != kc.sizes().slice(0, 3) || kp.size(3) != 2 ||
+        kp.sizes() != vp.sizes() || kp.scalar_type() != vp.scalar_type())
+      refuse(n + ": pairs must be two [pages, kv heads, page, 2] tensors of one type");
+    if (!kc.is_contiguous() || !vc.is_contiguous() || !kp.is_contiguous() || !vp.is_contiguous())
+      refuse(n + ": the cache's tensors must be contiguous");
+    dtype = dtype_code(kp.scalar_type());
+    pages = kc.size(0);
+    hkv = kc.size(1);
+    page = kc.size(2);
+    const int64_t row = kc.size(3);
+    if (row * 2 != d && row != d)
+      refuse(n + ": rows of " + std::to_string(row) + " bytes hold neither 4- nor 8-bit codes of head dim " +
+             std::to_string(d));
+    bits = row == d ? 8 : 4;
+  }
+};
+
+void kv_cache_write(const Tensor& k0, const Tensor& v0, const Tensor& kc, const Tensor& vc, const Tensor& kp,
+                    const Tensor& vp, const Tensor& slots0, int64_t status) {
+  same_device(k0, v0, kc, vc, kp, vp, slots0);
+  if (k0.dim() != 3 || k0.sizes() != v0.sizes() || k0.scalar_type() != v0.scalar_type())
+    refuse("kv_cache_write: k and v must be two [tokens, kv heads, d] tensors of one type");
+  const int64_t t = k0.size(0), hkv = k0.size(1), d = k0.size(2);
+  const Cache c("kv_cache_write", kc, vc, kp, vp, d);
+  if (kp.scalar_type() != k0.scalar_type())
+    refuse(std::string("kv_cache_write: the cache holds ") + c10::toString(kp.scalar_type()) + ", got " +
+           c10::toString(k0.scalar_type()));
+  if (c.hkv != hkv)
+    refuse("kv_cache_write: the cache has " + std::to_string(c.hkv) + " kv heads, got " + std::to_string(hkv));
+  if (slots0.scalar_type() != at::kLong || slots0.dim() != 1 || slots0.size(0) != t)
+    refuse("kv_cache_write: slots must be int64 [" + std::to_string(t) + "]");
+  const OnDevice on(k0);
+  const Tensor k = fixed(k0), v = fixed(v0), slots = slots0.contiguous();
+  check(gko_kv_cache_write(c.dtype, c.bits, t, hkv, d, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                           v.stride(0), v.stride(1), slots.data_ptr<int64_t>(), kc.data_ptr(), vc.data_ptr(),
+                           kp.data_ptr(), vp.data_ptr(), c.pages, c.page, status_word(status), on.stream),
+        "gko_kv_cache_write");
+}
+
+Tensor checked_table(const char* name, const Tensor& table, int64_t b) {
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != b)
+    refuse(std::string(name) + ": block_table must be int32 [" + std::to_string(b) + ", columns]");
+  return table.size(1) == 0 || table.stride(1) == 1 ? table : table.contiguous();
+}
+
+std::tuple<Tensor, Tensor> kv_cache_read(const Tensor& kc, const Tensor& vc, const Tensor& kp, const Tensor& vp,
+                                         const Tensor& table0, const Tensor& cu0, int64_t tokens, int64_t head_dim,
+                                         const OptTensor& k_out, const OptTensor& v_out, int64_t status) {
+  same_device(kc, vc, kp, vp, table0, cu0);
+  const Cache c("kv_cache_read", kc, vc, kp, vp, head_dim);
+  if (cu0.scalar_type() != at::kInt || cu0.dim() != 1 || cu0.size(0) < 1)
+    refuse("kv_cache_read: cu_seqlens must be int32 [b + 1]");
+  if (tokens < 0) refuse("kv_cache_read: a negative number of tokens");
+  const int64_t b = cu0.size(0) - 1;
+  const OnDevice on(kc);
+  const Tensor table = checked_table("kv_cache_read", table0, b), cu = cu0.contiguous();
+  const int64_t shape[3] = {tokens, c.hkv, c.d};
+  const Tensor k = k_out ? *k_out : at::empty(shape, kp.options()), v = v_out ? *v_out : at::empty(shape, kp.options());
+  for (const Tensor* t : {&k, &v}) {
+    same_device(kc, *t);
+    if (t->sizes() != at::IntArrayRef(shape, 3) || t->scalar_type() != kp.scalar_type() || !t->is_contiguous())
+      refuse("kv_cache_read: out must be two contiguous [" + std::to_string(tokens) + ", " + std::to_string(c.hkv) +
+             ", " + std::to_string(c.d) + "] tensors of the cache's element type");
+  }
+  check(gko_kv_cache_read(c.dtype, c.bits, b, c.hkv, c.d, tokens, kc.data_ptr(), vc.data_ptr(), kp.data_ptr(),
+                          vp.data_ptr(), c.pages, c.page, table.data_ptr<int>(), table.stride(0), table.size(1),
+                          cu.data_ptr<int>(), k.data_ptr(), v.data_ptr(), status_word(status), on.stream),
+        "gko_kv_cache_read");
+  return {k, v};
+}
+
+std::tuple<Tensor, Tensor> fmha_cache_fwd(const Tensor& q0, const Tensor& kc, const Tensor& vc, const Tensor& kp,
+                                          const Tensor& vp, const Tensor& table0, const Tensor& lens0,
+                                          const OptTensor& cu_q, int64_t max_q, const std::optional<int64_t>& max_k0,
+                                          const std::optional<double>& scale, int64_t causal, int64_t window,
+                                          double softcap, int64_t sinks, const OptTensor& out0, int64_t status) {
+  same_device(q0, kc, vc, kp, vp, table0, lens0);
+  if (q0.dim() != 3) refuse("fmha_cache: q must be 3-D [tokens, heads, d]");
+  const int64_t tq = q0.size(0), hq = q0.size(1), d = q0.size(2);
+  const Cache c("fmha_cache", kc, vc, kp, vp, d);
+  if (kp.scalar_type() != q0.scalar_type())
+    refuse(std::string("fmha_cache: the cache holds ") + c10::toString(kp.scalar_type()) + ", got " +
+           c10::toString(q0.scalar_type()));
+  if (lens0.scalar_type() != at::kInt || lens0.dim() != 1) refuse("fmha_cache: seq_lens must be int32 [b]");
+  const int64_t b = lens0.size(0);
+  Tensor cu;
+  if (!cu_q) {
+    if (tq != b || max_q != 1)
+      refuse("fmha_cache: without cu_seqlens_q there is one query row per sequence, got " + std::to_string(tq) +
+             " rows for " + std::to_string(b) + " sequences, max_seqlen_q " + std::to_string(max_q));
+  } else {
+    same_device(q0, *cu_q);
+    if (cu_q->scalar_type() != at::kInt || cu_q->dim() != 1 || cu_q->size(0) != b + 1)
+      refuse("fmha_cache: cu_seqlens_q must be int32 [" + std::to_string(b + 1) + "]");
+    cu = cu_q->contiguous();
+  }
+  const OnDevice on(q0);
+  const Tensor table = checked_table("fmha_cache", table0, b), lens = lens0.contiguous(), q = fixed(q0);
+  const int64_t max_k = max_k0 ? *max_k0 : table.size(1) * c.page;
+  const int64_t shape[3] = {tq, hq, d}, lse_shape[2] = {hq, tq};
+  if (out0) {
+    same_device(q0, *out0);
+    if (out0->sizes() != at::IntArrayRef(shape, 3) || out0->scalar_type() != q.scalar_type() || !out0->is_contiguous())
+      refuse("fmha_cache: out must be a contiguous [" + std::to_string(tq) + ", " + std::to_string(hq) + ", " +
+             std::to_string(d) + "] tensor of q's type");
+  }
+  if (window < 0 || sinks < 0 || window > INT32_MAX || sinks > INT32_MAX)
+    refuse("fmha_cache: negative or huge window or sinks");
+  const int64_t bytes =
+      gko_fmha_cache_workspace_size(c.bits, b, hq, c.hkv, d, tq, max_q, max_k, (int)window, (int)sinks);
+  if (bytes < 0) check(GKO_ERR_UNSUPPORTED, "gko_fmha_cache_workspace_size");
+  const Tensor out = out0 ? *out0 : at::empty(shape, q.options());
+  const Tensor lse = at::empty(lse_shape, q.options().dtype(at::kFloat));
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, kc.options());
+  check(gko_fmha_cache_fwd(c.dtype, c.bits, b, hq, c.hkv, d, tq, max_q, max_k, q.data_ptr(), q.stride(0), q.stride(1),
+                           kc.data_ptr(), vc.data_ptr(), kp.data_ptr(), vp.data_ptr(), c.pages, c.page,
+                           table.data_ptr<int>(), table.stride(0), table.size(1), lens.data_ptr<int>(),
+                           cu.defined() ? cu.data_ptr<int>() : nullptr,
+                           (float)(scale ? *scale : 1.0 / std::sqrt((double)d)), causal != 0, (int)window,
+                           (float)softcap, (int)sinks, out.data_ptr(), lse.data_ptr<float>(),
+                           bytes > 0 ? ws.data_ptr() : nullptr, bytes, status_word(status), on.stream),
+        "gko_fmha_cache_fwd");
+  return {out, lse};
+}
+
+// ---------------------------------------------------------------- windowed attention with sinks, dense, no bias
+struct Mask {
+  double scale, softcap;
+  int64_t causal, window, sinks;
+};
+
+void check_mask(const Mask& m) {
+  if (m.window < 0 || m.sinks < 0 || m.window > INT32_MAX || m.sinks > INT32_MAX)
+    refuse("fmha: window and sinks must be >= 0");
+}
+
+std::tuple<Tensor, Tensor> sinks_fwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Mask& m,
+                                     int64_t status) {
+  same_device(q0, k0, v0);
+  if (q0.dim() != 4 || k0.dim() != 4 || v0.dim() != 4) refuse("fmha: q, k, v must be 4-D [z, h, s, d]");
+  if (q0.scalar_type() != k0.scalar_type() || q0.scalar_type() != v0.scalar_type())
+    refuse("fmha: q, k, v dtypes differ");
+  const int64_t z = q0.size(0), hq = q0.size(1), sq = q0.size(2), d = q0.size(3);
+  if (k0.sizes() != v0.sizes() || k0.size(3) != d || k0.size(0) != z) refuse("fmha: shape mismatch of q, k, v");
+  check_mask(m);
+  const int dt = dtype_code(q0.scalar_type());
+  const OnDevice on(q0);
+  const Tensor q = fixed(q0), k = fixed(k0), v = fixed(v0);
+  const int64_t shape[4] = {z, hq, sq, d}, lse_shape[2] = {z * hq, sq};
+  const Tensor out = at::empty(shape, q.options());
+  const Tensor lse = at::empty(lse_shape, q.options().dtype(at::kFloat));
+  check(gko_fmha_sinks_fwd(dt, z, hq, k.size(1), sq, k.size(2), d, q.data_ptr(), q.strides().data(), k.data_ptr(),
+                           k.strides().data(), v.data_ptr(), v.strides().data(), nullptr, GKO_BIAS_NONE, 0, nullptr, 1,
+                           nullptr, (float)m.scale, m.causal != 0, (int)m.window, (float)m.softcap, (int)m.sinks,
+                           out.data_ptr(), lse.data_ptr<float>(), status_word(status), on.stream),
+        "gko_fmha_fwd");
+  return {out, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> sinks_bwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& out0,
+                                             const Tensor& lse0, const Tensor& dout0, const Mask& m, int64_t status) {
+  same_device(q0, k0, v0, out0, lse0, dout0);
+  if (dout0.scalar_type() != q0.scalar_type() || dout0.sizes() != q0.sizes())
+    refuse("fmha_bwd: out and dout must have q's shape and type");
+  const int64_t z = q0.size(0), hq = q0.size(1), sq = q0.size(2), d = q0.size(3), hkv = k0.size(1), sk = k0.size(2);
+  const int dt = dtype_code(q0.scalar_type());
+  const OnDevice on(q0);
+  const Tensor q = fixed(q0), k = fixed(k0), v = fixed(v0), out = fixed(out0), dout = fixed(dout0),
+               lse = lse0.contiguous();
+  const int64_t q_shape[4] = {z, hq, sq, d}, k_shape[4] = {z, hkv, sk, d};
+  const Tensor dq = at::empty(q_shape, q.options()), dk = at::empty(k_shape, k.options()),
+               dv = at::empty(k_shape, v.options());
+  const int64_t bytes = gko_fmha_sinks_bwd_workspace_size(z, hq, hkv, sq, sq, sk, d, m.causal != 0, (int)m.window,
+                                                          (int)m.sinks, 0);
+  if (bytes < 0) check(GKO_ERR_UNSUPPORTED, "gko_fmha_bwd_workspace_size");
+  const Tensor ws = at::empty({bytes > 16 ? bytes : 16}, q.options().dtype(at::kByte));
+  check(gko_fmha_sinks_bwd(dt, z, hq, hkv, sq, sk, d, q.data_ptr(), q.strides().data(), k.data_ptr(),
+                           k.strides().data(), v.data_ptr(), v.strides().data(), nullptr, GKO_BIAS_NONE, 0, nullptr, 1,
+                           out.data_ptr(), out.strides().data(), dout.data_ptr(), dout.strides().data(),
+                           lse.data_ptr<float>(), (float)m.scale, m.causal != 0, (int)m.window, (float)m.softcap,
+                           (int)m.sinks, dq.data_ptr(), dq.strides().data(), dk.data_ptr(), dk.strides().data(),
+                           dv.data_ptr(), dv.strides().data(), ws.data_ptr(), bytes, status_word(status), on.stream),
+        "gko_fmha_bwd");
+  return {dq, dk, dv};
+}
+
+struct SinksAttention : torch::autograd::Function<SinksAttention> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                        double scale, int64_t causal, int64_t window, double softcap, int64_t sinks, int64_t status) {
+    auto [out, lse] = sinks_fwd(q, k, v, Mask{scale, softcap, causal, window, sinks}, status);
+    ctx->save_for_backward({q, k, v, out, lse});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["softcap"] = softcap;
+    ctx->saved_data["mask"] = std::vector<int64_t>{causal, window, sinks, status};
+    return out;
+  }
+  static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx,
+                                               torch::autograd::tensor_list grads) {
+    if (at::GradMode::is_enabled()) refuse("attention with sinks has no second derivative (create_graph=True)");
+    const auto s = ctx->get_saved_variables();
+    const auto mask = ctx->saved_data["mask"].toIntVector();
+    const Mask m{ctx->saved_data["scale"].toDouble(), ctx->saved_data["softcap"].toDouble(), mask[0], mask[1], mask[2]};
+    auto [dq, dk, dv] = sinks_bwd(s[0], s[1], s[2], s[3], s[4], grads[0], m, mask[3]);
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor sinks_attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, int64_t causal, int64_t window,
+                       double softcap, int64_t sinks, int64_t status) {
+  return SinksAttention::apply(q, k, v, scale, causal, window, softcap, sinks, status);
+}
+
+std::tuple<Tensor, Tensor> sinks_forward(const Tensor& q, const Tensor& k, const Tensor& v, double scale,
+                                         int64_t causal, int64_t window, double softcap, int64_t sinks,
+                                         int64_t status) {
+  return sinks_fwd(q, k, v, Mask{scale, softcap, causal, window, sinks}, status);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_gko_torch, m) {
+  m.def("kv_cache_write", &kv_cache_write);
+  m.def("kv_cache_read", &kv_cache_read);
+  m.def("fmha_cache_fwd", &fmha_cache_fwd);
+  m.def("sinks_forward", &sinks_forward);
+  m.def("sinks_attention", &sinks_attention);
+}

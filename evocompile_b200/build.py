@@ -1,7 +1,8 @@
 """Build libgko_b200.so (all CUDA kernels + the C ABI) in-tree with nvcc for sm_100a.
 
 Usage: python -m evocompile_b200.build [--force]
-The library lands next to this file so that it travels with the source tree.
+The library lands next to this file so that it travels with the source tree, and so does _gko_torch.so, the
+compiled tensor-level host code of binding/ (g++ against torch's headers, linked to the library).
 """
 
 from __future__ import annotations
@@ -10,12 +11,15 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 REPO = PKG.parent
 LIB = PKG / "libgko_b200.so"
+BINDING_SRC = PKG / "binding" / "gko_torch.cpp"
+BINDING = PKG / "_gko_torch.so"
 BUILD_DIR = REPO / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -47,6 +51,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     stamp = PKG / ".libgko_b200.stamp"
     digest = _digest()
     if LIB.exists() and stamp.exists() and stamp.read_text().strip() == digest and not force:
+        build_binding()
         return LIB
     BUILD_DIR.mkdir(exist_ok=True)
     objs = []
@@ -79,7 +84,37 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
     os.replace(tmp, LIB)
     stamp.write_text(digest)
+    build_binding(force, verbose)
     return LIB
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile binding/gko_torch.cpp into _gko_torch.so, against this interpreter's torch. Returns its path."""
+    import torch
+
+    stamp = PKG / "._gko_torch.stamp"
+    h = hashlib.sha256(BINDING_SRC.read_bytes() + (REPO / "include" / "gko_b200.h").read_bytes())
+    h.update(f"{torch.__version__} {sys.version}".encode())
+    digest = h.hexdigest()[:16]
+    if BINDING.exists() and stamp.exists() and stamp.read_text().strip() == digest and not force:
+        return BINDING
+    home = Path(torch.__file__).resolve().parent
+    cuda = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_gko_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(home / "include"), "-I", str(home / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", str(cuda / "include"), "-I", sysconfig.get_paths()["include"], str(BINDING_SRC), "-o", str(tmp),
+           "-L", str(home / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python",
+           "-L", str(PKG), "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + r.stdout + r.stderr)
+    os.replace(tmp, BINDING)
+    stamp.write_text(digest)
+    return BINDING
 
 
 if __name__ == "__main__":

@@ -33,10 +33,21 @@ from typing import Tuple
 
 import torch
 
-from .. import ops
+from .. import _lib, ops
 
 _OP_READY = False
 _AUTOGRADED = False
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _untraced(*tensors):
+    """Whether nothing looks on (Dynamo, a dispatch mode, tensor subclasses): then the compiled autograd node of
+    ``gko::fmha_sinks_pair`` may run in the custom op's place, whose dispatch costs more host time (about 0.1 ms
+    each way) than a short sequence's kernels."""
+    return (not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
+            and all(type(t) in _PLAIN for t in tensors))
 
 
 # --------------------------------------------------------------------------- python entry points
@@ -50,13 +61,14 @@ def fused_attention(q, k, v, attn_bias, scale, causal=0, window=0, softcap=0.0, 
     squeeze = q.dim() == 3
     if squeeze:
         q, k, v = q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1)
+    if sinks and window and (attn_bias is None or attn_bias.numel() == 0) and _untraced(q, k, v):
+        out = _lib.binding().sinks_attention(q, k, v, float(scale), int(causal), int(window), float(softcap or 0.0),
+                                             int(sinks), _lib.status_address(q))
+        return out.squeeze(1) if squeeze else out
     if attn_bias is None:
         attn_bias = q.new_empty((0,))
     _ensure_op()
-    if sinks and window and not torch.compiler.is_compiling():
-        out = _SinksAttention.apply(q, k, v, attn_bias, float(scale), int(causal), int(window), float(softcap or 0.0),
-                                    int(sinks))
-    elif sinks and window:
+    if sinks and window:
         out, _ = torch.ops.gko.fmha_sinks_pair(q, k, v, attn_bias, float(scale), int(causal), int(window),
                                                float(softcap or 0.0), int(sinks))
     else:
@@ -89,24 +101,6 @@ def _bwd_sinks(ctx, dout, dlse):
     dq, dk, dv = torch.ops.gko.fmha_sinks_bwd(q, k, v, attn_bias, out, lse, dout, ctx.scale, ctx.causal, ctx.window,
                                               ctx.softcap, ctx.sinks)
     return dq, dk, dv, None, None, None, None, None, None
-
-
-class _SinksAttention(torch.autograd.Function):
-    """``gko::fmha_sinks_pair`` and its gradient outside Dynamo: the same calls without the custom op's
-    dispatch, which costs more host time (about 0.1 ms each way) than a short sequence's kernels."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, attn_bias, scale, causal, window, softcap, sinks):
-        out, lse = ops.fmha_fwd(q, k, v, attn_bias, scale, causal, window, softcap, sinks=sinks)
-        ctx.save_for_backward(q, k, v, attn_bias, out, lse)
-        ctx.args = scale, causal, window, softcap, sinks
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        dq, dk, dv = ops.fmha_bwd(*ctx.saved_tensors, dout, *ctx.args)
-        return dq, dk, dv, None, None, None, None, None, None
 
 
 def _setup_sinks_varlen(ctx, inputs, output):

@@ -386,6 +386,9 @@ def fmha_fwd(q, k, v, attn_bias=None, scale=None, causal=0, window=0, softcap=0.
     (eval/kernels/fused_sdpa.py:912-943). With a window, the first ``sinks`` keys stay visible to
     every query (that the causal mask lets see them).
     """
+    if sinks and window and attn_bias is None and out is None:
+        return _lib.binding().sinks_forward(q, k, v, q.shape[-1] ** -0.5 if scale is None else scale, int(causal),
+                                            int(window), softcap or 0.0, int(sinks), _lib.status_address(q))
     dev = _lib.require_cuda(q, k, v, attn_bias)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise RuntimeError("fmha: q, k, v must be 4-D [z, h, s, d]")
@@ -596,31 +599,6 @@ def kv_cache_alloc(pages, page_size, kv_heads, head_dim, bits=4, dtype=torch.bfl
     return KVCache(codes(), codes(), pairs(), pairs())
 
 
-def _cache_layout(name, cache, hkv=None, dtype=None):
-    """Type code of a cache whose four tensors fit together and, where given, its kv heads and element type."""
-    kc, vc, kp, vp = cache
-    codes, pairs = kc.shape, kp.shape
-    if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or len(codes) != 4 or vc.shape != codes:
-        raise RuntimeError(f"{name}: codes must be two uint8 [pages, kv heads, page, bytes] tensors of one shape")
-    if pairs[:3] != codes[:3] or pairs[3:] != (2,) or vp.shape != pairs or kp.dtype != vp.dtype:
-        raise RuntimeError(f"{name}: pairs must be two [pages, kv heads, page, 2] tensors of one type")
-    if not (kc.is_contiguous() and vc.is_contiguous() and kp.is_contiguous() and vp.is_contiguous()):
-        raise RuntimeError(f"{name}: the cache's tensors must be contiguous")
-    if dtype is not None and kp.dtype != dtype:
-        raise RuntimeError(f"{name}: the cache holds {kp.dtype}, got {dtype}")
-    if hkv is not None and codes[1] != hkv:
-        raise RuntimeError(f"{name}: the cache has {codes[1]} kv heads, got {hkv}")
-    return _lib.dtype_code(kp.dtype)
-
-
-def _cache_bits(name, row_bytes, d):
-    if row_bytes * 2 == d:
-        return 4
-    if row_bytes == d:
-        return 8
-    raise RuntimeError(f"{name}: rows of {row_bytes} bytes hold neither 4- nor 8-bit codes of head dim {d}")
-
-
 def kv_cache_write(k, v, cache, slots):
     """Quantise new keys and values into their slots of a paged cache, in place.
 
@@ -630,29 +608,7 @@ def kv_cache_write(k, v, cache, slots):
     (``_lib.read_status``). The slots of one call must be distinct.
     """
     kc, vc, kp, vp = cache
-    dev = _lib.require_cuda(k, v, kc, vc, kp, vp, slots)
-    if k.dim() != 3 or k.shape != v.shape or k.dtype != v.dtype:
-        raise RuntimeError("kv_cache_write: k and v must be two [tokens, kv heads, d] tensors of one type")
-    t, hkv, d = k.shape
-    dt = _cache_layout("kv_cache_write", cache, hkv, k.dtype)
-    bits = _cache_bits("kv_cache_write", kc.shape[3], d)
-    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != t:
-        raise RuntimeError(f"kv_cache_write: slots must be int64 [{t}], got {slots.dtype} {tuple(slots.shape)}")
-    k, v = _bwd_fix(k), _bwd_fix(v)
-    slots = slots.contiguous()
-    with _lib.on_device(dev):
-        rc = _lib.load().gko_kv_cache_write(
-            dt, bits, t, hkv, d, _ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(slots),
-            _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), kc.shape[0], kc.shape[2], _status_ptr(dev), _stream(dev),
-        )
-    _lib.check(rc, "gko_kv_cache_write")
-
-
-def _check_table(name, block_table, b, what):
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b:
-        raise RuntimeError(f"{name}: block_table must be int32 [{b}, columns] for {what}, got "
-                           f"{block_table.dtype} {tuple(block_table.shape)}")
-    return block_table if block_table.stride(1) == 1 or block_table.shape[1] == 0 else block_table.contiguous()
+    _lib.binding().kv_cache_write(k, v, kc, vc, kp, vp, slots, _lib.status_address(k))
 
 
 def kv_cache_read(cache, block_table, cu_seqlens, tokens, head_dim, out=None):
@@ -665,29 +621,9 @@ def kv_cache_read(cache, block_table, cu_seqlens, tokens, head_dim, out=None):
     what it had there).
     """
     kc, vc, kp, vp = cache
-    dev = _lib.require_cuda(kc, vc, kp, vp, block_table, cu_seqlens, *(out or ()))
-    dt = _cache_layout("kv_cache_read", cache)
-    pages, hkv, page_size, row = kc.shape
-    d = int(head_dim)
-    bits = _cache_bits("kv_cache_read", row, d)
-    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
-        raise RuntimeError("kv_cache_read: cu_seqlens must be int32 [b + 1]")
-    b = cu_seqlens.shape[0] - 1
-    block_table = _check_table("kv_cache_read", block_table, b, f"cu_seqlens of {b} sequences")
-    if out is None:
-        out = kp.new_empty((tokens, hkv, d)), kp.new_empty((tokens, hkv, d))
-    for t in out:
-        if t.shape != (tokens, hkv, d) or t.dtype != kp.dtype or not t.is_contiguous():
-            raise RuntimeError(f"kv_cache_read: out must be two contiguous [{tokens}, {hkv}, {d}] {kp.dtype} tensors")
-    cu_seqlens = cu_seqlens.contiguous()
-    with _lib.on_device(dev):
-        rc = _lib.load().gko_kv_cache_read(
-            dt, bits, b, hkv, d, tokens, _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), pages, page_size, _ptr(block_table),
-            block_table.stride(0), block_table.shape[1], _ptr(cu_seqlens), _ptr(out[0]), _ptr(out[1]),
-            _status_ptr(dev), _stream(dev),
-        )
-    _lib.check(rc, "gko_kv_cache_read")
-    return tuple(out)
+    k_out, v_out = out if out is not None else (None, None)
+    return _lib.binding().kv_cache_read(kc, vc, kp, vp, block_table, cu_seqlens, tokens, head_dim, k_out, v_out,
+                                        _lib.status_address(kc))
 
 
 def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqlen_q=1, max_seqlen_k=None, scale=None,
@@ -704,50 +640,9 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
     what it had). One call per cache step: repeated calls give the same bits.
     """
     kc, vc, kp, vp = cache
-    dev = _lib.require_cuda(q, kc, vc, kp, vp, block_table, seq_lens, cu_seqlens_q, out)
-    if q.dim() != 3:
-        raise RuntimeError("fmha_cache: q must be 3-D [tokens, heads, d]")
-    tq, hq, d = q.shape
-    dt = _cache_layout("fmha_cache", cache, None, q.dtype)
-    pages, hkv, page_size, row = kc.shape
-    bits = _cache_bits("fmha_cache", row, d)
-    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1:
-        raise RuntimeError("fmha_cache: seq_lens must be int32 [b]")
-    b = seq_lens.shape[0]
-    block_table = _check_table("fmha_cache", block_table, b, f"seq_lens of {b} sequences")
-    if cu_seqlens_q is None:
-        if tq != b or max_seqlen_q != 1:
-            raise RuntimeError(f"fmha_cache: without cu_seqlens_q there is one query row per sequence, got {tq} rows "
-                               f"for {b} sequences, max_seqlen_q {max_seqlen_q}")
-    else:
-        if cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] != b + 1:
-            raise RuntimeError(f"fmha_cache: cu_seqlens_q must be int32 [{b + 1}]")
-        cu_seqlens_q = cu_seqlens_q.contiguous()
-    if scale is None:
-        scale = d ** -0.5
-    if max_seqlen_k is None:
-        max_seqlen_k = block_table.shape[1] * page_size
-    q = _bwd_fix(q)
-    if out is None:
-        out = q.new_empty((tq, hq, d))
-    elif out.shape != (tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
-        raise RuntimeError(f"fmha_cache: out must be a contiguous [{tq}, {hq}, {d}] {q.dtype} tensor")
-    lse = q.new_empty((hq, tq), dtype=torch.float32)
-    seq_lens = seq_lens.contiguous()
-    lib = _lib.load()
-    with _lib.on_device(dev):
-        ws_bytes = _workspace_bytes("gko_fmha_cache_workspace_size", dev.index, bits, b, hq, hkv, d, tq,
-                                    int(max_seqlen_q), int(max_seqlen_k), int(window or 0), int(sinks or 0))
-        ws = kc.new_empty(ws_bytes) if ws_bytes else None
-        rc = lib.gko_fmha_cache_fwd(
-            dt, bits, b, hq, hkv, d, tq, int(max_seqlen_q), int(max_seqlen_k), _ptr(q), q.stride(0), q.stride(1),
-            _ptr(kc), _ptr(vc), _ptr(kp), _ptr(vp), pages, page_size, _ptr(block_table), block_table.stride(0),
-            block_table.shape[1], _ptr(seq_lens), _ptr(cu_seqlens_q), float(scale), int(bool(causal)),
-            int(window or 0), float(softcap or 0.0), int(sinks or 0), _ptr(out), _ptr(lse), _ptr(ws), ws_bytes,
-            _status_ptr(dev), _stream(dev),
-        )
-    _lib.check(rc, "gko_fmha_cache_fwd")
-    return out, lse
+    return _lib.binding().fmha_cache_fwd(q, kc, vc, kp, vp, block_table, seq_lens, cu_seqlens_q, max_seqlen_q,
+                                         max_seqlen_k, scale, int(causal), window or 0, softcap or 0.0, sinks or 0, out,
+                                         _lib.status_address(q))
 
 
 # --------------------------------------------------------------------------- tensor-parallel GEMM + all-reduce
