@@ -239,6 +239,36 @@ std::tuple<Tensor, Tensor> sinks_fwd(const Tensor& q0, const Tensor& k0, const T
   return {out, lse};
 }
 
+std::tuple<Tensor, Tensor> sinks_varlen_forward(const Tensor& q0, const Tensor& k0, const Tensor& v0,
+                                                const Tensor& cu_q0, const Tensor& cu_k0, int64_t max_q, double scale,
+                                                int64_t causal, int64_t window, double softcap, int64_t sinks,
+                                                int64_t status) {
+  same_device(q0, k0, v0, cu_q0, cu_k0);
+  if (q0.dim() != 3 || k0.dim() != 3 || v0.dim() != 3) refuse("fmha_varlen: q, k, v must be 3-D [tokens, heads, d]");
+  if (q0.scalar_type() != k0.scalar_type() || q0.scalar_type() != v0.scalar_type())
+    refuse("fmha_varlen: q, k, v dtypes differ");
+  if (cu_q0.scalar_type() != at::kInt || cu_k0.scalar_type() != at::kInt)
+    refuse("fmha_varlen: cu_seqlens must be int32");
+  if (cu_q0.numel() != cu_k0.numel() || cu_q0.numel() < 1)
+    refuse("fmha_varlen: cu_seqlens_q and cu_seqlens_k must both have b + 1 entries");
+  const int64_t tq = q0.size(0), hq = q0.size(1), d = q0.size(2);
+  if (k0.sizes() != v0.sizes() || k0.size(2) != d) refuse("fmha_varlen: shape mismatch of q, k, v");
+  check_mask(Mask{scale, softcap, causal, window, sinks});
+  const int dt = dtype_code(q0.scalar_type());
+  const OnDevice on(q0);
+  const Tensor q = fixed(q0), k = fixed(k0), v = fixed(v0), cu_q = cu_q0.contiguous(), cu_k = cu_k0.contiguous();
+  const int64_t shape[3] = {tq, hq, d}, lse_shape[2] = {hq, tq};
+  const Tensor out = at::empty(shape, q.options());
+  const Tensor lse = at::empty(lse_shape, q.options().dtype(at::kFloat));
+  check(gko_fmha_sinks_varlen_fwd(dt, cu_q.numel() - 1, hq, k.size(1), d, tq, k.size(0), max_q, q.data_ptr(),
+                                  q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                                  v.stride(0), v.stride(1), cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), (float)scale,
+                                  causal != 0, (int)window, (float)softcap, (int)sinks, out.data_ptr(),
+                                  lse.data_ptr<float>(), status_word(status), on.stream),
+        "gko_fmha_varlen_fwd");
+  return {out, lse};
+}
+
 std::tuple<Tensor, Tensor, Tensor> sinks_bwd(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& out0,
                                              const Tensor& lse0, const Tensor& dout0, const Mask& m, int64_t status) {
   same_device(q0, k0, v0, out0, lse0, dout0);
@@ -305,5 +335,6 @@ PYBIND11_MODULE(_gko_torch, m) {
   m.def("kv_cache_read", &kv_cache_read);
   m.def("fmha_cache_fwd", &fmha_cache_fwd);
   m.def("sinks_forward", &sinks_forward);
+  m.def("sinks_varlen_forward", &sinks_varlen_forward);
   m.def("sinks_attention", &sinks_attention);
 }

@@ -435,6 +435,10 @@ def fmha_varlen_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqle
     token count (not checked on the host, which would need a device sync; the kernel writes no row outside
     [0, tq)), and max_seqlen_q at least the longest query sequence.
     """
+    if sinks and window:
+        return _lib.binding().sinks_varlen_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
+                                                   q.shape[-1] ** -0.5 if scale is None else scale, int(causal),
+                                                   int(window), softcap or 0.0, int(sinks), _lib.status_address(q))
     dev = _lib.require_cuda(q, k, v, cu_seqlens_q, cu_seqlens_k)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise RuntimeError("fmha_varlen: q, k, v must be 3-D [tokens, heads, d]")

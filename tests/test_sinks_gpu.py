@@ -266,6 +266,22 @@ def test_new_host_thread():
     _status_clear()
 
 
+def test_traced_and_subclassed():
+    """Under a dispatch mode the custom op runs, so a trace has it; a second derivative is refused."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    q, k, v, _ = (_dev(t) for t in _qkv(3, 1, 2, 2, 40, 40, 64, torch.bfloat16))
+    call = lambda a, b, c: fused_sdpa.fused_attention(a, b, c, None, 0.125, 1, 8, sinks=2)  # noqa: E731
+    graph = make_fx(call)(q, k, v)
+    assert any("fmha_sinks_pair" in str(n.target) for n in graph.graph.nodes)
+    assert torch.equal(graph(q, k, v), call(q, k, v))
+    leaf = q.detach().requires_grad_(True)
+    out = call(leaf, k, v)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.sum(), leaf, create_graph=True)
+    _status_clear()
+
+
 def test_refusals():
     q = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError, match="sinks"):
@@ -275,3 +291,15 @@ def test_refusals():
         ops.fmha_bwd(q, q, q, None, out, lse, q, 0.1, 1, 4, 0.0, -1)
     with pytest.raises(RuntimeError, match="window"):
         ops.fmha_fwd(q, q, q, None, 0.1, 1, -4, sinks=1)
+    for bad in ((q[0], q, q), (q, q.half(), q), (q, q[:, :, :3], q), (q, q[..., :32], q[..., :32]), (q.float(),) * 3,
+                (q.cpu(), q, q)):
+        with pytest.raises(RuntimeError):
+            ops.fmha_fwd(*bad, None, 0.1, 1, 4, sinks=1)
+        with pytest.raises(RuntimeError):
+            fused_sdpa.fused_attention(*bad, None, 0.1, 1, 4, sinks=1)
+    p = q[0].transpose(0, 1)
+    cu = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    for bad in ((q, q, q, cu, cu), (p, p, p, cu.long(), cu), (p, p, p[:4], cu, cu), (p, p, p, cu, cu[:1]),
+                (p, p.half(), p, cu, cu)):
+        with pytest.raises(RuntimeError, match="fmha_varlen"):
+            ops.fmha_varlen_fwd(*bad, 8, 8, 0.1, 1, 4, sinks=1)
