@@ -32,27 +32,42 @@ namespace gko {
 namespace fmha {
 
 constexpr int kBM = 128;           // rows of one query tile
-constexpr int kQTiles = 2;         // query tiles per CTA
-constexpr int kBlockM = kBM * kQTiles;
 constexpr int kBN = 128;           // keys per tile
-constexpr int kThreads = 384;      // 2 x 4 softmax warps, producer, MMA, 2 idle
-constexpr int kProducerWarp = 8;
-constexpr int kMmaWarp = 9;
-constexpr uint32_t kRegsSoftmax = 216;
-constexpr uint32_t kRegsControl = 72;
-static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsControl <= 384 * 168, "register split exceeds the launch");
-constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRescaleThreshold = 8.f;  // log2 units
 constexpr int kFewSinks = 32;             // sinks of a tile that takes part with 32 keys only
 constexpr int kMaxWindow = (1 << 30) - 1024;  // wider ones hide nothing; position + window stays an int
-// K tiles are double or triple buffered (V always double): the S MMA of the next key tile
-// waits on K, so a deeper K ring hides more TMA latency when shared memory allows it.
-#ifndef GKO_FMHA_K_STAGES
-#define GKO_FMHA_K_STAGES 2
-#endif
-constexpr int kKStages = GKO_FMHA_K_STAGES;
+// What the softmax of a kernel handles: kPlain an optional causal mask; kExtra also bias, softcap and
+// windows, element by element; kWindow a window with sinks and a positive scale, the scale folded into
+// the exponent as in kPlain and masks only on the key tiles that cross the edge of what a warp's rows
+// see. Up to 32 sinks, ahead of the window, cost a quarter of a key tile: S has 32 columns, P V two steps.
+// Bound by the chain S -> softmax -> P -> P V of each key tile, as kPlain is (its rate on dense causal
+// attention, 0.9 PFLOP/s, is what the tiles here run at too); the window leaves 9 to 10 tiles per block.
+// 4096 tokens, 64 / 8 heads of 128, window 1024, 4 sinks: 175 us, 0.69 PFLOP/s of visible pairs (196 us with a
+// whole tile for the sinks, one mask for every edge and two query tiles per CTA); kExtra takes some ten times as
+// long.
+enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
+
+// A CTA takes two query tiles, whose softmax and products hide one another, and has an SM to itself (K and V
+// in two stages, 512 TMEM columns). In kWindow it takes one, with half of everything, and two CTAs share an
+// SM: they hide one another's softmax as well, and also one another's start and end, which a window's few
+// key tiles do not outweigh (packed prompts of 31 to 2047 tokens, window 512: 93 us with two tiles, 88 with one;
+// 4096 tokens, window 1024: 178 and 175; 513 tokens, window 128, where blocks of 256 rows fill a quarter of the
+// SMs: 11.6 and 8.6).
+template <int MODE>
+struct Shape {
+  static constexpr int kQTiles = MODE == kWindow ? 1 : 2;
+  static constexpr int kCtas = 3 - kQTiles;                 // per SM
+  static constexpr int kBlockM = kBM * kQTiles;
+  static constexpr int kThreads = 128 * (kQTiles + 1);      // softmax warps, producer, MMA, 2 idle
+  static constexpr uint32_t kRegsSoftmax = kQTiles == 2 ? 216 : 200;
+  static constexpr uint32_t kRegsControl = kQTiles == 2 ? 72 : 56;
+  static constexpr uint32_t kRegsLaunch = kQTiles == 2 ? 168 : 128;
+  static_assert(kQTiles * 128 * kRegsSoftmax + 128 * kRegsControl <= kThreads * kRegsLaunch,
+                "register split exceeds the launch");
+  static constexpr uint32_t kTmemCols = 256 * kQTiles;
+};
 // Wait for K(j+1) right before the first S MMA that reads it (1) or before the PV MMAs of
 // tile j (0).
 #ifndef GKO_FMHA_LATE_KWAIT
@@ -63,7 +78,6 @@ struct Params {
   int hq, hkv, group;  // group = hq / hkv
   int sq, sk;          // dense: per-batch lengths; varlen: unused
   int q_tiles;         // query blocks along the query axis (grid.x)
-  int half;            // kWindow: query blocks of 128 rows, the second tile unused (else 256 rows)
   int zh;              // batch (or sequences) x query heads
   float scale, scale_log2, softcap;
   int causal, window, sinks;  // sinks: leading keys that the window does not hide (0 without a window)
@@ -82,17 +96,20 @@ struct Params {
   unsigned* status;
 };
 
-template <int D>
+template <int D, int MODE>
 struct Layout {
+  static constexpr int kQTiles = Shape<MODE>::kQTiles;
+  static constexpr int kStages = kQTiles == 1 && D == 128 ? 1 : 2;  // of K and of V
   static constexpr uint32_t kChunk = 128 * 128;  // one [128 rows x 128 B] swizzle block
   static constexpr int kChunks = D / 64;
   static constexpr uint32_t kTile = kChunks * kChunk;  // 128 x D elements
-  static constexpr uint32_t kQ = 0;                          // Q0, Q1
-  static constexpr uint32_t kK0 = kQ + 2 * kTile;            // K stages
-  static constexpr uint32_t kV0 = kK0 + kKStages * kTile;    // V stages 0, 1
-  static constexpr uint32_t kMeta = kV0 + 2 * kTile;
-  // at least 120 KB so that a single CTA (and its 512 TMEM columns) occupies an SM
-  static constexpr uint32_t kBytes = (1024 + kMeta + 256) > 122880 ? (1024 + kMeta + 256) : 122880;
+  static constexpr uint32_t kQ = 0;                          // Q tiles
+  static constexpr uint32_t kK0 = kQ + kQTiles * kTile;      // K stages
+  static constexpr uint32_t kV0 = kK0 + kStages * kTile;     // V stages
+  static constexpr uint32_t kMeta = kV0 + kStages * kTile;
+  // two query tiles: at least 120 KB, so that a single CTA (and its 512 TMEM columns) occupies an SM
+  static constexpr uint32_t kBytes = kQTiles == 1 || (1024 + kMeta + 256) > 122880 ? (1024 + kMeta + 256) : 122880;
+  static_assert(kQTiles == 2 || 2 * (kBytes + 1024) <= 233472, "two CTAs share an SM's shared memory");
 };
 
 __device__ __forceinline__ float bias_value(const Params& p, int z, int h, int q, int k) {
@@ -104,21 +121,14 @@ __device__ __forceinline__ float bias_value(const Params& p, int z, int h, int q
   return __half2float(__ldg(reinterpret_cast<const __half*>(p.bias) + off));
 }
 
-// What the softmax of a kernel handles: kPlain an optional causal mask; kExtra also bias, softcap and
-// windows, element by element; kWindow a window with sinks and a positive scale, the scale folded into
-// the exponent as in kPlain and masks only on the key tiles that cross the edge of what a warp's rows
-// see. Up to 32 sinks, ahead of the window, cost a quarter of a key tile: S has 32 columns, P V two steps.
-// Bound by the chain S -> softmax -> P -> P V of each key tile, as kPlain is (its rate on dense causal
-// attention, 0.9 PFLOP/s, is what the tiles here run at too); the window leaves 9 to 10 tiles per block.
-// 4096 tokens, 64 / 8 heads of 128, window 1024, 4 sinks: 179 us, 0.68 PFLOP/s of visible pairs (196 us with a
-// whole tile for the sinks and one mask for every edge); kExtra takes some ten times as long.
-enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
-
 template <typename T, int D, bool VARLEN, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<MODE>::kThreads, Shape<MODE>::kCtas)
     fmha_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const Params p) {
-  using L = Layout<D>;
+  using L = Layout<D, MODE>;
+  using C = Shape<MODE>;
+  constexpr int kQTiles = C::kQTiles, kBlockM = C::kBlockM, kStages = L::kStages;
+  constexpr int kProducerWarp = 4 * kQTiles, kMmaWarp = kProducerWarp + 1;
   constexpr bool EXTRA = MODE == kExtra;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = make_idesc_f16(kBF16, kBM, kBN, false, false);
@@ -132,8 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h = bh % p.hq;
   const int zb = bh / p.hq;  // batch (dense) or sequence (varlen)
   const int qb = p.q_tiles - 1 - (int)blockIdx.x;
-  const bool half = MODE == kWindow && p.half;
-  const int m0 = qb * (half ? kBM : kBlockM);
+  const int m0 = qb * kBlockM;
   int len_q, len_k, row_q0, row_k0;
   if constexpr (VARLEN) {
     row_q0 = p.cu_q[zb];
@@ -167,15 +176,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     sk_t[t] = 0;
     few_t[t] = false;
-    const bool idle = mt >= len_q || (half && t > 0);
-    if (idle || k_hi <= k_lo) {
+    if (mt >= len_q || k_hi <= k_lo) {
       lo_t[t] = hi_t[t] = 0;
     } else {
       lo_t[t] = k_lo / kBN;
       hi_t[t] = (k_hi + kBN - 1) / kBN;
     }
     if constexpr (MODE != kPlain) {
-      if (p.sinks > 0 && !idle) {
+      if (p.sinks > 0 && mt < len_q) {
         const int end = min(min(p.sinks, len_k), p.causal ? mt + kBM : len_k);
         sk_t[t] = (end + kBN - 1) / kBN;
         few_t[t] = MODE == kWindow && p.sinks <= kFewSinks && k_lo >= kBN;
@@ -207,8 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* meta = smem_raw + pad + L::kMeta;
   const uint32_t smeta = sb + L::kMeta;
   const uint32_t bar_q = smeta;
-  const uint32_t bar_kfull = smeta + 8;     // [kKStages <= 3]
-  const uint32_t bar_kempty = smeta + 32;   // [kKStages <= 3]
+  const uint32_t bar_kfull = smeta + 8;     // [kStages <= 2]
+  const uint32_t bar_kempty = smeta + 32;   // [kStages <= 2]
   const uint32_t bar_vfull = smeta + 56;    // [2]
   const uint32_t bar_vempty = smeta + 72;   // [2]
   const uint32_t bar_sfull = smeta + 88;    // [2] per query tile
@@ -225,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
-    for (int i = 0; i < kKStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(bar_kfull + 8 * i, 1);
       mbar_init(bar_kempty + 8 * i, 1);
     }
@@ -245,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tm_v);
   }
   if (warp == kMmaWarp) {
-    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Each role's code is dominated by its warpgroup's setmaxnreg (no join in between),
   // so the compiler allocates the softmax code against 216 registers.
   if (warp >= kProducerWarp) {
-  setmaxnreg_dec<kRegsControl>();
+  setmaxnreg_dec<C::kRegsControl>();
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n_tiles > 0) {
@@ -268,17 +276,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_4d(sb + L::kQ + t * L::kTile + c * L::kChunk, &tm_q, bar_q, c * 64,
                       row_q0 + m0 + t * kBM, h, zc);
       for (int u = 0; u < n_tiles; ++u) {
-        const int st = u & 1;
-        const uint32_t ph = (u >> 1) & 1;
-        const int ks = u % kKStages;
-        const uint32_t kph = (u / kKStages) & 1;
+        const int st = u % kStages;
+        const uint32_t ph = (u / kStages) & 1;
         const int krow = row_k0 + tile_at(u) * kBN;
-        if (!wait_bounded(bar_kempty + 8 * ks, kph ^ 1, abort_flag, p.status, kStatusTimeoutProducer))
+        if (!wait_bounded(bar_kempty + 8 * st, ph ^ 1, abort_flag, p.status, kStatusTimeoutProducer))
           break;
-        mbar_arrive_expect_tx(bar_kfull + 8 * ks, L::kTile);
+        mbar_arrive_expect_tx(bar_kfull + 8 * st, L::kTile);
 #pragma unroll
         for (int c = 0; c < L::kChunks; ++c)
-          tma_load_4d(sb + L::kK0 + ks * L::kTile + c * L::kChunk, &tm_k, bar_kfull + 8 * ks, c * 64,
+          tma_load_4d(sb + L::kK0 + st * L::kTile + c * L::kChunk, &tm_k, bar_kfull + 8 * st, c * 64,
                       krow, hk, zc);
         if (!wait_bounded(bar_vempty + 8 * st, ph ^ 1, abort_flag, p.status, kStatusTimeoutProducer))
           break;
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto issue_s = [&](int t, int u) {
         const uint32_t idesc =
             few(t, tile_at(u)) ? make_idesc_f16(kBF16, kBM, kFewSinks, false, false) : kIdescS;
-        const uint32_t k_addr = sb + L::kK0 + (u % kKStages) * L::kTile;
+        const uint32_t k_addr = sb + L::kK0 + (u % kStages) * L::kTile;
         const uint32_t q_addr = sb + L::kQ + t * L::kTile;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -309,9 +315,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // O_t += P_t V_j over keys [64 * half, 64 * half + 64) of the tile
       auto issue_pv = [&](int t, int u, bool first, int half) {
-        const int st = u & 1;
+        const int st = u % kStages;
         const uint32_t v_addr = sb + L::kV0 + st * L::kTile;
-        const uint32_t o_tmem = tmem_base + 256 + t * 128;
+        const uint32_t o_tmem = tmem_base + kQTiles * 128 + t * 128;
         const uint32_t p_tmem = tmem_base + t * kBN;
 #pragma unroll
         for (int k4 = 0; k4 < kBN / 32; ++k4) {
@@ -332,12 +338,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int u = 0; u < n_tiles && ok; ++u) {
         const int j = tile_at(u), jn = tile_at(u + 1);
-        const int st = u & 1;
-        const uint32_t ph = (u >> 1) & 1;
+        const int st = u % kStages;
+        const uint32_t ph = (u / kStages) & 1;
         ok = wait_bounded(bar_vfull + 8 * st, ph, abort_flag, p.status, kStatusTimeoutMma);
         const bool next = (u + 1 < n_tiles);
-        const int kn = (u + 1) % kKStages;
-        const uint32_t knph = ((u + 1) / kKStages) & 1;
+        const int kn = (u + 1) % kStages;
+        const uint32_t knph = ((u + 1) / kStages) & 1;
         bool k_ready = !next;
         if (!GKO_FMHA_LATE_KWAIT && ok && next) {
           ok = wait_bounded(bar_kfull + 8 * kn, knph, abort_flag, p.status, kStatusTimeoutMma);
@@ -384,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   } else {
-    setmaxnreg_inc<kRegsSoftmax>();
+    setmaxnreg_inc<C::kRegsSoftmax>();
     // ------------------------------------------------------------ softmax / epilogue
     const int t = warp >> 2;            // query tile of this warpgroup
     const int quarter = warp & 3;       // TMEM lane quarter
@@ -392,10 +398,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int qi = m0 + t * kBM + r;    // query index within the sequence
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_tmem = tmem_base + lane_off + t * kBN;
-    const uint32_t o_tmem = tmem_base + lane_off + 256 + t * 128;
-    const int jlo = t ? lo_t[1] : lo_t[0];
-    const int jsk = t ? sk_t[1] : sk_t[0];
-    const int n_mine = jsk + (t ? hi_t[1] : hi_t[0]) - jlo;
+    const uint32_t o_tmem = tmem_base + lane_off + kQTiles * 128 + t * 128;
+    constexpr int kLast = kQTiles - 1;
+    const int jlo = t ? lo_t[kLast] : lo_t[0];
+    const int jsk = t ? sk_t[kLast] : sk_t[0];
+    const int n_mine = jsk + (t ? hi_t[kLast] : hi_t[0]) - jlo;
     const int mt = m0 + t * kBM;
     float m_run = -INFINITY;  // running max, log2 domain
     float l_run = 0.f;
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       if constexpr (MODE == kWindow) {
-        if (i < jsk && (t ? few_t[1] : few_t[0])) {  // the first tile: nothing to rescale yet
+        if (i < jsk && (t ? few_t[kLast] : few_t[0])) {  // the first tile: nothing to rescale yet
           uint32_t su[kFewSinks];
           tmem_ld32p(s_tmem, su);
           tmem_wait_ld();
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
     }
     // varlen: rows outside [0, total_q) (cu_seqlens past the packed tokens) are never written
-    const bool write = qi < len_q && !(half && t > 0) && (!VARLEN || (row_q0 >= 0 && row_q0 + qi < p.total_q));
+    const bool write = qi < len_q && (!VARLEN || (row_q0 >= 0 && row_q0 + qi < p.total_q));
     T* orow;
     if constexpr (VARLEN)
       orow = reinterpret_cast<T*>(p.out) + ((int64_t)(row_q0 + qi) * p.hq + h) * D;
@@ -614,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(tmem_base, kTmemCols);
+  if (warp == kMmaWarp) tmem_dealloc(tmem_base, C::kTmemCols);
 }
 
 // ------------------------------------------------------------------ host side
@@ -627,11 +634,11 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
     cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes);
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D, MODE>::kBytes);
     if (e != cudaSuccess) return host::cuda_check(e, "cudaFuncSetAttribute(fmha)");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  kern<<<grid, kThreads, Layout<D>::kBytes, s>>>(tq, tk, tv, p);
+  kern<<<grid, Shape<MODE>::kThreads, Layout<D, MODE>::kBytes, s>>>(tq, tk, tv, p);
   return host::cuda_check(cudaGetLastError(), "fmha kernel launch");
 }
 
@@ -659,12 +666,7 @@ int mode_of(bool bias, float softcap, int window, int sinks, float scale) {
   return kPlain;
 }
 
-// Whether windows with sinks take query blocks of 128 rows: where blocks of 256 would leave half of the
-// SMs idle. A lone tile cannot hide its softmax behind another's products, but the CTAs run side by side
-// (2 x 8 heads, 1000 queries, 1777 keys, window 300 both ways: 27.6 us with 256 rows, 21.9 with 128; 12 heads,
-// 513 tokens, window 128: 11.6 and 8.5 us). With more blocks than that 256 rows are faster: K and V are
-// fetched half as often.
-bool half_blocks(int mode, int64_t blocks) { return mode == kWindow && 2 * blocks <= host::sm_count(); }
+int block_rows(int mode) { return mode == kWindow ? Shape<kWindow>::kBlockM : Shape<kPlain>::kBlockM; }
 
 // Grid: query blocks along x, (batch, head) pairs along y (and z beyond 65535).
 dim3 grid_of(int q_blocks, int zh) {
@@ -748,7 +750,6 @@ extern "C" int gko_fmha_sinks_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv,
   p.group = (int)(hq / hkv);
   p.sq = (int)sq;
   p.sk = (int)sk;
-  p.q_tiles = (int)((sq + fmha::kBlockM - 1) / fmha::kBlockM);
   p.scale = scale;
   p.scale_log2 = scale * fmha::kLog2e;
   p.softcap = softcap;
@@ -792,9 +793,8 @@ extern "C" int gko_fmha_sinks_fwd(int dtype, int64_t z, int64_t hq, int64_t hkv,
   p.lse_stride_h = sq;
   p.status = status;
   const int mode = fmha::mode_of(bias_mode != GKO_BIAS_NONE, softcap, window, p.sinks, scale);
+  p.q_tiles = (int)((sq + fmha::block_rows(mode) - 1) / fmha::block_rows(mode));
   p.zh = (int)(z * hq);
-  p.half = fmha::half_blocks(mode, (int64_t)p.q_tiles * p.zh);
-  if (p.half) p.q_tiles = (int)((sq + fmha::kBM - 1) / fmha::kBM);
   const dim3 grid = fmha::grid_of(p.q_tiles, p.zh);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, false>((int)d, mode, tq, tk, tv, p, grid, s);
@@ -845,7 +845,6 @@ extern "C" int gko_fmha_sinks_varlen_fwd(int dtype, int64_t b, int64_t hq, int64
   p.hq = (int)hq;
   p.hkv = (int)hkv;
   p.group = (int)(hq / hkv);
-  p.q_tiles = (int)((max_seqlen_q + fmha::kBlockM - 1) / fmha::kBlockM);
   p.scale = scale;
   p.scale_log2 = scale * fmha::kLog2e;
   p.softcap = softcap;
@@ -862,9 +861,8 @@ extern "C" int gko_fmha_sinks_varlen_fwd(int dtype, int64_t b, int64_t hq, int64
   p.total_q = (int)tq;
   p.status = status;
   const int mode = fmha::mode_of(false, softcap, window, p.sinks, scale);
+  p.q_tiles = (int)((max_seqlen_q + fmha::block_rows(mode) - 1) / fmha::block_rows(mode));
   p.zh = (int)(b * hq);
-  p.half = fmha::half_blocks(mode, (int64_t)p.q_tiles * p.zh);
-  if (p.half) p.q_tiles = (int)((max_seqlen_q + fmha::kBM - 1) / fmha::kBM);
   const dim3 grid = fmha::grid_of(p.q_tiles, p.zh);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == GKO_BF16) return fmha::dispatch<__nv_bfloat16, true>((int)d, mode, mq, mk, mv, p, grid, s);

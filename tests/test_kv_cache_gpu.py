@@ -384,40 +384,55 @@ def test_attend_captured_on_a_side_stream():
 
 
 # --------------------------------------------------------------------------- together, and refusals
-@pytest.mark.parametrize("bits,tol", [(4, 0.2), (8, 0.02)])
-def test_prompt_then_tokens(bits, tol):
-    """A prompt is written, read back for the packed attention, and answered token by token from the cache: the
-    cached answers equal those over the read-back rows, and are near those over the unquantised ones."""
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompt_then_tokens(bits):
+    """A prompt's attention with window and sinks, its keys and values written, then answered token by token from the
+    cache, and read back: every answer is the 64-bit attention over the rows the cache stands for, those rows are within
+    half a step of what was written, and the packed attention over the read-back rows gives the last answers again."""
     kernels.register("kv_cache")
     gen = torch.Generator().manual_seed(20)
-    lens, hq, hkv, d, page, steps = [70, 33], 8, 2, 128, 16, 3
+    lens, hq, hkv, d, page, steps, window, sinks = [70, 33], 8, 2, 128, 16, 3, 24, 4
     full = [n + steps for n in lens]
     table = torch.randperm(12, generator=gen)[:12].view(2, 6).to(torch.int32)
     cache = ops.kv_cache_alloc(12, page, hkv, d, bits)
     q, k, v = ([_rows(gen, n, h, d, dtype=torch.bfloat16) for n in full] for h in (hq, hkv, hkv))
     slot = lambda i, t: int(table[i, t // page]) * page + t % page  # noqa: E731
     prompt = lambda x: torch.cat([t[:n] for t, n in zip(x, lens)]).to(DEV)  # noqa: E731
+    cu = torch.tensor([0, lens[0], sum(lens)], dtype=torch.int32, device=DEV)
+    first, _ = ops.fmha_varlen_fwd(prompt(q), prompt(k), prompt(v), cu, cu, max(lens), max(lens), None, 1, window, sinks=sinks)
+    for i, (a, e) in enumerate(((0, lens[0]), (lens[0], sum(lens)))):
+        want, _, p = oracle.attention64(q[i][:lens[i]], k[i][:lens[i]], v[i][:lens[i]], d ** -0.5, 1, window, 0.0, sinks)
+        # bf16 probabilities and outputs, and the logits' f32 rounding (far below those)
+        tol = 2.0 ** -8 * (torch.einsum("hij,jhd->ihd", p, v[i][:lens[i]].double().abs().repeat_interleave(4, 1)) + want.abs())
+        assert ((first[a:e].cpu().double() - want).abs() <= tol + 1e-3 * tol.amax()).all()
     torch.ops.gko.kv_cache_write(prompt(k), prompt(v), *cache,
                                  torch.tensor([slot(i, t) for i, n in enumerate(lens) for t in range(n)], device=DEV))
     for s in range(steps):
         at = [n + s for n in lens]
-        now = lambda x: torch.stack([t[n] for t, n in zip(x, at)]).to(DEV)  # noqa: E731
-        torch.ops.gko.kv_cache_write(now(k), now(v), *cache, torch.tensor([slot(i, t) for i, t in enumerate(at)], device=DEV))
-        out, _ = torch.ops.gko.fmha_cache_fwd(now(q), *cache, table.to(DEV),
-                                              torch.tensor([t + 1 for t in at], dtype=torch.int32, device=DEV), None, 1,
-                                              100, d ** -0.5, 1, 24, 0.0, 4)
-        for i, t in enumerate(at):
-            want, _, _ = oracle.attention64(q[i][t:t + 1], k[i][:t + 1], v[i][:t + 1], d ** -0.5, 1, 24, 0.0, 4, t)
-            assert (out[i].cpu().double() - want[0]).abs().max() <= tol * want.abs().max()
+        now = lambda x: torch.stack([t[n] for t, n in zip(x, at)])  # noqa: E731
+        torch.ops.gko.kv_cache_write(now(k).to(DEV), now(v).to(DEV), *cache,
+                                     torch.tensor([slot(i, t) for i, t in enumerate(at)], device=DEV))
+        seen = [t + 1 for t in at]
+        got = torch.ops.gko.fmha_cache_fwd(now(q).to(DEV), *cache, table.to(DEV),
+                                           torch.tensor(seen, dtype=torch.int32, device=DEV), None, 1, 100, d ** -0.5, 1,
+                                           window, 0.0, sinks)
+        held = ops.KVCache(*(t.cpu() for t in cache))
+        _check_attention(got, now(q), held, table, seen, [1, 1], bits, 1, window, 0.0, sinks, d ** -0.5)
     cu = torch.tensor([0, full[0], sum(full)], dtype=torch.int32, device=DEV)
     kb, vb = torch.ops.gko.kv_cache_read(*cache, table.to(DEV), cu, sum(full), d)
-    packed, _ = ops.fmha_varlen_fwd(torch.cat(q).to(DEV), kb, vb, cu, cu, max(full), max(full), d ** -0.5, 1)
+    for x, c, back in ((k, 0, kb), (v, 1, vb)):
+        for i, (a, e) in enumerate(((0, full[0]), (full[0], sum(full)))):
+            used = table[i, : -(-full[i] // page)].long()
+            step = held[c + 2][used].transpose(1, 2).flatten(0, 1)[: full[i], :, :1].double()
+            held_rows = oracle.kv_sequence(held[c], held[c + 2], table[i], full[i], bits)
+            assert ((back[a:e].cpu().double() - held_rows).abs() <= held_rows.abs() * 2.0 ** -8).all()
+            assert ((held_rows - x[i].double()).abs() <= step * (0.5 + 2.0 ** -14)).all()
+    packed, _ = ops.fmha_varlen_fwd(torch.cat(q).to(DEV), kb, vb, cu, cu, max(full), max(full), d ** -0.5, 1, window,
+                                    sinks=sinks)
     last = torch.tensor([full[0] - 1, sum(full) - 1])
-    out, _ = ops.fmha_cache_fwd(torch.cat(q)[last].to(DEV), cache, table.to(DEV),
-                                torch.tensor(full, dtype=torch.int32, device=DEV))
+    # both round probabilities (bf16 there) and outputs; the read-back rows are rounded to bf16 once more
+    assert (got[0] - packed[last]).abs().max() <= 4 * 2.0 ** -8 * packed[last].abs().max()
     _status_clear()
-    # both round P (bf16 there) and their outputs; the read-back rows are rounded to bf16 once more
-    assert (out - packed[last]).abs().max() <= 4 * 2.0 ** -8 * packed[last].abs().max()
 
 
 def test_refusals():
