@@ -26,21 +26,22 @@
 // Columns of a CTA are (new token, query head) pairs of one kv head, kCols at a time. A CTA takes
 // one range of the keys of one column tile, kv head and sequence; its warps take slabs of 32 keys in turn,
 // each with its own running maximum, sum and accumulators, and join at the end in a fixed order.
-// Every warp keeps a ring of slabs in flight for itself (bulk copies of codes and pairs into shared
-// memory, completing on an mbarrier of the warp), so the loop has no barrier between warps and the
-// memory system always has several slabs per warp to work on.
+// Every warp keeps a ring of slabs in flight for itself (asynchronous copies of codes and pairs into
+// shared memory: its lanes' own for 4 bits; the copy engine's, completing on an mbarrier of the warp, for
+// 8), so the loop has no barrier between warps and the memory system always has several slabs per warp
+// to work on.
 // A tile whose keys are split goes to the workspace in parts and a second kernel adds them, again in
 // a fixed order, so results do not vary from run to run. Splits follow the lengths on the device (see
 // `place`): sequences of 512 to 8192 tokens are shared out as evenly as one of 131072.
 //
 // Measured, 8 kv heads of 128, groups of 8, bf16 (both kernels):
-//   4 bits  131072 tokens 43 us (3.3 TB/s); 16 sequences of 512 to 8192 tokens 35 us; 64 of 8192 145 us
-//           (3.95 TB/s; the same from L2: 141 us)
+//   4 bits  131072 tokens 41 us (3.5 TB/s); 16 sequences of 512 to 8192 tokens 34 us; 64 of 8192 133 us
+//           (4.3 TB/s)
 //   8 bits  131072 tokens 54 us (5.1 TB/s); 64 sequences of 8192 203 us (5.5 TB/s)
-// 8 bits are bound by memory, 4 bits by the work on the codes: per slab and SM 306 cycles, of which the V
+// 8 bits are bound by memory, 4 bits by the work on the codes: per slab and SM 280 cycles, of which the V
 // products and their unpacking take 67, the S products as much (51 of them the tensor pipe's), and copies
-// alone would need 205 at their 5.85 TB/s. No pipe is full (issue slots 61 %, integer 55 %, tensor 28 %); five
-// CTAs per SM instead of four, two stages instead of three, or 16 fewer instructions a slab change nothing.
+// alone would need 205 at their 5.85 TB/s; without any fetch the rest takes 250. No pipe is full; five CTAs
+// per SM instead of four, or two stages instead of three, change nothing.
 // About 10 us of a single sequence's time are the two launches, the first loads and the joining.
 #include <type_traits>
 
@@ -298,6 +299,11 @@ struct Row {
   static constexpr int kStage = kVP + kSlab * 4;
   static constexpr int kStages = kStage > 4096 ? 2 : 3;
   static constexpr int kRing = kWarps * kStages * kStage;
+  // How slabs are fetched: by the copy engine, two or four copies of rows and as many of pairs, or by
+  // 16-byte copies of the lanes. Measured, 8 kv heads of 128: lanes cost fewer instructions, which 4 bits
+  // are bound by (64 sequences of 8192: 134 us, copy engine 145; 131072 tokens 41 us, 43), but keep
+  // memory less busy, which 8 bits are bound by (216 us, 203; 60 us, 54).
+  static constexpr bool kBulk = BITS == 8;
 };
 
 // Key rows of 16 of a half slab go to the operand's rows in this order: neighbours swap places in
@@ -351,7 +357,6 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   __shared__ int q_pos[kCols];
   __shared__ float w_max[kWarps][kCols], w_sum[kWarps][kCols], w_zero[kWarps][kCols];
   __shared__ __align__(8) uint64_t bars[kWarps][R::kStages];
-  __shared__ int have_s[kWarps][R::kStages];
   __shared__ int abort_s;
   extern __shared__ __align__(16) uint8_t ring[];
   // after the loop the ring is done with, and each warp's part takes its accumulators
@@ -385,77 +390,98 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int li = lane & 3, lj = lane >> 2;
   volatile int* abort_flag = &abort_s;
-  if (threadIdx.x == 0) {
-    abort_s = 0;
-    for (int i = 0; i < kWarps * R::kStages; ++i) mbar_init(smem_u32(&bars[0][i]), 1);
-    fence_mbar_init();
+  if (R::kBulk) {
+    if (threadIdx.x == 0) {
+      abort_s = 0;
+      for (int i = 0; i < kWarps * R::kStages; ++i) mbar_init(smem_u32(&bars[0][i]), 1);
+      fence_mbar_init();
+    }
+    __syncthreads();
   }
-  __syncthreads();
 
-  // The ring. Lane 4 j + x copies part x (codes of K, V, pairs of K, V) of the warp's j-th slab of a
-  // batch of eight; where pages do not hold whole slabs, lane 8 j + 4 hf + x copies that part of half hf
-  // and a batch is four slabs. Addresses are worked out a batch at a time, page numbers fetched a batch
-  // ahead, so a slab costs a handful of instructions and never waits for the block table.
+  // The ring. Lane 2 j + hf works out where half hf of the warp's j-th slab of a batch of 16 starts (its
+  // row of the cache, all pages and heads counted); page numbers are fetched a batch ahead, so a slab
+  // costs a handful of instructions and never waits for the block table.
   const int32_t* table = p.table + (int64_t)b * p.table_stride;
   const uint32_t my_ring = smem_u32(ring) + warp * (R::kStages * R::kStage);
   const uint32_t my_bar = smem_u32(&bars[warp][0]);
-  const bool whole = p.page_size % kSlab == 0;
-  const int lane_shift = whole ? 2 : 3;
-  const int my_slab = lane >> lane_shift, my_part = lane & 3, my_half = whole ? 0 : (lane >> 2) & 1;
   const int jump = (rg.lo - rg.first) * kSlab;
   auto first_key = [&](int v) { return v * kSlab + (v < rg.first ? 0 : jump); };
-  const int copy_width = my_part < 2 ? R::kBytes : 4;  // bytes of a row of this lane's part
-  const int64_t copy_page = (int64_t)p.hkv * p.page_size * copy_width;
-  const uint8_t* copy_from = (my_part == 0   ? p.k_codes
-                              : my_part == 1 ? p.v_codes
-                              : my_part == 2 ? reinterpret_cast<const uint8_t*>(p.k_pairs)
-                                             : reinterpret_cast<const uint8_t*>(p.v_pairs)) +
-                             (int64_t)hk * p.page_size * copy_width;
-  const uint32_t copy_to = my_ring + (my_part == 0 ? 0 : my_part == 1 ? R::kV : my_part == 2 ? R::kKP : R::kVP) +
-                           my_half * 16 * copy_width;
-  const uint32_t copy_bytes = (whole ? kSlab : 16) * copy_width;
-  auto lookup = [&](int v) {  // page of this lane's slab of the batch that starts at v
-    const int t = first_key(v + my_slab * kWarps) + my_half * 16;
+  auto first_of = [&](int v) { return first_key(v + (lane >> 1) * kWarps) + (lane & 1) * 16; };
+  auto lookup = [&](int v) {  // page of this lane's half slab of the batch that starts at v
+    const int t = first_of(v);
     const int col = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
-    return v + my_slab * kWarps < v1 && t < sq.len && col < p.table_width ? table[col] : -1;
+    return v + (lane >> 1) * kWarps < v1 && t < sq.len && col < p.table_width ? table[col] : -1;
   };
-  const uint8_t* copy_src = nullptr;
-  unsigned good = 0;  // lanes whose copy exists
+  constexpr uint32_t kNoRow = 0xffffffffu;
+  uint32_t row = kNoRow;
   auto plan_batch = [&](int v, int page) {
-    const int t = first_key(v + my_slab * kWarps) + my_half * 16;
+    const int t = first_of(v);
     const bool ok = page >= 0 && page < p.pages;
-    if (!ok && v + my_slab * kWarps < v1 && t < sq.len && my_part == 0 && p.status) atomicOr(p.status, kStatusBadIndex);
+    if (!ok && v + (lane >> 1) * kWarps < v1 && t < sq.len && p.status) atomicOr(p.status, kStatusBadIndex);
     const int inside = p.page_shift >= 0 ? t & (p.page_size - 1) : t % p.page_size;
-    copy_src = copy_from + (ok ? page : 0) * copy_page + inside * copy_width;
-    good = __ballot_sync(0xffffffffu, ok);
+    row = ok ? ((uint32_t)page * p.hkv + hk) * p.page_size + inside : kNoRow;
   };
-  int turn = 0;  // the batch's next slab
+  int turn = 0;           // the batch's next slab
+  uint32_t halves = 0;    // which halves of the slabs in flight exist, two bits each, the oldest lowest
+  const bool whole = p.page_size % kSlab == 0;  // both halves of a slab lie in one page
+  // lanes: 16 bytes of every 512 of codes; lanes 0 to 7 four pairs of K each, lanes 8 to 15 four of V
+  // copy engine: lane 4 hf + x copies part x (codes of K, V, pairs of K, V) of half hf, or of the whole slab
+  const int part = lane & 3, width = part < 2 ? R::kBytes : 4;
+  const uint8_t* const parts[4] = {p.k_codes, p.v_codes, reinterpret_cast<const uint8_t*>(p.k_pairs),
+                                   reinterpret_cast<const uint8_t*>(p.v_pairs)};
+  const uint8_t* from0 = R::kBulk ? part == 0 ? parts[0] : part == 1 ? parts[1] : part == 2 ? parts[2] : parts[3]
+                                  : parts[0] + lane * 16;
+  const uint8_t* from1 = parts[1] + lane * 16;
+  const uint8_t* from2 = ((lane & 8) ? parts[3] : parts[2]) + (lane & 3) * 16;
+  const uint32_t copy_to = R::kBulk ? my_ring + (part == 0 ? 0 : part == 1 ? R::kV : part == 2 ? R::kKP : R::kVP) +
+                                          (lane >> 2) * 16 * width
+                                    : my_ring + lane * 16;
   auto fetch = [&](int st) {
-    const unsigned g = good >> (turn << lane_shift);
-    if (lane == 0) {
-      const int have = whole ? ((g & 1) ? 3 : 0) : ((g & 1) | ((g >> 3) & 2));
-      have_s[warp][st] = have;
-      mbar_arrive_expect_tx(my_bar + 8 * st, ((have & 1) + (have >> 1)) * 16 * (2 * R::kBytes + 8));
+    const uint32_t r[2] = {__shfl_sync(0xffffffffu, row, turn), __shfl_sync(0xffffffffu, row, turn + 1)};
+    const uint32_t mine = (lane & 4) ? r[1] : r[0];
+    const uint32_t to = copy_to + st * R::kStage;
+    uint32_t have = (r[0] != kNoRow ? 1u : 0u) | (r[1] != kNoRow ? 2u : 0u);
+    if (R::kBulk) {
+      if (whole) have = r[0] != kNoRow ? 3 : 0;
+      if (lane == 0) mbar_arrive_expect_tx(my_bar + 8 * st, __popc(have) * 16 * (2 * R::kBytes + 8));
+      __syncwarp();
+      if (lane < (whole ? 4 : 8) && mine != kNoRow)
+        bulk_load(to, from0 + (uint64_t)mine * width, (whole ? kSlab : 16) * width, my_bar + 8 * st);
+      return have;
     }
-    __syncwarp();
-    if (my_slab == turn && ((good >> lane) & 1)) bulk_load(copy_to + st * R::kStage, copy_src, copy_bytes, my_bar + 8 * st);
+    constexpr int kHalf = R::kBytes / 32;  // 512-byte copies of a half slab's codes
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      if (r[hf] == kNoRow) continue;
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i) {
+        cp_async16(to + (hf * kHalf + i) * 512, from0 + (uint64_t)r[hf] * R::kBytes + i * 512);
+        cp_async16(to + R::kV + (hf * kHalf + i) * 512, from1 + (uint64_t)r[hf] * R::kBytes + i * 512);
+      }
+    }
+    if (lane < 16 && mine != kNoRow) cp_async16(to + R::kKP, from2 + (uint64_t)mine * 4);
+    return have;
   };
-  const int batch = 32 >> lane_shift;
+  constexpr int kBatch = 16;
   int ahead = v0 + warp;  // the next slab to fetch
   plan_batch(ahead, lookup(ahead));
-  int next_page = lookup(ahead + batch * kWarps);
-  auto fetch_next = [&](int st) {
-    fetch(st);
-    ahead += kWarps;
-    if (++turn == batch) {
-      turn = 0;
-      plan_batch(ahead, next_page);
-      next_page = lookup(ahead + batch * kWarps);
+  int next_page = lookup(ahead + kBatch * kWarps);
+  auto fetch_next = [&](int st, int place) {
+    if (ahead < v1) {
+      halves |= fetch(st) << (2 * place);
+      ahead += kWarps;
+      turn += 2;
+      if (turn == 2 * kBatch) {
+        turn = 0;
+        plan_batch(ahead, next_page);
+        next_page = lookup(ahead + kBatch * kWarps);
+      }
     }
+    if (!R::kBulk) cp_async_commit();  // a group per slab, empty ones past the end
   };
 #pragma unroll
-  for (int i = 0; i < R::kStages; ++i)
-    if (ahead < v1) fetch_next(i);
+  for (int i = 0; i < R::kStages; ++i) fetch_next(i, i);
 
   // queries, each column divided by the power of two below its largest value (exact, and any size of
   // bf16 query comes within range), in pieces; the factor that undoes it and the sum over d
@@ -559,11 +585,17 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
   int v = v0 + warp;
   for (; v < v1; v += kWarps) {
     const int t0 = first_key(v);
-    if (!wait_bounded(my_bar + 8 * st, phase, abort_flag, p.status, kStatusTimeoutProducer)) {
-      ok = false;
-      break;
+    if (R::kBulk) {
+      if (!wait_bounded(my_bar + 8 * st, phase, abort_flag, p.status, kStatusTimeoutProducer)) {
+        ok = false;
+        break;
+      }
+    } else {
+      cp_async_wait<R::kStages - 1>();
+      __syncwarp();
     }
-    const int have_bits = have_s[warp][st];
+    const uint32_t have_bits = halves & 3;
+    halves >>= 2;
     const uint8_t* slab = ring + (warp * R::kStages + st) * R::kStage;
     // whether some key of the slab is hidden from some column (or is not there at all)
     const bool edge = have_bits != 3 || ((t0 < whole_from || t0 + kSlab > whole_to) && t0 + kSlab > whole_sinks);
@@ -785,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
     // every lane has read the slab: its place goes to the slab kStages further on
     __syncwarp();
-    if (ahead < v1) fetch_next(st);
+    fetch_next(st, R::kStages - 1);
     if (++st == R::kStages) {
       st = 0;
       phase ^= 1;
@@ -1085,8 +1117,9 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
     return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: the page size must be a multiple of 16 up to 2^20, got %lld",
                 (long long)page_size);
   if (pages < 0 || table_width < 0 || table_stride < 0) return fail(GKO_ERR_INVALID, "fmha over a cache: bad sizes");
-  if (table_width * page_size >= (1ll << 31) || pages >= (1ll << 31))
-    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: a sequence may hold fewer than 2^31 tokens");
+  if (table_width * page_size >= (1ll << 31) || pages >= (1ll << 31) ||
+      (pages > 0 && hkv > 0 && page_size > 0 && pages * hkv >= 0xffffffffll / page_size))
+    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: a sequence may hold fewer than 2^31 tokens, the cache fewer than 2^32 rows");
   if (b == 0 || tq == 0 || max_seqlen_q == 0) return GKO_OK;
   if (!q || !k_codes || !v_codes || !k_pairs || !v_pairs || (!table && table_width > 0) || !seq_lens || !out || !lse)
     return fail(GKO_ERR_INVALID, "fmha over a cache: null pointer argument");

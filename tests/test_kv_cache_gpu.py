@@ -291,6 +291,26 @@ def test_attend_bad_values_and_pages():
     assert _same(got, base)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page,holes", [(16, [0, 3, 4, 9, 70, 99]), (32, [1, 2, 30]), (48, [0, 5, 21])])
+def test_attend_pages_missing_anywhere(bits, d, page, holes):
+    """Pages that are none, at either half of a slab of 32 keys, in pairs and far into a sequence, count as
+    masked: the result is that of the sequence without them."""
+    gen = torch.Generator().manual_seed(bits + d + page)
+    lens = [1650, 1650]
+    cache, table = _cache(gen, lens, page, 2, d, bits, torch.bfloat16)
+    q = _rows(gen, 2, 8, d, dtype=torch.bfloat16)
+    bad = table.clone()
+    bad[1, holes] = -5
+    got = ops.fmha_cache_fwd(q.to(DEV), _to(cache), bad.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    _status_clear(0x20)
+    left = [c for c in range(table.shape[1]) if c not in holes]
+    short = table.clone()
+    short[1, : len(left)] = table[1, left]
+    _check_attention(got, q, cache, short, [1650, 1650 - page * len(holes)], [1, 1], bits, 1, 0, 0.0, 0, d ** -0.5)
+
+
 def test_empty_tables():
     """No sequence has a token yet: a block table of no columns, rows of zeros and -inf, nothing read back."""
     cache = ops.kv_cache_alloc(2, 16, 2, 64, 4)
