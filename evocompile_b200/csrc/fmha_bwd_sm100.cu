@@ -18,7 +18,7 @@
 // With a window and sinks (leading keys that stay visible) the key tiles that hold sinks are seen by
 // every query, the others by a window of them. A sink tile's queries are split over several CTAs of
 // about a window tile's work each, first in the grid; their dk / dv parts go to the workspace in f32 and
-// a fourth kernel adds them in a fixed order. There (no bias, no softcap) dq = scale dS k also takes its keys
+// the convert kernel adds them in a fixed order. There (no bias, no softcap) dq = scale dS k also takes its keys
 // minus one vector per kv head, about their mean: each row of dS sums to zero, so the product is the same, but
 // the roundings of dS and of delta, which do not, no longer meet the keys' common part (keys whose channels have
 // means of 1.5 deviations: relative error of dq 0.0050 to 0.0029 in bf16).
@@ -130,6 +130,7 @@ struct RowParams {
   int sk, group, total_k;
   const int* cu_k;
   float* centre;
+  int join;  // blocks of the convert kernel that join the sinks' parts of one kv head
 };
 
 // Rows [row0, row0 + len) of sequence b (varlen), clamped to the packed tokens [0, total):
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return (VARLEN ? (int64_t)h : (int64_t)zb * p.hq + h) * p.tiles_per_head + tile_base + jb;
   };
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);  // uniform, and known to be
   const int lane = threadIdx.x & 31;
   T* dk_base;
   T* dv_base;
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     setmaxnreg_dec<kRegsControl>();
     if (warp == kProducerWarp) {
       // ---------------------------------------------------------- TMA producer
-      if (lane == 0) {
+      if (elect_one()) {
         mbar_arrive_expect_tx(bar_kv, 2 * L::kTileKV);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == kMmaWarp) {
       // ---------------------------------------------------------- MMA issuer
-      if (lane == 0) {
+      if (elect_one()) {
         // Shared-memory descriptors are built once: a K step or a stage only adds a constant to
         // the 14-bit start-address field (every address here is below 256 KB, so it never
         // carries). Per-MMA descriptor arithmetic would otherwise cost the single issuing thread
@@ -819,15 +820,54 @@ __global__ void __launch_bounds__(256) fmha_bwd_prep_kernel(const RowParams p) {
   }
 }
 
-// ------------------------------------------------------------------ convert: dq = scale * accumulator
-// One CTA per 64-query block: 256 threads, each converting 8-element chunks of rows.
+// ------------------------------------------------------------------ sinks: dk, dv = sum of a tile's parts
+// Block x of a kv head adds 1024 elements of dk or dv of one sink tile: four a thread, pieces in order.
+template <int D>
+constexpr int kJoinBlocks = 2 * kBN * D / 1024;  // of a sink tile
 template <typename T, int D, bool VARLEN>
-__global__ void __launch_bounds__(256) fmha_bwd_dq_kernel(const RowParams p) {
+__device__ __forceinline__ void join_parts(const Params& p, int bh, int x) {
+  const int hk = bh % p.hkv, zb = bh / p.hkv;
+  const int tile = x / kJoinBlocks<D>, which = (x / (kJoinBlocks<D> / 2)) & 1;
+  const int i = x % (kJoinBlocks<D> / 2) * 256 + (int)threadIdx.x;
+  int row_k0 = 0, len_k = p.sk;
+  if constexpr (VARLEN) varlen_rows(p.cu_k, zb, p.total_k, row_k0, len_k);
+  const int r = tile * kBN + i / (D / 4), c = i % (D / 4);
+  if (r >= len_k) return;
+  const float4* src = reinterpret_cast<const float4*>(
+      p.parts + ((int64_t)bh * p.sink_tiles + tile) * p.pieces * (2 * kBN * D) + which * (kBN * D)) + i;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int e = 0; e < p.pieces; ++e) {
+    const float4 x4 = src[(int64_t)e * (2 * kBN * D / 4)];
+    a.x += x4.x;
+    a.y += x4.y;
+    a.z += x4.z;
+    a.w += x4.w;
+  }
+  const int64_t ss = which ? p.dv_ss : p.dk_ss;
+  T* dst = reinterpret_cast<T*>(which ? p.dv : p.dk) + (int64_t)hk * (which ? p.dv_sh : p.dk_sh) +
+           (VARLEN ? (int64_t)row_k0 * ss : (int64_t)zb * (which ? p.dv_sz : p.dk_sz));
+  *reinterpret_cast<uint2*>(dst + (int64_t)r * ss + c * 4) =
+      make_uint2(Cvt<T>::pack(a.x, a.y), Cvt<T>::pack(a.z, a.w));
+}
+
+// ------------------------------------------------------------------ convert: dq = scale * accumulator
+// One CTA per 64-query block: 256 threads, each converting 8-element chunks of rows. With JOIN the first
+// p.join blocks of a kv head's first query head join the sinks' parts instead.
+template <typename T, int D, bool VARLEN, bool JOIN>
+__global__ void __launch_bounds__(256) fmha_bwd_dq_kernel(const RowParams p, const Params m) {
   const int bh = (int)blockIdx.y + (int)blockIdx.z * (int)gridDim.y;
   if (bh >= p.zh) return;
   const int h = bh % p.hq;
   const int zb = bh / p.hq;
-  const int jb = blockIdx.x;
+  int jb = blockIdx.x;
+  if constexpr (JOIN) {
+    if (jb < p.join) {
+      if (h % m.group == 0) join_parts<T, D, VARLEN>(m, bh / m.group, jb);
+      return;
+    }
+    jb -= p.join;
+  }
   int row_q0 = 0, len_q = p.sq;
   int64_t base = 0;
   if constexpr (VARLEN) {
@@ -853,36 +893,6 @@ __global__ void __launch_bounds__(256) fmha_bwd_dq_kernel(const RowParams p) {
     *reinterpret_cast<uint4*>(dst + c * 8) =
         make_uint4(Cvt<T>::pack(a.x * s, a.y * s), Cvt<T>::pack(a.z * s, a.w * s), Cvt<T>::pack(b.x * s, b.y * s),
                    Cvt<T>::pack(b.z * s, b.w * s));
-  }
-}
-
-// ------------------------------------------------------------------ sinks: dk, dv = sum of a tile's parts
-// One CTA per (sink tile, dk or dv) of one kv head; each thread adds four elements of the pieces in order.
-template <typename T, int D, bool VARLEN>
-__global__ void __launch_bounds__(256) fmha_bwd_sinks_kernel(const Params p) {
-  const int bh = (int)blockIdx.y + (int)blockIdx.z * (int)gridDim.y;
-  if (bh >= p.zh_kv) return;
-  const int hk = bh % p.hkv, zb = bh / p.hkv;
-  const int tile = (int)blockIdx.x >> 1, which = (int)blockIdx.x & 1;
-  int row_k0 = 0, len_k = p.sk;
-  if constexpr (VARLEN) varlen_rows(p.cu_k, zb, p.total_k, row_k0, len_k);
-  const float* src = p.parts + ((int64_t)bh * p.sink_tiles + tile) * p.pieces * (2 * kBN * D) + which * (kBN * D);
-  const int64_t ss = which ? p.dv_ss : p.dk_ss;
-  T* dst = reinterpret_cast<T*>(which ? p.dv : p.dk) + (int64_t)hk * (which ? p.dv_sh : p.dk_sh) +
-           (VARLEN ? (int64_t)row_k0 * ss : (int64_t)zb * (which ? p.dv_sz : p.dk_sz));
-  for (int i = threadIdx.x; i < kBN * D / 4; i += 256) {
-    const int r = i / (D / 4), c = i % (D / 4);
-    if (tile * kBN + r >= len_k) break;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int e = 0; e < p.pieces; ++e) {
-      const float4 x = reinterpret_cast<const float4*>(src + (int64_t)e * (2 * kBN * D))[i];
-      a.x += x.x;
-      a.y += x.y;
-      a.z += x.z;
-      a.w += x.w;
-    }
-    *reinterpret_cast<uint2*>(dst + (int64_t)(tile * kBN + r) * ss + c * 4) =
-        make_uint2(Cvt<T>::pack(a.x, a.y), Cvt<T>::pack(a.z, a.w));
   }
 }
 
@@ -957,14 +967,15 @@ int run_all(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
              : mode == kWindow ? launch_main<T, D, VARLEN, kWindow>(tq, tk, tv, tdo, p, g, s)
                                : launch_main<T, D, VARLEN, kExtra>(tq, tk, tv, tdo, p, g, s);
     if (rc) return rc;
-    if (p.sink_tiles > 0 && p.pieces > 1) {
-      fmha_bwd_sinks_kernel<T, D, VARLEN><<<grid_of(2 * p.sink_tiles, p.zh_kv), 256, 0, s>>>(p);
-      rc = host::cuda_check(cudaGetLastError(), "fmha bwd sinks launch");
-      if (rc) return rc;
-    }
   }
   if (q_blocks > 0) {
-    fmha_bwd_dq_kernel<T, D, VARLEN><<<rgrid, 256, 0, s>>>(rp);
+    if (p.sink_tiles > 0 && p.pieces > 1) {  // pieces > 1 only where there are queries and key tiles
+      RowParams jp = rp;
+      jp.join = p.sink_tiles * kJoinBlocks<D>;
+      fmha_bwd_dq_kernel<T, D, VARLEN, true><<<grid_of(q_blocks + jp.join, rp.zh), 256, 0, s>>>(jp, p);
+    } else {
+      fmha_bwd_dq_kernel<T, D, VARLEN, false><<<rgrid, 256, 0, s>>>(rp, p);
+    }
     return host::cuda_check(cudaGetLastError(), "fmha bwd dq launch");
   }
   return GKO_OK;

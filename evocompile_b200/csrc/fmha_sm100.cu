@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(Shape<MODE>::kThreads, Shape<MODE>::kCtas)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meta + 160);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(meta + 164);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);  // uniform, and known to be
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(Shape<MODE>::kThreads, Shape<MODE>::kCtas)
   setmaxnreg_dec<C::kRegsControl>();
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && n_tiles > 0) {
+    if (n_tiles > 0 && elect_one()) {
       mbar_arrive_expect_tx(bar_q, kQTiles * L::kTile);
 #pragma unroll
       for (int t = 0; t < kQTiles; ++t)
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(Shape<MODE>::kThreads, Shape<MODE>::kCtas)
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0 && n_tiles > 0) {
+    if (n_tiles > 0 && elect_one()) {
       bool ok = wait_bounded(bar_q, 0, abort_flag, p.status, kStatusTimeoutMma);
       auto few = [&](int t, int j) { return MODE == kWindow && few_t[t] && j < sk_t[t]; };
       auto issue_s = [&](int t, int u) {
