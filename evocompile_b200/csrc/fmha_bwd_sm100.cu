@@ -22,36 +22,40 @@
 // minus one vector per kv head, about their mean: each row of dS sums to zero, so the product is the same, but
 // the roundings of dS and of delta, which do not, no longer meet the keys' common part (keys whose channels have
 // means of 1.5 deviations: relative error of dq 0.0050 to 0.0029 in bf16).
-// 4096 tokens, 32 / 8 heads of 128, window 512, 4 sinks: 223 us at the main loop's rate, about 2.3 us for each of a
-// CTA's 44 steps; the sinks' pieces are 48 of its 296 CTAs.
+// 4096 tokens, 32 / 8 heads of 128, window 512, 4 sinks: 173 us, of which the main kernel takes about 140, some 1.4 us
+// for each of a CTA's 40 to 44 steps (the tensor pipe is busy for 45 % of them); the sinks' pieces are 48 of its
+// 296 CTAs. Causal without a window: 466 us.
 //
-// The main kernel is laid out around two costs of B200: shared-memory bandwidth
-// (about 128 B per clock per SM, which limits MMAs that read both operands from shared
-// memory at N <= 64) and the latency of a hand-off between warps through an mbarrier
-// (a few hundred cycles, more after a tcgen05.commit). K is copied once into TMEM and is
+// The main kernel is laid out around the costs of B200 that its steps meet: shared-memory bandwidth
+// (about 128 B per clock per SM, which limits MMAs that read both operands from shared memory at N <= 64), the
+// latency of a hand-off between warps through an mbarrier (a few hundred cycles, more after a tcgen05.commit),
+// and the queue that shared and global accesses of an SM share. K is copied once into TMEM and is
 // the A operand (TS form) of S^T = K Q^T; dV and dK take P^T / dS^T from TMEM; dQ^T has
 // its own TMEM buffer, so the MMA for the next step's dP^T never waits for dQ^T to be
-// drained, and the dS^T smem tile is double buffered. dQ^T leaves TMEM through registers
-// as fp32 reductions into L2 (no shared-memory staging).
+// drained, and the dS^T smem tile is double buffered. dQ^T leaves TMEM through registers into a tile in shared
+// memory, [queries][D] in f32, whose halves the copy engine adds to the accumulator in L2 (64 reductions
+// of each drain thread instead filled the queue in which the compute warps' loads and stores wait:
+// 183 us against 173). One elected thread issues the MMAs; were it chosen as lane 0, each issue would cost
+// some 80 cycles, and a step's 36 of them more than anything else in it (606 us against 528, causal).
 // TMEM columns: K [0, 64)  dQ^T [64, 128)  dV [128, 256)  dK [256, 384)
 //               S^T|P^T [384, 448)  dP^T|dS^T [448, 512)
-//   warp 13    MMA issuer. Step j, in issue order:
+// Warps, with 16 (kPlain, kWindow) or 8 (kExtra, whose mask and softcap need the registers) for compute:
+//   compute    warp w owns key rows 32 (w & 3) .. +31 (its TMEM lane quarter) and 16 or 32 of the step's 64
+//              query columns: first K into TMEM (64 channels of the rows a warp); then per step
+//              P^T = 2^(s * scale * log2 e - lse * log2 e) over S^T (bf16/f16 pairs) and
+//              dS^T = P^T (dP^T - delta) over dP^T and into smem dS tile j & 1.
+//              At the end dk = scale * dK (32 columns at a time).
+//   drain (4)  one head-dim row of dQ^T_j per thread into the shared-memory tile; at the end dv = dV.
+//   producer   K, V once by TMA; Q_j, dO_j, -lse_j, -delta_j per step (3 stages).
+//   MMA        Step j, in issue order:
 //                dV += P^T_j dO_j        (A = P^T in TMEM, B = dO_j MN-major)
 //                S^T_{j+1} = K Q_{j+1}^T (A = K in TMEM) — the S columns are free once dV_j is issued
 //                dK += dS^T_j Q_j        (A = dS^T in TMEM)
 //                dP^T_{j+1} = V dO_{j+1}^T (both from smem) — the dP columns are free once dK_j is issued
-//                dQ^T_j = K^T dS^T_j     (both from smem, MN-major) once warps 8-11 have read dQ^T_{j-1}
-//   warp 12    TMA producer: K, V once; Q_j, dO_j, -lse_j, -delta_j per step (3 stages).
-//   warps 0-7  compute: warp w owns key rows 32 (w & 3) .. +31 (its TMEM lane quarter) and
-//              query columns 32 (w >> 2) .. +31: first K (w < 4) into TMEM; then per step
-//              P^T = 2^(s * scale * log2 e - lse * log2 e) over S^T (bf16/f16 pairs) and
-//              dS^T = P^T (dP^T - delta) over dP^T and into smem dS tile j & 1.
-//              At the end dk = scale * dK (half the columns each).
-//   warps 8-11 one head-dim row of dQ^T_j per thread: 64 fp32 reductions (red.global.add)
-//              into the row-major [queries][D] accumulator; at the end dv = dV.
-// Registers: 16 warps x 128 at launch; the compute warpgroups rise to 152, the drain
-// warpgroup drops to 112 and the producer/MMA warpgroup to 96
-// (128 x (2 x 152 + 112 + 96) = 65536 = 512 x 128).
+//                dQ^T_j = K^T dS^T_j     (both from smem, MN-major) once the drain warps have read dQ^T_{j-1}
+//   reduce     adds the halves of the dQ tile to the row-major [queries][D] accumulator.
+// 16 compute warps rather than 8 gain 1 to 2 %, two S^T buffers (K read from shared memory instead) nothing.
+// Registers: counted against the launch's in `Warps`.
 #include <mutex>
 #include <type_traits>
 
@@ -63,15 +67,7 @@ namespace fmha_bwd {
 
 constexpr int kBN = 128;  // keys per CTA (one per TMEM lane)
 constexpr int kBM = 64;   // queries per step
-constexpr int kThreads = 512;
-constexpr int kDrainWarp0 = 8;
-constexpr int kProducerWarp = 12;
-constexpr int kMmaWarp = 13;
 constexpr int kStages = 3;
-constexpr uint32_t kRegsCompute = 152;
-constexpr uint32_t kRegsDrain = 112;
-constexpr uint32_t kRegsControl = 96;
-static_assert(128 * (2 * kRegsCompute + kRegsDrain + kRegsControl) <= 512 * 128, "register split exceeds the launch");
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmK = 0, kTmDQ = 64, kTmDV = 128, kTmDK = 256, kTmS = 384, kTmDP = 448;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -159,6 +155,11 @@ __device__ __forceinline__ float bias_at(const Params& p, int z, int h, int q, i
   return __half2float(__ldg(reinterpret_cast<const __half*>(p.bias) + off));
 }
 
+__device__ __forceinline__ void tmem_ldc(uint32_t at, uint32_t (&r)[32]) { tmem_ld32(at, r); }
+__device__ __forceinline__ void tmem_ldc(uint32_t at, uint32_t (&r)[16]) { tmem_ld16(at, r); }
+__device__ __forceinline__ void tmem_stc(uint32_t at, const uint32_t (&r)[16]) { tmem_st16(at, r); }
+__device__ __forceinline__ void tmem_stc(uint32_t at, const uint32_t (&r)[8]) { tmem_st8(at, r); }
+
 template <int D>
 struct Layout {
   static constexpr uint32_t kChunkKV = 128 * 128;  // [128 rows][128 B]
@@ -171,7 +172,9 @@ struct Layout {
   static constexpr uint32_t kStageBytes = 2 * kTileQ;
   static constexpr uint32_t kDS = kStage0 + kStages * kStageBytes;  // 2 x [128 keys][64 q] bf16, SW128
   static constexpr uint32_t kDSBytes = kBN * 128;
-  static constexpr uint32_t kRow = kDS + 2 * kDSBytes;  // per stage: -lse log2 e [64], -delta [64]
+  static constexpr uint32_t kOut = kDS + 2 * kDSBytes;  // dQ of a step, [64 q][D] f32, on its way to the accumulator
+  static constexpr uint32_t kOutHalf = 32 * D * 4;
+  static constexpr uint32_t kRow = kOut + 2 * kOutHalf;  // per stage: -lse log2 e [64], -delta [64]
   static constexpr uint32_t kMeta = kRow + kStages * 512;
   static constexpr uint32_t kBytes = (1024 + kMeta + 256) > 122880 ? (1024 + kMeta + 256) : 122880;
   static_assert(kDS % 1024 == 0 && kStageBytes % 1024 == 0, "swizzled tiles need 1024-byte alignment");
@@ -183,12 +186,33 @@ struct Layout {
 // interval, so the mask is two bounds per key row.
 enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
 
+// Warps of the main kernel. Compute warps come in groups of four, which share the 64 queries of a step by
+// columns; registers are counted against the launch's.
+template <int MODE>
+struct Warps {
+  static constexpr int kGroups = MODE == kExtra ? 2 : 4;
+  static constexpr int kCols = kBM / kGroups;
+  static constexpr int kDrain0 = 4 * kGroups;
+  static constexpr int kProducer = kDrain0 + 4;
+  static constexpr int kMma = kDrain0 + 5;
+  static constexpr int kReduce = kDrain0 + 6;
+  static constexpr int kThreads = 32 * (kDrain0 + 8);
+  static constexpr uint32_t kLaunch = MODE == kExtra ? 128 : 80;
+  static constexpr uint32_t kCompute = MODE == kExtra ? 152 : 80;
+  static constexpr uint32_t kDrain = MODE == kExtra ? 112 : 96;
+  static constexpr uint32_t kControl = MODE == kExtra ? 96 : 64;
+  static_assert(128 * (kGroups * kCompute + kDrain + kControl) <= kThreads * kLaunch, "register split exceeds the launch");
+  static_assert(kThreads * kLaunch <= 65536, "registers of an SM");
+};
+
 template <typename T, int D, bool VARLEN, int MODE>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
     fmha_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                     const Params p) {
   using L = Layout<D>;
+  using W = Warps<MODE>;
+  constexpr int kC = W::kCols;
   constexpr bool EXTRA = MODE == kExtra;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescS = make_idesc_f16(kBF16, kBN, kBM, false, false);  // S^T, dP^T
@@ -262,11 +286,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (n_steps == 0) {  // no query sees these keys: dk = dv = 0
     if (MODE != kPlain && part) {
-      for (int i = threadIdx.x; i < 2 * kBN * D / 4; i += kThreads)
+      for (int i = threadIdx.x; i < 2 * kBN * D / 4; i += W::kThreads)
         reinterpret_cast<float4*>(part)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       return;
     }
-    for (int i = threadIdx.x; i < kBN * (D / 8); i += kThreads) {
+    for (int i = threadIdx.x; i < kBN * (D / 8); i += W::kThreads) {
       const int r = i / (D / 8), c = i % (D / 8);
       if (n0 + r < len_k) {
         reinterpret_cast<uint4*>(dk_base + (int64_t)(n0 + r) * p.dk_ss)[c] = make_uint4(0, 0, 0, 0);
@@ -284,36 +308,42 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sgen = smem_raw + pad;  // generic pointer to the same base
   const uint32_t smeta = sb + L::kMeta;
   const uint32_t bar_kv = smeta;            // K, V landed in smem (TMA)
-  const uint32_t bar_kvtm = smeta + 8;      // K copied into TMEM (4 arrivals)
+  const uint32_t bar_kvtm = smeta + 8;      // K copied into TMEM
   const uint32_t bar_full = smeta + 16;     // [3]
   const uint32_t bar_empty = smeta + 40;    // [3]
   const uint32_t bar_sfull = smeta + 64;
-  const uint32_t bar_pfull = smeta + 72;    // 8 arrivals
+  const uint32_t bar_pfull = smeta + 72;    // an arrival of each compute warp
   const uint32_t bar_dpfull = smeta + 80;
-  const uint32_t bar_dsfull = smeta + 88;   // 8 arrivals
+  const uint32_t bar_dsfull = smeta + 88;   // an arrival of each compute warp
   const uint32_t bar_dqfull = smeta + 96;
   const uint32_t bar_dqempty = smeta + 104;  // 4 arrivals
   const uint32_t bar_dsfree = smeta + 112;   // [2] per smem dS tile: dQ^T has read it
   const uint32_t bar_final = smeta + 128;
   const uint32_t bar_drain = smeta + 136;
+  const uint32_t bar_outfull = smeta + 152;  // [2] per half of the dQ tile: written, 4 arrivals
+  const uint32_t bar_outfree = smeta + 168;  // [2] read by the copy engine
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + L::kMeta + 144);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + L::kMeta + 148);
 
   if (threadIdx.x == 0) {
     mbar_init(bar_kv, 1);
-    mbar_init(bar_kvtm, 4);
+    mbar_init(bar_kvtm, 4 * (D / 64));
     for (int i = 0; i < kStages; ++i) {
       mbar_init(bar_full + 8 * i, 1);
       mbar_init(bar_empty + 8 * i, 1);
     }
     mbar_init(bar_sfull, 1);
-    mbar_init(bar_pfull, 8);
+    mbar_init(bar_pfull, W::kDrain0);
     mbar_init(bar_dpfull, 1);
-    mbar_init(bar_dsfull, 8);
+    mbar_init(bar_dsfull, W::kDrain0);
     mbar_init(bar_dqfull, 1);
     mbar_init(bar_dqempty, 4);
     mbar_init(bar_dsfree, 1);
     mbar_init(bar_dsfree + 8, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_outfull + 8 * i, 4);
+      mbar_init(bar_outfree + 8 * i, 1);
+    }
     mbar_init(bar_final, 1);
     mbar_init(bar_drain, 1);
     *abort_flag = 0;
@@ -323,7 +353,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tm_v);
     prefetch_tmap(&tm_do);
   }
-  if (warp == kMmaWarp) {
+  // kWindow: the centre, in the dQ tile, which is first written when all compute warps have had it
+  float* centre_s = reinterpret_cast<float*>(sgen + L::kOut);
+  if constexpr (MODE == kWindow)
+    if (threadIdx.x < D) centre_s[threadIdx.x] = p.centre[(int64_t)bh * D + threadIdx.x];
+  if (warp == W::kMma) {
     tmem_alloc(smem_u32(tmem_slot), kTmemCols);
     tmem_relinquish();
   }
@@ -332,9 +366,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp >= kProducerWarp) {
-    setmaxnreg_dec<kRegsControl>();
-    if (warp == kProducerWarp) {
+  if (warp >= W::kProducer) {
+    setmaxnreg_dec<W::kControl>();
+    if (warp == W::kProducer) {
       // ---------------------------------------------------------- TMA producer
       if (elect_one()) {
         mbar_arrive_expect_tx(bar_kv, 2 * L::kTileKV);
@@ -343,11 +377,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_4d(sb + L::kK + c * L::kChunkKV, &tm_k, bar_kv, c * 64, row_k0 + n0, hk, zc);
           tma_load_4d(sb + L::kV + c * L::kChunkKV, &tm_v, bar_kv, c * 64, row_k0 + n0, hk, zc);
         }
+        int jq = 0, hh = 0;
         for (int j = 0; j < n_steps; ++j) {
           const int st = j % kStages;
           const uint32_t ph = (j / kStages) & 1;
-          const int hh = j / nq;
-          const int jb = jb_lo + j % nq;
+          const int jb = jb_lo + jq;
           if (!wait_bounded(bar_empty + 8 * st, ph ^ 1, abort_flag, p.status, kStatusTimeoutProducer)) break;
           const uint32_t stage = sb + L::kStage0 + st * L::kStageBytes;
           const uint32_t full = bar_full + 8 * st;
@@ -361,9 +395,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t t = tile_of(hh, jb);
           bulk_load(sb + L::kRow + st * 512, p.nl + t * kBM, kBM * 4, full);
           bulk_load(sb + L::kRow + st * 512 + 256, p.nd + t * kBM, kBM * 4, full);
+          if (++jq == nq) {
+            jq = 0;
+            ++hh;
+          }
         }
       }
-    } else if (warp == kMmaWarp) {
+    } else if (warp == W::kMma) {
       // ---------------------------------------------------------- MMA issuer
       if (elect_one()) {
         // Shared-memory descriptors are built once: a K step or a stage only adds a constant to
@@ -407,14 +445,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t st_mn = d_qmn + (uint64_t)((j % kStages) * kStageU);  // Q_j (MN-major); dO_j at + kTileQU
           const uint32_t ph = j & 1;
           const uint32_t acc0 = j > 0 ? 1u : 0u;
-          // P^T and dS^T are packed: the 16 columns of query group g sit at + 32 g
+          // P^T and dS^T are packed: the kC / 2 columns of query group g sit at + kC g
+          auto packed = [](int kk) -> uint32_t { return kk * 16 / kC * kC + kk * 16 % kC / 2; };
           // dV += P^T_j dO_j: B = dO_j as [q][d] (MN-major), 16 rows (2048 bytes) per K step
           ok = wait_bounded(bar_pfull, ph, abort_flag, p.status, kStatusTimeoutMma);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < kBM / 16; ++kk)
-            mma_f16_ts(t_dv, t_s + (kk >> 1) * 32 + (kk & 1) * 8, st_mn + kTileQU + kk * 128, kIdescKV,
+            mma_f16_ts(t_dv, t_s + packed(kk), st_mn + kTileQU + kk * 128, kIdescKV,
                        kk > 0 ? 1u : acc0);
           const bool next = j + 1 < n_steps;
           if (next) {
@@ -430,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < kBM / 16; ++kk)
-            mma_f16_ts(t_dk, t_dp + (kk >> 1) * 32 + (kk & 1) * 8, st_mn + kk * 128, kIdescKV, kk > 0 ? 1u : acc0);
+            mma_f16_ts(t_dk, t_dp + packed(kk), st_mn + kk * 128, kIdescKV, kk > 0 ? 1u : acc0);
           mma_commit(bar_empty + 8 * (j % kStages));  // Q_j, dO_j, -lse_j, -delta_j no longer needed
           if (next) issue_dp(j + 1);                  // after dK_j in issue order, so dS^T_j has been read
           // dQ^T_j = K^T dS^T_j: A = K as [key][d] (MN-major over d; for D = 64 the second 64-row
@@ -453,53 +492,69 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait_for(bar_drain, 0, p.status, kStatusTimeoutDrain);
         }
       }
+    } else if (warp == W::kReduce) {
+      // ---------------------------------------------------------- dQ tile halves added to the accumulator
+      if (elect_one()) {
+        int jq = 0, hh = 0;
+        for (int j = 0, ok = 1; j < n_steps && ok; ++j) {
+          float* dst = p.dq_acc + tile_of(hh, jb_lo + jq) * (kBM * D);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!wait_bounded(bar_outfull + 8 * h, j & 1, abort_flag, p.status, kStatusTimeoutEpilogue)) {
+              ok = 0;
+              break;
+            }
+            bulk_reduce_add(dst + h * (32 * D), sb + L::kOut + h * L::kOutHalf, L::kOutHalf);
+            bulk_commit_group();
+            bulk_wait_group_read<1>();  // the half before has been read
+            if (j + h > 0) mbar_arrive(bar_outfree + 8 * (h ^ 1));
+          }
+          if (++jq == nq) {
+            jq = 0;
+            ++hh;
+          }
+        }
+        bulk_wait_group<0>();
+      }
     }
-  } else if (warp < kDrainWarp0) {
-    setmaxnreg_inc<kRegsCompute>();
-    // ------------------------------------------------------------ compute (key row x 32 query columns)
+  } else if (warp < W::kDrain0) {
+    if constexpr (W::kCompute > W::kLaunch) setmaxnreg_inc<W::kCompute>();
+    // ------------------------------------------------------------ compute (key row x kC query columns)
     const int quarter = warp & 3;
-    const int cg = warp >> 2;  // query columns 32 cg .. 32 cg + 31; warps of cg 0 copy K into TMEM
+    const int cg = warp >> 2;  // query columns kC cg ..; also copies 64 columns of K into TMEM
     const int r = quarter * 32 + lane;
     const int kj = n0 + r;
     const bool row_valid = kj < len_k;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tm_row = tmem_base + lane_off;
     const uint64_t k2 = f2pack(p.scale_log2, p.scale_log2);
-    bool ok = cg ? true : wait_bounded(bar_kv, 0, abort_flag, p.status, kStatusTimeoutSoftmax);
-    if (ok && cg == 0) {
+    bool ok = cg >= D / 64 ? true : wait_bounded(bar_kv, 0, abort_flag, p.status, kStatusTimeoutSoftmax);
+    if (ok && cg < D / 64) {
       // row r of K from the swizzled smem tile into TMEM as bf16/f16 pairs along d
-      const uint8_t* src = sgen + L::kK + r * 128;
+      uint8_t* src = sgen + L::kK + r * 128 + cg * L::kChunkKV;
+      uint32_t w[32];
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 x = *reinterpret_cast<const uint4*>(src + c * L::kChunkKV + ((i ^ (r & 7)) << 4));
-          w[4 * i] = x.x;
-          w[4 * i + 1] = x.y;
-          w[4 * i + 2] = x.z;
-          w[4 * i + 3] = x.w;
-        }
-        tmem_st32(tm_row + kTmK + c * 32, w);
+      for (int i = 0; i < 8; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src + ((i ^ (r & 7)) << 4));
+        w[4 * i] = x.x;
+        w[4 * i + 1] = x.y;
+        w[4 * i + 2] = x.z;
+        w[4 * i + 3] = x.w;
       }
+      tmem_st32(tm_row + kTmK + cg * 32, w);
       if constexpr (MODE == kWindow) {
         // from here on the shared-memory tile serves dq alone: the same row minus the centre
-        const float4* centre = reinterpret_cast<const float4*>(p.centre + (int64_t)bh * D);
+        const float4* centre = reinterpret_cast<const float4*>(centre_s) + cg * 16;
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
+        for (int i = 0; i < 8; ++i) {
+          const float4 m0 = centre[i * 2], m1 = centre[i * 2 + 1];
+          float a[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint4* at = reinterpret_cast<uint4*>(sgen + L::kK + r * 128 + c * L::kChunkKV + ((i ^ (r & 7)) << 4));
-            const uint4 x = *at;
-            const float4 m0 = __ldg(centre + c * 16 + i * 2), m1 = __ldg(centre + c * 16 + i * 2 + 1);
-            float a[8];
-            Cvt<T>::unpack(x.x, a[0], a[1]);
-            Cvt<T>::unpack(x.y, a[2], a[3]);
-            Cvt<T>::unpack(x.z, a[4], a[5]);
-            Cvt<T>::unpack(x.w, a[6], a[7]);
-            *at = make_uint4(Cvt<T>::pack(a[0] - m0.x, a[1] - m0.y), Cvt<T>::pack(a[2] - m0.z, a[3] - m0.w),
-                             Cvt<T>::pack(a[4] - m1.x, a[5] - m1.y), Cvt<T>::pack(a[6] - m1.z, a[7] - m1.w));
-          }
+          for (int e = 0; e < 4; ++e) Cvt<T>::unpack(w[4 * i + e], a[2 * e], a[2 * e + 1]);
+          *reinterpret_cast<uint4*>(src + ((i ^ (r & 7)) << 4)) =
+              make_uint4(Cvt<T>::pack(a[0] - m0.x, a[1] - m0.y), Cvt<T>::pack(a[2] - m0.z, a[3] - m0.w),
+                         Cvt<T>::pack(a[4] - m1.x, a[5] - m1.y), Cvt<T>::pack(a[6] - m1.z, a[7] - m1.w));
+        }
         fence_proxy_async_smem();
       }
       tmem_wait_st();
@@ -507,35 +562,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_kvtm);
     }
+    // counted along, as divisions would sit in the chain of every step: the stage with its phase, the query
+    // block within the head, the head
+    int st = 0, jq = 0, hh = 0;
+    uint32_t st_ph = 0;
     for (int j = 0; j < n_steps && ok; ++j) {
       const uint32_t ph = j & 1;
-      const int jb = jb_lo + j % nq;
-      const int hh = j / nq;
-      const int q0 = jb * kBM + cg * 32;  // first query of this warp's columns
-      const float2* nl2 = reinterpret_cast<const float2*>(sgen + L::kRow + (j % kStages) * 512) + cg * 16;
-      const float2* nd2 = reinterpret_cast<const float2*>(sgen + L::kRow + (j % kStages) * 512 + 256) + cg * 16;
+      const int q0 = (jb_lo + jq) * kBM + cg * kC;  // first query of this warp's columns
+      const float2* nl2 = reinterpret_cast<const float2*>(sgen + L::kRow + st * 512) + cg * (kC / 2);
+      const float2* nd2 = reinterpret_cast<const float2*>(sgen + L::kRow + st * 512 + 256) + cg * (kC / 2);
       // the stage's -lse / -delta rows were written by the bulk copy: observe its barrier
       // here too (it completed before S^T_j; the stage is refilled only after dS_j)
       if (!wait_bounded(bar_sfull, ph, abort_flag, p.status, kStatusTimeoutSoftmax) ||
-          !wait_bounded(bar_full + 8 * (j % kStages), (j / kStages) & 1, abort_flag, p.status,
-                        kStatusTimeoutSoftmax)) {
+          !wait_bounded(bar_full + 8 * st, st_ph, abort_flag, p.status, kStatusTimeoutSoftmax)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      float pv[32];  // S^T row, then P^T row
+      float pv[kC];  // S^T row, then P^T row
       {
-        uint32_t su[32];
-        tmem_ld32p(tm_row + kTmS + cg * 32, su);
+        uint32_t su[kC];
+        tmem_ldc(tm_row + kTmS + cg * kC, su);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 32; ++c) pv[c] = __uint_as_float(su[c]);
+        for (int c = 0; c < kC; ++c) pv[c] = __uint_as_float(su[c]);
       }
-      float gsc[EXTRA ? 32 : 1];  // softcap derivative
+      float gsc[EXTRA ? kC : 1];  // softcap derivative
       if constexpr (EXTRA) {
         const int h = hk * p.group + hh;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
+        for (int c = 0; c < kC; ++c) {
           const int qi = q0 + c;
           float x = pv[c] * p.scale;
           if (p.bias_mode != GKO_BIAS_NONE && row_valid && qi < len_q) x += bias_at(p, zb, h, qi, kj);
@@ -555,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
+        for (int c = 0; c < kC; c += 2) {
           const float2 nlp = nl2[c >> 1];
           float a, bb;
           f2unpack(fma2(f2pack(pv[c], pv[c + 1]), k2, f2pack(nlp.x, nlp.y)), a, bb);
@@ -565,24 +621,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (MODE == kWindow) {
           // queries [first, last] see this key: all of them a sink, else those within the window
           const int first = max(p.causal ? kj : 0, kj < p.sinks ? 0 : kj - p.window) - q0;
-          const int last = !row_valid ? -1 : (kj < p.sinks ? 31 : kj + p.window - q0);
-          if (first > 0 || last < 31) {
+          const int last = !row_valid ? -1 : (kj < p.sinks ? kC - 1 : kj + p.window - q0);
+          if (first > 0 || last < kC - 1) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) pv[c] = (c >= first && c <= last) ? pv[c] : 0.f;
+            for (int c = 0; c < kC; ++c) pv[c] = (c >= first && c <= last) ? pv[c] : 0.f;
           }
         }
         // keys past the end, and (causal) queries before the key, get P = 0
-        const int lim = MODE == kWindow ? 0 : row_valid ? (p.causal ? kj - q0 : 0) : 32;
+        const int lim = MODE == kWindow ? 0 : row_valid ? (p.causal ? kj - q0 : 0) : kC;
         if (lim > 0) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) pv[c] = (c < lim) ? 0.f : pv[c];
+          for (int c = 0; c < kC; ++c) pv[c] = (c < lim) ? 0.f : pv[c];
         }
       }
       {
-        uint32_t pk[16];
+        uint32_t pk[kC / 2];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) pk[c] = Cvt<T>::pack(pv[2 * c], pv[2 * c + 1]);
-        tmem_st16(tm_row + kTmS + cg * 32, pk);
+        for (int c = 0; c < kC / 2; ++c) pk[c] = Cvt<T>::pack(pv[2 * c], pv[2 * c + 1]);
+        tmem_stc(tm_row + kTmS + cg * kC, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -594,12 +650,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
-      uint32_t dsu[32];
-      tmem_ld32p(tm_row + kTmDP + cg * 32, dsu);
+      uint32_t dsu[kC];
+      tmem_ldc(tm_row + kTmDP + cg * kC, dsu);
       tmem_wait_ld();
-      uint32_t pk[16];
+      uint32_t pk[kC / 2];
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
+      for (int c = 0; c < kC; c += 2) {
         const float2 ndp = nd2[c >> 1];
         const uint64_t t = add2(f2pack(__uint_as_float(dsu[c]), __uint_as_float(dsu[c + 1])), f2pack(ndp.x, ndp.y));
         float a, bb;
@@ -610,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         pk[c >> 1] = Cvt<T>::pack(a, bb);
       }
-      tmem_st16(tm_row + kTmDP + cg * 32, pk);
+      tmem_stc(tm_row + kTmDP + cg * kC, pk);
       // dS^T row r into smem tile j & 1 ([128 keys][64 q], 16-byte chunk i at (i ^ (r & 7))),
       // once dQ^T_{j-2} has finished reading that tile
       if (j >= 2 &&
@@ -620,8 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const uint32_t ds_row = sb + L::kDS + (j & 1) * L::kDSBytes + r * 128;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ci = cg * 4 + i;
+      for (int i = 0; i < kC / 8; ++i) {
+        const int ci = cg * (kC / 8) + i;
         st_shared_v4(ds_row + ((ci ^ (r & 7)) << 4), pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
       }
       fence_proxy_async_smem();
@@ -629,15 +685,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_dsfull);
+      if (++st == kStages) {
+        st = 0;
+        st_ph ^= 1;
+      }
+      if (++jq == nq) {
+        jq = 0;
+        ++hh;
+      }
     }
-    // ------------------------------------------------------------ dk = scale * dK (columns cg * D/2 ..)
+    // ------------------------------------------------------------ dk = scale * dK (32 columns at a time)
     if (ok) ok = wait_bounded(bar_final, 0, abort_flag, p.status, kStatusTimeoutSoftmax);
     if (ok) {
       tc_fence_after();
       T* row = dk_base + (int64_t)kj * p.dk_ss;
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const int col = cg * (D / 2) + c * 32;
+      for (int c = 0; c < D; c += 32 * W::kGroups) {
+        const int col = c + cg * 32;
+        if (col >= D) break;
         uint32_t v[32];
         tmem_ld32(tm_row + kTmDK + col, v);
         tmem_wait_ld();
@@ -664,14 +729,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
   } else {
-    setmaxnreg_dec<kRegsDrain>();
+    if constexpr (W::kDrain > W::kLaunch) setmaxnreg_inc<W::kDrain>();
+    else setmaxnreg_dec<W::kDrain>();
     // ------------------------------------------------------------ dQ^T drain (one head-dim row per thread)
-    const int wq = warp - kDrainWarp0;
+    const int wq = warp - W::kDrain0;
     const int dr = wq * 32 + lane;  // TMEM lane: dQ^T row d, later dV row (key)
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t tm_row = tmem_base + lane_off;
     bool ok = true;
-    for (int j = 0; j < n_steps; ++j) {
+    for (int j = 0; j < n_steps && ok; ++j) {
       if (!wait_bounded(bar_dqfull, j & 1, abort_flag, p.status, kStatusTimeoutEpilogue)) {
         ok = false;
         break;
@@ -684,11 +750,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_dqempty);
-      if (dr < D) {
-        // accumulator block: row-major [64 queries][D]; a warp's 32 rows d are 128 contiguous bytes
-        float* dst = p.dq_acc + tile_of(j / nq, jb_lo + j % nq) * (kBM * D) + dr;
+      // row-major [64 queries][D]: a warp's 32 rows d are 128 contiguous bytes
 #pragma unroll
-        for (int q = 0; q < kBM; ++q) atomicAdd(dst + q * D, __uint_as_float(v[q]));
+      for (int h = 0; h < 2; ++h) {
+        if (!wait_bounded(bar_outfree + 8 * h, (j & 1) ^ 1, abort_flag, p.status, kStatusTimeoutEpilogue)) {
+          ok = false;
+          break;
+        }
+        if (dr < D) {
+          const uint32_t to = sb + L::kOut + h * L::kOutHalf + dr * 4;
+#pragma unroll
+          for (int q = 0; q < 32; ++q) st_shared_u32(to + q * (D * 4), v[h * 32 + q]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_outfull + 8 * h);
       }
     }
     // ------------------------------------------------------------ dv = dV
@@ -728,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(tmem_base, kTmemCols);
+  if (warp == W::kMma) tmem_dealloc(tmem_base, kTmemCols);
 }
 
 // ------------------------------------------------------------------ prep: -delta, -lse log2 e, zero dq
@@ -947,7 +1023,7 @@ int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
     if (e != cudaSuccess) return host::cuda_check(e, "cudaFuncSetAttribute(fmha bwd)");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  kern<<<grid, kThreads, Layout<D>::kBytes, s>>>(tq, tk, tv, tdo, p);
+  kern<<<grid, Warps<MODE>::kThreads, Layout<D>::kBytes, s>>>(tq, tk, tv, tdo, p);
   return host::cuda_check(cudaGetLastError(), "fmha bwd kernel launch");
 }
 
