@@ -573,8 +573,15 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
       const float2* nd2 = reinterpret_cast<const float2*>(sgen + L::kRow + st * 512 + 256) + cg * (kC / 2);
       // the stage's -lse / -delta rows were written by the bulk copy: observe its barrier
       // here too (it completed before S^T_j; the stage is refilled only after dS_j)
-      if (!wait_bounded(bar_sfull, ph, abort_flag, p.status, kStatusTimeoutSoftmax) ||
-          !wait_bounded(bar_full + 8 * st, st_ph, abort_flag, p.status, kStatusTimeoutSoftmax)) {
+      if (!wait_bounded(bar_full + 8 * st, st_ph, abort_flag, p.status, kStatusTimeoutSoftmax)) {
+        ok = false;
+        break;
+      }
+      // fetched before the wait for S^T, as the queries' -delta are before that for dP^T
+      float2 nl[kC / 2];
+#pragma unroll
+      for (int c = 0; c < kC / 2; ++c) nl[c] = nl2[c];
+      if (!wait_bounded(bar_sfull, ph, abort_flag, p.status, kStatusTimeoutSoftmax)) {
         ok = false;
         break;
       }
@@ -605,14 +612,14 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
           bool keep = row_valid;
           if (p.causal) keep = keep && (kj <= qi);
           if (p.window > 0) keep = keep && ((kj - qi <= p.window && qi - kj <= p.window) || kj < p.sinks);
-          const float2 nlp = nl2[c >> 1];
+          const float2 nlp = nl[c >> 1];
           pv[c] = keep ? fast_exp2(fmaf(x, kLog2e, (c & 1) ? nlp.y : nlp.x)) : 0.f;
           gsc[c] = g;
         }
       } else {
 #pragma unroll
         for (int c = 0; c < kC; c += 2) {
-          const float2 nlp = nl2[c >> 1];
+          const float2 nlp = nl[c >> 1];
           float a, bb;
           f2unpack(fma2(f2pack(pv[c], pv[c + 1]), k2, f2pack(nlp.x, nlp.y)), a, bb);
           pv[c] = fast_exp2(a);
@@ -644,7 +651,15 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_pfull);
       }
-      // dS^T = P^T (dP^T - delta)
+      // dS^T = P^T (dP^T - delta), its smem tile j & 1 free once dQ^T_{j-2} has read it
+      float2 nd[kC / 2];
+#pragma unroll
+      for (int c = 0; c < kC / 2; ++c) nd[c] = nd2[c];
+      if (j >= 2 &&
+          !wait_bounded(bar_dsfree + 8 * (j & 1), ((j - 2) >> 1) & 1, abort_flag, p.status, kStatusTimeoutSoftmax)) {
+        ok = false;
+        break;
+      }
       if (!wait_bounded(bar_dpfull, ph, abort_flag, p.status, kStatusTimeoutSoftmax)) {
         ok = false;
         break;
@@ -656,7 +671,7 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
       uint32_t pk[kC / 2];
 #pragma unroll
       for (int c = 0; c < kC; c += 2) {
-        const float2 ndp = nd2[c >> 1];
+        const float2 ndp = nd[c >> 1];
         const uint64_t t = add2(f2pack(__uint_as_float(dsu[c]), __uint_as_float(dsu[c + 1])), f2pack(ndp.x, ndp.y));
         float a, bb;
         f2unpack(mul2(f2pack(pv[c], pv[c + 1]), t), a, bb);
@@ -667,13 +682,7 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
         pk[c >> 1] = Cvt<T>::pack(a, bb);
       }
       tmem_stc(tm_row + kTmDP + cg * kC, pk);
-      // dS^T row r into smem tile j & 1 ([128 keys][64 q], 16-byte chunk i at (i ^ (r & 7))),
-      // once dQ^T_{j-2} has finished reading that tile
-      if (j >= 2 &&
-          !wait_bounded(bar_dsfree + 8 * (j & 1), ((j - 2) >> 1) & 1, abort_flag, p.status, kStatusTimeoutSoftmax)) {
-        ok = false;
-        break;
-      }
+      // dS^T row r into its smem tile ([128 keys][64 q], 16-byte chunk i at (i ^ (r & 7)))
       const uint32_t ds_row = sb + L::kDS + (j & 1) * L::kDSBytes + r * 128;
 #pragma unroll
       for (int i = 0; i < kC / 8; ++i) {
