@@ -22,9 +22,9 @@
 // minus one vector per kv head, about their mean: each row of dS sums to zero, so the product is the same, but
 // the roundings of dS and of delta, which do not, no longer meet the keys' common part (keys whose channels have
 // means of 1.5 deviations: relative error of dq 0.0050 to 0.0029 in bf16).
-// 4096 tokens, 32 / 8 heads of 128, window 512, 4 sinks: 173 us, of which the main kernel takes about 140, some 1.4 us
+// 4096 tokens, 32 / 8 heads of 128, window 512, 4 sinks: 170 us, of which the main kernel takes about 137, some 1.4 us
 // for each of a CTA's 40 to 44 steps (the tensor pipe is busy for 45 % of them); the sinks' pieces are 48 of its
-// 296 CTAs. Causal without a window: 466 us.
+// 296 CTAs. Causal without a window: 460 us.
 //
 // The main kernel is laid out around the costs of B200 that its steps meet: shared-memory bandwidth
 // (about 128 B per clock per SM, which limits MMAs that read both operands from shared memory at N <= 64), the
@@ -219,9 +219,13 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
   constexpr uint32_t kIdescKV = make_idesc_f16(kBF16, kBN, D, false, true);    // dV, dK
   constexpr uint32_t kIdescQ = make_idesc_f16(kBF16, 128, kBM, true, true);    // dQ^T
 
+  launch_dependents();
   // ---------------------------------------------------------- block geometry
   const int bh = (int)blockIdx.y + (int)blockIdx.z * (int)gridDim.y;
-  if (bh >= p.zh_kv) return;
+  if (bh >= p.zh_kv) {
+    wait_prerequisites();
+    return;
+  }
   const int hk = bh % p.hkv;
   const int zb = bh / p.hkv;
   // with sinks, grid.x is (sink tile, piece) pairs and then the other key tiles
@@ -244,7 +248,10 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
     row_k0 = 0;
     len_k = p.sk;
   }
-  if (n0 >= len_k) return;  // uniform across the CTA
+  if (n0 >= len_k) {  // uniform across the CTA
+    wait_prerequisites();
+    return;
+  }
   const int zc = VARLEN ? 0 : zb;
   // query range the masks allow for keys [n0, n0 + 128)
   int q_lo = 0, q_hi = len_q;
@@ -285,6 +292,7 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
     dv_base = reinterpret_cast<T*>(p.dv) + (int64_t)zb * p.dv_sz + (int64_t)hk * p.dv_sh;
   }
   if (n_steps == 0) {  // no query sees these keys: dk = dv = 0
+    wait_prerequisites();
     if (MODE != kPlain && part) {
       for (int i = threadIdx.x; i < 2 * kBN * D / 4; i += W::kThreads)
         reinterpret_cast<float4*>(part)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -355,12 +363,13 @@ __global__ void __launch_bounds__(Warps<MODE>::kThreads, 1)
   }
   // kWindow: the centre, in the dQ tile, which is first written when all compute warps have had it
   float* centre_s = reinterpret_cast<float*>(sgen + L::kOut);
-  if constexpr (MODE == kWindow)
-    if (threadIdx.x < D) centre_s[threadIdx.x] = p.centre[(int64_t)bh * D + threadIdx.x];
   if (warp == W::kMma) {
     tmem_alloc(smem_u32(tmem_slot), kTmemCols);
     tmem_relinquish();
   }
+  wait_prerequisites();
+  if constexpr (MODE == kWindow)
+    if (threadIdx.x < D) centre_s[threadIdx.x] = p.centre[(int64_t)bh * D + threadIdx.x];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -827,6 +836,7 @@ __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
 
 template <typename T, int D, bool VARLEN, bool CENTRE>
 __global__ void __launch_bounds__(256) fmha_bwd_prep_kernel(const RowParams p) {
+  launch_dependents();
   const int bh = (int)blockIdx.y + (int)blockIdx.z * (int)gridDim.y;
   if (bh >= p.zh) return;
   const int h = bh % p.hq;
@@ -941,6 +951,7 @@ __device__ __forceinline__ void join_parts(const Params& p, int bh, int x) {
 // p.join blocks of a kv head's first query head join the sinks' parts instead.
 template <typename T, int D, bool VARLEN, bool JOIN>
 __global__ void __launch_bounds__(256) fmha_bwd_dq_kernel(const RowParams p, const Params m) {
+  wait_prerequisites();
   const int bh = (int)blockIdx.y + (int)blockIdx.z * (int)gridDim.y;
   if (bh >= p.zh) return;
   const int h = bh % p.hq;
@@ -1007,6 +1018,25 @@ SinkPlan sink_plan(int64_t zh_kv, int64_t max_q, int64_t max_k, int64_t d, int c
   return s;
 }
 
+// A launch whose blocks, if `early`, may be set up before the kernel ahead of it on the stream has ended. The
+// three kernels follow one another: the first is launched as usual, so that the call's inputs can be read once it
+// runs, and the others wait for the one before (wait_prerequisites) before they touch the workspace or a result.
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kern)(P...), bool early, dim3 grid, int threads, size_t smem, cudaStream_t s,
+                         const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 dim3 grid_of(int x, int64_t yz) {
   const unsigned y = (unsigned)(yz < 65535 ? yz : 65535);
   return dim3((unsigned)x, y, (unsigned)((yz + (int64_t)y - 1) / (int64_t)y));
@@ -1022,7 +1052,7 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int64_t z, int64_t h,
 
 template <typename T, int D, bool VARLEN, int MODE>
 int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
-                const Params& p, dim3 grid, cudaStream_t s) {
+                const Params& p, bool early, dim3 grid, cudaStream_t s) {
   auto kern = fmha_bwd_kernel<T, D, VARLEN, MODE>;
   static bool configured[64] = {false};
   int dev = 0;
@@ -1032,8 +1062,9 @@ int launch_main(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
     if (e != cudaSuccess) return host::cuda_check(e, "cudaFuncSetAttribute(fmha bwd)");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  kern<<<grid, Warps<MODE>::kThreads, Layout<D>::kBytes, s>>>(tq, tk, tv, tdo, p);
-  return host::cuda_check(cudaGetLastError(), "fmha bwd kernel launch");
+  return host::cuda_check(launch_after(kern, early, grid, Warps<MODE>::kThreads, Layout<D>::kBytes, s, tq, tk,
+                                       tv, tdo, p),
+                          "fmha bwd kernel launch");
 }
 
 template <typename T, int D, bool VARLEN>
@@ -1046,22 +1077,28 @@ int run_all(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
     int rc = host::cuda_check(cudaGetLastError(), "fmha bwd prep launch");
     if (rc) return rc;
   }
+  const int64_t key_blocks = kv_tiles + p.sink_tiles * (p.pieces - 1);
+  // early launches: only after the prep kernel, and where the key tiles fit the SMs at once. There launches count
+  // (333 tokens, 2 x 12 heads: 25.3 to 23.6 us); with more tiles than SMs, blocks that start one by one as
+  // the prep kernel's end cost about 1 % (4096 tokens, 8 kv heads: 170 to 171.5 us).
+  const bool early = q_blocks > 0 && key_blocks * p.zh_kv <= host::sm_count();
   if (kv_tiles > 0) {
-    const dim3 g = grid_of(kv_tiles + p.sink_tiles * (p.pieces - 1), p.zh_kv);
-    int rc = mode == kPlain    ? launch_main<T, D, VARLEN, kPlain>(tq, tk, tv, tdo, p, g, s)
-             : mode == kWindow ? launch_main<T, D, VARLEN, kWindow>(tq, tk, tv, tdo, p, g, s)
-                               : launch_main<T, D, VARLEN, kExtra>(tq, tk, tv, tdo, p, g, s);
+    const dim3 g = grid_of((int)key_blocks, p.zh_kv);
+    int rc = mode == kPlain    ? launch_main<T, D, VARLEN, kPlain>(tq, tk, tv, tdo, p, early, g, s)
+             : mode == kWindow ? launch_main<T, D, VARLEN, kWindow>(tq, tk, tv, tdo, p, early, g, s)
+                               : launch_main<T, D, VARLEN, kExtra>(tq, tk, tv, tdo, p, early, g, s);
     if (rc) return rc;
   }
   if (q_blocks > 0) {
     if (p.sink_tiles > 0 && p.pieces > 1) {  // pieces > 1 only where there are queries and key tiles
       RowParams jp = rp;
       jp.join = p.sink_tiles * kJoinBlocks<D>;
-      fmha_bwd_dq_kernel<T, D, VARLEN, true><<<grid_of(q_blocks + jp.join, rp.zh), 256, 0, s>>>(jp, p);
-    } else {
-      fmha_bwd_dq_kernel<T, D, VARLEN, false><<<rgrid, 256, 0, s>>>(rp, p);
+      return host::cuda_check(launch_after(fmha_bwd_dq_kernel<T, D, VARLEN, true>, early,
+                                           grid_of(q_blocks + jp.join, rp.zh), 256, 0, s, jp, p),
+                              "fmha bwd dq launch");
     }
-    return host::cuda_check(cudaGetLastError(), "fmha bwd dq launch");
+    return host::cuda_check(launch_after(fmha_bwd_dq_kernel<T, D, VARLEN, false>, early, rgrid, 256, 0, s, rp, p),
+                            "fmha bwd dq launch");
   }
   return GKO_OK;
 }

@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, NT > 1 ? 2 : BITS == 4 ? 4 : 3) fmha
     }
   }
 
-  asm volatile("griddepcontrol.launch_dependents;");  // the join kernel may be set up from here on
+  launch_dependents();  // the join kernel may be set up from here on
   // join the warps: sums over the lanes of a column, a common maximum, then warp after warp
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -935,7 +935,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fmha_cache_join_kernel(const 
   const int tok = col / p.group, head = hk * p.group + col % p.group;
   const int64_t r = (int64_t)(sq.row0 + tok) * p.hq + head;
   const int64_t first = (w.part0 + tile) * p.cols + col - c0, stride = (int64_t)w.stride * p.cols;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // all parts are written from here on
+  wait_prerequisites();  // all parts are written from here on
   float mx = kNoMax;
   for (int s = lane; s < used; s += 32) mx = fmaxf(mx, p.part_ml[first + s * stride].x);
 #pragma unroll

@@ -254,6 +254,11 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 
+// Programmatic launches: from here on the next kernel of the stream may be set up; and, in that kernel, all that
+// the kernel before it wrote can be read from here on.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // True on one lane of a converged warp. Branching on it, unlike on lane == 0, tells the compiler that a single
 // thread goes on, so it need not guard each MMA or copy, whose operands are uniform, against other lanes.
 __device__ __forceinline__ bool elect_one() {
