@@ -7,7 +7,8 @@ Tolerances, from the arithmetic (u = half a step of a type: f16 2^-11, bf16 2^-8
 * attention: a logit is an f32 sum of d exact products, two f32 multiply-adds and a product, off by at
   most (d + 8) u32 times the sum of the products' magnitudes (``mag``), and its exponential by 2^-21 more.
   Each probability times scale_v is rounded to f16 (u16, or 2^-25 of twice the largest scale_v when it
-  underflows), so the code part of the output is off by u16 of itself; the output is rounded once.
+  underflows) and meets the code less the middle one, so the output is off by u16 of the sum of
+  p scale |code - middle|; it is rounded once itself.
 """
 
 import pytest
@@ -193,7 +194,8 @@ def _check_attention(got, q, cache, table, lens, news, bits, causal, window, sof
         qa = qs.double().abs().sum(-1).amax().item()
         mag = abs(scale) * qa * ((2 ** bits - 1) * pair[0][..., 0].amax() + pair[0][..., 1].abs().amax()).item()
         logit = (d + 8) * 2.0 ** -24 * mag + 2.0 ** -21
-        codes = (v - pair[1][..., 1:]).repeat_interleave(group, 1)
+        # a code enters less the middle one: a rounding of p scale is off by 2^-11 of p scale |code - middle|
+        codes = (v - pair[1][..., 1:] - pair[1][..., :1] * 2 ** (bits - 1)).abs().repeat_interleave(group, 1)
         part = torch.einsum("hij,jhd->ihd", p, codes)
         under = n * 2.0 ** -25 * 2 * pair[1][..., 0].amax().item() * (2 ** bits - 1)
         tol = want.abs() * HALF[dtype] + part * 2.0 ** -11 + under + 2 * logit * v.abs().amax().item()
