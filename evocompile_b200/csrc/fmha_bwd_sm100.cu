@@ -36,7 +36,7 @@
 // memory, [queries][D] in f32, whose halves the copy engine adds to the accumulator in L2 (64 reductions
 // of each drain thread instead filled the queue in which the compute warps' loads and stores wait:
 // 183 us against 173). One elected thread issues the MMAs; were it chosen as lane 0, each issue would cost
-// some 80 cycles, and a step's 36 of them more than anything else in it (606 us against 528, causal).
+// some 80 cycles, and a step's 36 of them more than anything else in it (606 us against 528, causal, 4096 tokens, 32 / 8 heads).
 // TMEM columns: K [0, 64)  dQ^T [64, 128)  dV [128, 256)  dK [256, 384)
 //               S^T|P^T [384, 448)  dP^T|dS^T [448, 512)
 // Warps, with 16 (kPlain, kWindow) or 8 (kExtra, whose mask and softcap need the registers) for compute:

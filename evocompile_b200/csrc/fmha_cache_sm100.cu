@@ -1124,7 +1124,8 @@ extern "C" int gko_fmha_cache_fwd(int dtype, int bits, int64_t b, int64_t hq, in
   if (pages < 0 || table_width < 0 || table_stride < 0) return fail(GKO_ERR_INVALID, "fmha over a cache: bad sizes");
   if (table_width * page_size >= (1ll << 31) || pages >= (1ll << 31) ||
       (pages > 0 && hkv > 0 && page_size > 0 && pages * hkv >= 0xffffffffll / page_size))
-    return fail(GKO_ERR_UNSUPPORTED, "fmha over a cache: a sequence may hold fewer than 2^31 tokens, the cache fewer than 2^32 rows");
+    return fail(GKO_ERR_UNSUPPORTED,
+                "fmha over a cache: a sequence may hold fewer than 2^31 tokens, the cache fewer than 2^32 rows");
   if (b == 0 || tq == 0 || max_seqlen_q == 0) return GKO_OK;
   if (!q || !k_codes || !v_codes || !k_pairs || !v_pairs || (!table && table_width > 0) || !seq_lens || !out || !lse)
     return fail(GKO_ERR_INVALID, "fmha over a cache: null pointer argument");

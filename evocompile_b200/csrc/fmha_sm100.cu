@@ -1,8 +1,9 @@
 // Fused multi-head attention forward for sm_100a (gko::fused_sdpa_pair,
 // gko::cutlass_fmha_pair, gko::fmha_varlen_fwd).
 //
-// One CTA computes a 256-row query block (two 128-row tiles Q0, Q1) of one
-// (batch, head) against the key range the masks allow, in 128-key tiles:
+// One CTA computes a 256-row query block (two 128-row tiles Q0, Q1; with a window and sinks
+// one tile, see Shape) of one (batch, head) against the key range the masks allow, in
+// 128-key tiles:
 //   warp 8     TMA producer: Q0/Q1 once, then K_j / V_j into a 2-stage ring
 //   warp 9     MMA issuer + TMEM owner. Per key tile j and query tile t it issues
 //              S_t = Q_t K_j^T into TMEM, then (once softmax has written P_t)
@@ -44,9 +45,9 @@ constexpr int kMaxWindow = (1 << 30) - 1024;  // wider ones hide nothing; positi
 // see. Up to 32 sinks, ahead of the window, cost a quarter of a key tile: S has 32 columns, P V two steps.
 // Bound by the chain S -> softmax -> P -> P V of each key tile, as kPlain is (its rate on dense causal
 // attention, 0.9 PFLOP/s, is what the tiles here run at too); the window leaves 9 to 10 tiles per block.
-// 4096 tokens, 64 / 8 heads of 128, window 1024, 4 sinks: 175 us, 0.69 PFLOP/s of visible pairs (196 us with a
-// whole tile for the sinks, one mask for every edge and two query tiles per CTA); kExtra takes some ten times as
-// long.
+// 4096 tokens, 64 / 8 heads of 128, window 1024, 4 sinks: 165 us, 0.73 PFLOP/s of visible pairs (175 before the
+// issuers were chosen by elect.sync; 196 with a whole tile for the sinks, one mask for every edge and two query
+// tiles per CTA); kExtra takes some ten times as long.
 enum : int { kPlain = 0, kExtra = 1, kWindow = 2 };
 
 // A CTA takes two query tiles, whose softmax and products hide one another, and has an SM to itself (K and V
