@@ -58,6 +58,7 @@ def _attend(lib, dtype=_lib.BF16, bits=4, b=2, hq=4, hkv=2, d=64, tq=2, max_q=1,
     (_attend, dict(scale=float("nan")), _lib.ERR_INVALID, "scale"),
     (_attend, dict(page=8), _lib.ERR_UNSUPPORTED, "multiple of 16"),
     (_attend, dict(width=1 << 27), _lib.ERR_UNSUPPORTED, "2^31"),
+    (_attend, dict(hq=1024, hkv=1024, page=1 << 20), _lib.ERR_UNSUPPORTED, "2^32 rows"),
     (_attend, dict(b=70000, tq=70000), _lib.ERR_UNSUPPORTED, "out of range"),
     (_attend, dict(q=0), _lib.ERR_INVALID, "null"),
     (_attend, dict(out=(1 << 20) + 4), _lib.ERR_UNSUPPORTED, "16-byte"),

@@ -249,6 +249,38 @@ def test_captured_backward():
     assert torch.equal(out, o) and torch.equal(grads[1], direct[1]) and torch.equal(grads[2], direct[2])
 
 
+@pytest.mark.parametrize("s", [70, 700])
+def test_calls_in_a_row(s):
+    """Steps on changing inputs with nothing waited for in between, their kernels set up early after one another
+    (few key tiles) or not: dk and dv are those of the same step by itself, to the bit."""
+    hq, hkv = (4, 2) if s < 100 else (64, 32)
+    sets = [[_dev(t) for t in _qkv(40 + i, 1, hq, hkv, s, s, 64, torch.bfloat16)] for i in range(2)]
+
+    def step(q, k, v, dout):
+        o, lse = ops.fmha_fwd(q, k, v, None, 0.125, 1, 40, sinks=4)
+        return o, *ops.fmha_bwd(q, k, v, None, o, lse, dout, 0.125, 1, 40, 0.0, 4)
+
+    alone = []
+    for x in sets:
+        alone.append(step(*x))
+        torch.cuda.synchronize()
+    now = [torch.empty_like(t) for t in sets[0]]
+    rows = []
+    for i in range(12):
+        for t, n in zip(now, sets[i & 1]):
+            t.copy_(n)
+        rows.append(step(*now))
+    torch.cuda.synchronize()
+    _status_clear()
+    for i, (o, dq, dk, dv) in enumerate(rows):
+        want = alone[i & 1]
+        assert torch.equal(o, want[0]) and torch.equal(dk, want[2]) and torch.equal(dv, want[3])
+        # dq is a sum of the key tiles' shares in f32 in any order, rounded once: at most a step apart, or 2^-20 of
+        # the shares where they cancel
+        room = want[1].float().abs() * 2.0 ** -7 + 2.0 ** -20 * want[1].float().abs().max()
+        assert ((dq.float() - want[1].float()).abs() <= room).all()
+
+
 def test_new_host_thread():
     """The first CUDA call of a host thread may be one of these (autograd's thread when nothing is copied)."""
     import threading
