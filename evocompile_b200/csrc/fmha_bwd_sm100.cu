@@ -23,7 +23,7 @@
 // the roundings of dS and of delta, which do not, no longer meet the keys' common part (keys whose channels have
 // means of 1.5 deviations: relative error of dq 0.0050 to 0.0029 in bf16).
 // 4096 tokens, 32 / 8 heads of 128, window 512, 4 sinks: 170 us, of which the main kernel takes about 137, some 1.4 us
-// for each of a CTA's 40 to 44 steps (the tensor pipe is busy for 45 % of them); the sinks' pieces are 48 of its
+// for each of a CTA's 40 to 44 steps (the tensor pipe is busy for 53 % of them); the sinks' pieces are 48 of its
 // 296 CTAs. Causal without a window: 460 us.
 //
 // The main kernel is laid out around the costs of B200 that its steps meet: shared-memory bandwidth
@@ -36,7 +36,8 @@
 // memory, [queries][D] in f32, whose halves the copy engine adds to the accumulator in L2 (64 reductions
 // of each drain thread instead filled the queue in which the compute warps' loads and stores wait:
 // 183 us against 173). One elected thread issues the MMAs; were it chosen as lane 0, each issue would cost
-// some 80 cycles, and a step's 36 of them more than anything else in it (606 us against 528, causal, 4096 tokens, 32 / 8 heads).
+// some 80 cycles, and a step's 36 of them more
+// than anything else in it (606 us against 528, causal, 4096 tokens, 32 / 8 heads).
 // TMEM columns: K [0, 64)  dQ^T [64, 128)  dV [128, 256)  dK [256, 384)
 //               S^T|P^T [384, 448)  dP^T|dS^T [448, 512)
 // Warps, with 16 (kPlain, kWindow) or 8 (kExtra, whose mask and softcap need the registers) for compute:
