@@ -641,7 +641,8 @@ def fmha_cache_fwd(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqle
     causal keeps keys up to that position, window > 0 those within it, plus the first ``sinks`` keys.
     ``max_seqlen_k`` (default: what the block table holds) sets how the work is split, not what is
     read. Rows that see no key give zeros and -inf; rows of no sequence are not written (``out`` keeps
-    what it had). One call per cache step: repeated calls give the same bits.
+    what it had). One call per cache step: repeated calls give the same bits. A cache of 2^32 rows (tokens times kv
+    heads) or more is refused.
     """
     kc, vc, kp, vp = cache
     return _lib.binding().fmha_cache_fwd(q, kc, vc, kp, vp, block_table, seq_lens, cu_seqlens_q, max_seqlen_q,

@@ -375,7 +375,7 @@ int gko_kv_cache_read(int dtype, int bits, int64_t b, int64_t hkv, int64_t d, in
  * longer sequence is still answered in full. out [tq, hq, d] contiguous, lse f32 [hq, tq]; a row that
  * sees no key gives zeros and -inf; rows of no sequence are left as they were. A page outside
  * [0, pages) counts as masked and sets GKO_STATUS_BAD_INDEX, as does a length past the table, which
- * is cut to it. The result does not vary from run to run. workspace: 16-byte aligned device memory of
+ * is cut to it. pages * hkv * page_size stays below 2^32. The result does not vary from run to run. workspace: 16-byte aligned device memory of
  * gko_fmha_cache_workspace_size bytes (may be 0; -1: sizes out of range), overwritten by the call.
  */
 int64_t gko_fmha_cache_workspace_size(int bits, int64_t b, int64_t hq, int64_t hkv, int64_t d, int64_t tq,
